@@ -43,6 +43,15 @@ class FlushSrc(C.Structure):
                 ("residual_b_stride", C.c_int64), ("residual_h_stride", C.c_int64)]
 
 
+class Prompt(C.Structure):
+    _fields_ = [("dtype", C.c_int32), ("D", C.c_int32), ("nh_q", C.c_int32), ("nh_kv", C.c_int32), ("n_seqs", C.c_int32),
+                ("causal", C.c_int32), ("scale", C.c_float), ("total_q", C.c_int64), ("total_k", C.c_int64), ("prefix_len", C.c_int64),
+                ("q", C.c_void_p), ("k", C.c_void_p), ("v", C.c_void_p), ("prefix_k", C.c_void_p), ("prefix_v", C.c_void_p),
+                ("q_token", C.c_int64), ("q_head", C.c_int64), ("k_token", C.c_int64), ("k_head", C.c_int64),
+                ("v_token", C.c_int64), ("v_head", C.c_int64), ("prefix_k_token", C.c_int64), ("prefix_k_head", C.c_int64),
+                ("prefix_v_token", C.c_int64), ("prefix_v_head", C.c_int64), ("q_starts", C.c_void_p), ("k_starts", C.c_void_p)]
+
+
 _SIGNATURES = {
     "hqkv_last_error": (C.c_char_p, []),
     "hqkv_version": (C.c_int, []),
@@ -112,6 +121,13 @@ _SIGNATURES = {
     "hqkv_flush_evict": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int64, C.c_void_p, C.c_void_p, C.c_int64, C.c_int, C.c_void_p]),
     "hqkv_gather_columns_f16": (C.c_int, [C.c_void_p, C.c_int64, C.c_int, C.c_void_p, C.c_int64, C.c_void_p,
                                           C.c_int64, C.c_void_p]),
+    "hqkv_prompt_workspace_bytes": (C.c_size_t, [C.POINTER(Prompt)]),
+    "hqkv_prompt_attention": (C.c_int, [C.POINTER(Prompt), C.c_void_p, C.c_void_p, C.c_void_p, C.c_size_t, C.c_void_p]),
+    "hqkv_prompt_importance": (C.c_int, [C.POINTER(Prompt), C.c_void_p, C.c_int, C.c_void_p, C.c_void_p]),
+    "hqkv_decode_prefix_workspace_bytes": (C.c_size_t, [C.POINTER(CacheDesc), C.c_int64]),
+    "hqkv_decode_attention_prefix": (C.c_int, [C.POINTER(CacheDesc), C.c_void_p, C.c_void_p, C.c_void_p, C.c_int64, C.c_int64,
+                                               C.c_int64, C.c_int64, C.c_int64, C.c_void_p, C.c_void_p, C.c_void_p, C.c_size_t,
+                                               C.c_void_p, C.c_size_t, C.c_void_p]),
 }
 
 EXPORTED_SYMBOLS = tuple(_SIGNATURES)

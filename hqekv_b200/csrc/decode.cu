@@ -26,6 +26,7 @@
 #include <string.h>
 
 #include "common.cuh"
+#include "prompt.cuh"
 
 namespace hqkv {
 
@@ -90,6 +91,7 @@ struct DecodeParams {
   unsigned* peer_state;  // call number, status, finished (batch, kv head) count
   long long max_spins;
   unsigned* counters;  // [B][virtual kv head]
+  float* out32;        // [B][nh_q][D] the outputs before they are rounded to fp16, for a caller that goes on with them (null: not wanted)
 };
 
 // The tokens of a (batch, virtual kv head) plane are a list of UNITS, tiers in order, and its CTAs take consecutive shares of
@@ -1693,7 +1695,9 @@ __device__ __forceinline__ void v_finish(const DecodeParams& P, const VShared<NW
     const unsigned odd = static_cast<unsigned>(a[k] >> 62);
     double sum = (v_part(a[k]) + v_part(b[k]) * (1. / (1ull << V_LOW_BITS))) * P.v_unit;
     if (odd) sum = odd == 1u ? INFINITY : odd == 2u ? -INFINITY : __int_as_float(0x7FC00000);
-    P.out[out0 + h * D + c] = __float2half_rn(static_cast<float>(sum) * sh.ginv[h]);
+    const float o = static_cast<float>(sum) * sh.ginv[h];
+    P.out[out0 + h * D + c] = __float2half_rn(o);
+    if (P.out32) P.out32[out0 + h * D + c] = o;
     high[h * D] = low[h * D] = 0ull;   // (nobody else comes: a V pass without a K pass before it starts from zero, too)
   }
 }
@@ -1964,9 +1968,11 @@ __global__ void __launch_bounds__(NW * 32, V_SM_WARPS / NW) v_pass_kernel(const 
       const double2 v = __ldcg(reinterpret_cast<const double2*>(accum + i));
       *reinterpret_cast<double2*>(accum + i) = make_double2(0., 0.);   // (as in v_finish)
       const float inv = MODE == V_GIVEN ? 1.f : sh.ginv[i >> 7];
-      const __half2 o = __floats2half2_rn(static_cast<float>(v.x) * inv, static_cast<float>(v.y) * inv);
+      const float2 f = make_float2(static_cast<float>(v.x) * inv, static_cast<float>(v.y) * inv);
+      const __half2 o = __floats2half2_rn(f.x, f.y);
       const int64_t at = (static_cast<int64_t>(w.b) * P.nh_q + w.h0) * D + i;
       *reinterpret_cast<__half2*>(P.out + at) = o;
+      if (P.out32) *reinterpret_cast<float2*>(P.out32 + at) = f;
       // kv-head sharding: the same rows go straight into every peer's copy of the gathered output
       // (plain stores over NVLink; the callers' cross-GPU barrier makes them visible before use)
       if (P.peer_flagged) {
@@ -2257,7 +2263,7 @@ struct PeerArgs {
 static int decode_launch(const hqkv_cache_desc_t* cache_host, const void* q, void* attn_weights, void* attn_output,
                          void* workspace, size_t workspace_bytes, int phases, const PeerArgs& peers, void* stream,
                          const void* probs_in = nullptr, const void* mask = nullptr, long long mask_bstride = 0,
-                         long long mask_hstride = 0, void* head_sum = nullptr);
+                         long long mask_hstride = 0, void* head_sum = nullptr, float* out32 = nullptr);
 // the V pass emits the importance row itself up to these sizes (a CTA reads B*nh_q probabilities per token)
 constexpr int HEAD_SUM_MAX_ROWS = 64;
 constexpr int HEAD_SUM_MAX_CHUNKS = (HQKV_WS_HEADER_BYTES - 4096) / 4;
@@ -2307,7 +2313,7 @@ static constexpr const PassKernel* v_kernels[3][2][2] = {  // [VMode][8, 4 warps
 static int hqkv::decode_launch(const hqkv_cache_desc_t* cache_host, const void* q, void* attn_weights, void* attn_output,
                                void* workspace, size_t workspace_bytes, int phases, const PeerArgs& peers, void* stream,
                                const void* probs_in, const void* mask, long long mask_bstride, long long mask_hstride,
-                               void* head_sum) {
+                               void* head_sum, float* out32) {
   HQKV_REQUIRE(phases >= 1 && phases <= 3, "decode: phases must be 1 (K pass), 2 (V pass) or 3 (both)");
   DecodeParams P;
   Layout lay;
@@ -2345,6 +2351,7 @@ static int hqkv::decode_launch(const hqkv_cache_desc_t* cache_host, const void* 
   P.counters = reinterpret_cast<unsigned*>(ws);
   P.hs_count = reinterpret_cast<unsigned*>(ws + 4096);
   P.head_sum = static_cast<__half*>(head_sum);
+  P.out32 = out32;
   P.logits = reinterpret_cast<float*>(ws + lay.logits_off);
   P.k_part = reinterpret_cast<float2*>(ws + lay.kpart_off);
   P.v_acc = reinterpret_cast<double*>(ws + lay.acc_off);
@@ -2436,6 +2443,136 @@ extern "C" int hqkv_decode_attention_headsum(const hqkv_cache_desc_t* cache_host
   if (rc || fused) return rc;
   // larger batches: one more launch over the probabilities just written
   return hqkv_head_sum(attn_weights, P.B, P.nh_q, P.L, P.L, head_sum_row, stream);
+}
+
+// ------------------------------------------------------------------------------------------------
+// A batch that shares a dense prefix: the prefix once for all of it (prompt.cu), each cache as ever, and both joined
+// ------------------------------------------------------------------------------------------------
+namespace hqkv {
+struct JoinParams {
+  const float2* k_part;    // the cache's softmax pairs, logits and unrounded outputs, as the two passes leave them
+  const float* logits;
+  const float* own;
+  const float* part_o;     // [splits][B * nh_q][D], [splits][B * nh_q]
+  const float2* part_ml;
+  __half *out, *weights;
+  int nk_ctas, r4, L, rows, splits;
+};
+constexpr int JOIN_THREADS = 128, JOIN_TOKENS = 2048;   // tokens whose weights a CTA writes
+static_assert(JOIN_THREADS == D, "a thread per channel");
+
+// CTA: a (sequence, query head) and a share of its own tokens.  With M the largest of all logits (base 2) the parts' outputs are
+// scaled by 2^(m - M), the cache's by its own sum, and the sum of all of them divides.  The weights are formed from the
+// fp32 logits again: scaling the fp16 probabilities that the V pass has written would round them twice.
+__global__ void __launch_bounds__(JOIN_THREADS) join_prefix_kernel(const __grid_constant__ JoinParams P) {
+  const int row = blockIdx.x, tid = threadIdx.x, plane = row / P.r4, head = row - plane * P.r4;
+  __shared__ float2 warp_ml[JOIN_THREADS / 32];
+  // (maximum, sum) of the cache, in base 2
+  float m = -INFINITY, l = 0.f;
+  const float2* pairs = P.k_part + static_cast<int64_t>(row) * P.nk_ctas;
+  auto add = [&](float m2, float l2) {
+    const float mx = fmaxf(m, m2), ref = mx == -INFINITY ? 0.f : mx;
+    l = l * fast_exp2(m - ref) + l2 * fast_exp2(m2 - ref);
+    m = mx;
+  };
+  for (int c = tid; c < P.nk_ctas; c += JOIN_THREADS) add(pairs[c].x * LOG2E, pairs[c].y);
+#pragma unroll
+  for (int k = 1; k < 32; k <<= 1) add(__shfl_xor_sync(0xffffffffu, m, k), __shfl_xor_sync(0xffffffffu, l, k));
+  if ((tid & 31) == 0) warp_ml[tid >> 5] = make_float2(m, l);
+  __syncthreads();
+  m = -INFINITY, l = 0.f;
+  for (int w = 0; w < JOIN_THREADS / 32; ++w) add(warp_ml[w].x, warp_ml[w].y);
+  const float own_m = m, own_l = l;
+  for (int s = 0; s < P.splits; ++s) {
+    const float2 part = P.part_ml[static_cast<int64_t>(s) * P.rows + row];
+    add(part.x, part.y);
+  }
+  const float ref = m == -INFINITY ? 0.f : m, inv = 1.f / l;
+  if (blockIdx.y == 0) {
+    const int64_t at = static_cast<int64_t>(row) * D + tid;
+    float o = own_l * fast_exp2(own_m - ref) * P.own[at];
+    for (int s = 0; s < P.splits; ++s) {
+      const int64_t r = static_cast<int64_t>(s) * P.rows + row;
+      const float2 part = P.part_ml[r];
+      if (part.y != 0.f) o += fast_exp2(part.x - ref) * P.part_o[r * D + tid];   // (a split without tokens has no output)
+    }
+    P.out[at] = __float2half_rn(o * inv);
+  }
+  const float* logits = P.logits + static_cast<int64_t>(plane) * P.r4 * P.L;
+  __half* weights = P.weights + static_cast<int64_t>(row) * P.L;
+  const int end = min(P.L, (static_cast<int>(blockIdx.y) + 1) * JOIN_TOKENS);
+  for (int t = blockIdx.y * JOIN_TOKENS + tid; t < end; t += JOIN_THREADS)
+    weights[t] = __float2half_rn(fast_exp2(fmaf(logits[logit_at(t, head, P.r4, P.L)], LOG2E, -ref)) * inv);
+}
+
+// the prefix's side of such a call
+static hqkv_prompt_t prefix_of(const hqkv_cache_desc_t* c, int64_t prefix_len) {
+  hqkv_prompt_t p = {};
+  p.dtype = HQKV_F16;
+  p.D = c->D;
+  p.nh_q = c->nh_q;
+  p.nh_kv = c->H;
+  p.scale = c->softmax_scale;
+  p.total_q = c->B;
+  p.q_token = static_cast<int64_t>(c->nh_q) * D;
+  p.q_head = D;
+  p.prefix_len = prefix_len;
+  return p;
+}
+static size_t join_bytes(const hqkv_cache_desc_t* c, int splits, size_t* part_o, size_t* part_ml) {
+  const size_t rows = static_cast<size_t>(c->B) * c->nh_q;
+  *part_o = rows * D * sizeof(float);   // (behind the cache's outputs)
+  *part_ml = *part_o + splits * rows * D * sizeof(float);
+  return *part_ml + splits * rows * sizeof(float2);
+}
+}  // namespace hqkv
+
+extern "C" size_t hqkv_decode_prefix_workspace_bytes(const hqkv_cache_desc_t* cache_host, int64_t prefix_len) {
+  DecodeParams P;
+  Layout lay;
+  if (build_params(cache_host, P, lay) != HQKV_OK || prefix_len < 1 || prefix_len >= (1ll << 30)) return 0;
+  const hqkv_prompt_t p = prefix_of(cache_host, prefix_len);
+  size_t o, ml;
+  return join_bytes(cache_host, prefix_splits(&p), &o, &ml);
+}
+
+extern "C" int hqkv_decode_attention_prefix(const hqkv_cache_desc_t* cache_host, const void* q, const void* prefix_k, const void* prefix_v,
+                                            int64_t prefix_len, int64_t k_token, int64_t k_head, int64_t v_token, int64_t v_head,
+                                            void* attn_weights, void* attn_output, void* workspace, size_t workspace_bytes,
+                                            void* prefix_workspace, size_t prefix_workspace_bytes, void* stream) {
+  DecodeParams P;
+  Layout lay;
+  if (int rc = build_params(cache_host, P, lay)) return rc;
+  HQKV_REQUIRE(prefix_len >= 1 && prefix_len < (1ll << 30), "decode_prefix: the prefix must hold 1 to 2^30 - 1 tokens");
+  HQKV_REQUIRE(workspace && q && aligned(q, 16) && attn_output && attn_weights, "decode_prefix: null pointer, or q is not 16-byte aligned");
+  HQKV_REQUIRE(prefix_workspace && aligned(prefix_workspace, 256), "decode_prefix: the prefix workspace is null or not 256-byte aligned");
+  hqkv_prompt_t p = prefix_of(cache_host, prefix_len);
+  p.q = q, p.prefix_k = prefix_k, p.prefix_v = prefix_v;
+  p.prefix_k_token = k_token, p.prefix_k_head = k_head, p.prefix_v_token = v_token, p.prefix_v_head = v_head;
+  JoinParams J = {};
+  J.splits = prefix_splits(&p);
+  size_t o, ml;
+  const size_t need = join_bytes(cache_host, J.splits, &o, &ml);
+  if (prefix_workspace_bytes < need)
+    return fail(HQKV_E_WORKSPACE, "decode_prefix: the prefix workspace holds %zu bytes, %zu needed", prefix_workspace_bytes, need);
+  unsigned char* pw = static_cast<unsigned char*>(prefix_workspace);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (int rc = prefix_partial(&p, reinterpret_cast<float*>(pw + o), reinterpret_cast<float2*>(pw + ml), J.splits, st)) return rc;
+  if (int rc = decode_launch(cache_host, q, attn_weights, attn_output, workspace, workspace_bytes, 3, hqkv::PeerArgs(), stream, nullptr, nullptr, 0, 0,
+                             nullptr, reinterpret_cast<float*>(pw)))
+    return rc;
+  const unsigned char* ws = static_cast<const unsigned char*>(workspace);
+  J.k_part = reinterpret_cast<const float2*>(ws + lay.kpart_off);
+  J.logits = reinterpret_cast<const float*>(ws + lay.logits_off);
+  J.own = reinterpret_cast<const float*>(pw);
+  J.part_o = reinterpret_cast<const float*>(pw + o);
+  J.part_ml = reinterpret_cast<const float2*>(pw + ml);
+  J.out = static_cast<__half*>(attn_output);
+  J.weights = static_cast<__half*>(attn_weights);
+  J.nk_ctas = P.nk_ctas, J.r4 = P.r4, J.L = P.L, J.rows = P.B * P.nh_q;
+  join_prefix_kernel<<<dim3(J.rows, static_cast<unsigned>(ceil_div(P.L, JOIN_TOKENS))), JOIN_THREADS, 0, st>>>(J);
+  HQKV_LAUNCH_CHECK("join_prefix");
+  return HQKV_OK;
 }
 
 // ------------------------------------------------------------------------------------------------

@@ -1,0 +1,27 @@
+// What prompt.cu offers to decode.cu, and the arguments of its kernels.
+#pragma once
+
+#include <cuda_bf16.h>
+
+#include "common.cuh"
+
+namespace hqkv {
+
+struct PromptArgs {
+  const void *q, *k, *v, *pk, *pv;                  // element (token, head, channel) at token * stride + head * stride + channel
+  int64_t q_token, q_head, k_token, k_head, v_token, v_head, pk_token, pk_head, pv_token, pv_head;
+  const int *q_starts, *k_starts;                   // [n_seqs + 1]
+  int n_seqs, total_q, total_k, prefix_len, nh_q, nh_kv;
+  bool causal, bf16;
+  float scale_log2;                                 // scale * log2(e)
+  void* out;                                        // [total_q][nh_q][128]
+  float* lse;                                       // [nh_q][total_q]
+  float* part_o;                                    // [splits][total_q * nh_q][128], not yet normalised (null: out and lse)
+  float2* part_ml;                                  // [splits][total_q * nh_q] (maximum, sum), in powers of two
+};
+
+// Attention of p's queries (a token each, no sequences) to its prefix alone: splits parts per row, to be joined.
+int prefix_splits(const hqkv_prompt_t* p);
+int prefix_partial(const hqkv_prompt_t* p, float* part_o, float2* part_ml, int splits, cudaStream_t st);
+
+}  // namespace hqkv

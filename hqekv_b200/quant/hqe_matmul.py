@@ -75,6 +75,57 @@ def _launch(desc, q, attn_weights, attn_output, dev, head_sum_out=None):
         _raise_from_status(rc)
 
 
+def qkv_matmul_hqe_prefix(q: torch.Tensor, past_key_value: Tuple, prefix: Tuple[torch.Tensor, torch.Tensor], head_dim: int,
+                          quant_strategy: str, block_size: int = 32, group_size: int = 32):
+    """One decode step of a batch whose sequences share a prefix: ``qkv_matmul_hqe_2`` over [prefix | own cache], where the dense
+    prefix is read once for the whole batch and ``past_key_value`` holds what is each sequence's own.
+
+    ``prefix`` = (k, v), float16 [P, nh_kv, 128] with P >= 1 and any strides with adjacent channels (rotated like the cache's keys; what a
+    prefill of the prefix leaves in slots 39 and 40, ``k[0].transpose(0, 1)``).  The other arguments, the errors and the results are
+    those of ``qkv_matmul_hqe_2``: (attn_weights [B, nh_q, 1, L] of the cache's own tokens, which add up to 1 minus the prefix's share
+    per head; attn_output [B, nh_q, 1, 128]).  Probabilities are rounded to fp16 before the product with V, the parts are joined in fp32.  No
+    counterpart in the reference."""
+    if quant_strategy not in UNIFORM_STRATEGIES:
+        raise ValueError("invalid quant_strategy")
+    if len(past_key_value) != 42:
+        raise ValueError("invalid past_key_value")
+    low_codec = CODEC_UNIFORM if quant_strategy == "uniform_group" else CODEC_NORMAL
+    pk, pv = prefix
+    if q.dtype != torch.float16 or q.dim() != 4 or q.shape[2] != 1:
+        raise ValueError("q must be float16 of shape [B, nh_q, 1, head_dim]")
+    if torch.is_grad_enabled() and (q.requires_grad or pk.requires_grad or pv.requires_grad):
+        raise RuntimeError("the decode has no backward pass: call it under torch.no_grad()")
+    desc, keep, L, dev = cached_cache_desc(past_key_value, q.shape[1], block_size, group_size, low_codec)
+    if dev != q.device or q.shape[0] != desc.B or q.shape[3] != desc.D:
+        raise ValueError("q does not match the cache (device, batch or head_dim)")
+    for x in (pk, pv):
+        if x.dtype != torch.float16 or x.device != dev or x.dim() != 3 or tuple(x.shape[1:]) != (desc.H, desc.D):
+            raise ValueError("the prefix must be float16 [P, nh_kv, head_dim] on the cache's device")
+    if pk.shape[0] != pv.shape[0] or pk.shape[0] == 0:
+        raise ValueError("the prefix's k and v must hold the same number of tokens, at least one")
+    require_cuda(q, pk, pv)
+    pk, pv = (x if x.stride(2) == 1 and x.data_ptr() % 16 == 0 and x.stride(0) % 8 == 0 and x.stride(1) % 8 == 0
+              else x.clone(memory_format=torch.contiguous_format) for x in (pk, pv))
+    q = q.contiguous()
+    if q.data_ptr() % 16:
+        q = q.clone()
+    B, nh_q, D = q.shape[0], q.shape[1], q.shape[3]
+    attn_weights = torch.empty(B, nh_q, 1, L, dtype=torch.float16, device=dev)
+    attn_output = torch.empty(B, nh_q, 1, D, dtype=torch.float16, device=dev)
+    with torch.cuda.device(dev):
+        need, more = lib.hqkv_decode_workspace_bytes(desc), lib.hqkv_decode_prefix_workspace_bytes(desc, pk.shape[0])
+        if need == 0:
+            _raise_from_status(lib.hqkv_decode_attention(desc, ptr(q), ptr(attn_weights), ptr(attn_output), None, 0, None))
+        st = stream_ptr(dev)
+        ws = decode_workspace(dev, need, st)
+        parts = torch.empty(more, dtype=torch.uint8, device=dev)
+        rc = lib.hqkv_decode_attention_prefix(desc, ptr(q), ptr(pk), ptr(pv), pk.shape[0], pk.stride(0), pk.stride(1), pv.stride(0),
+                                              pv.stride(1), ptr(attn_weights), ptr(attn_output), ptr(ws), ws.numel(), ptr(parts), more, st)
+    if rc:
+        _raise_from_status(rc)
+    return attn_weights, attn_output
+
+
 def _raise_from_status(rc):
     if rc == -2:
         raise NotImplementedError(lib.hqkv_last_error().decode())

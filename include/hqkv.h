@@ -492,6 +492,65 @@ int hqkv_flush_evict(const hqkv_flush_t* flush_host, const void* workspace, int6
 int hqkv_gather_columns_f16(const void* in, int64_t in_stride, int rows, const int64_t* ids, int64_t n, void* out,
                             int64_t out_stride, void* stream);
 
+/* ---------------------------------------------------------------------------------------------
+ * Prompts
+ * ------------------------------------------------------------------------------------------- */
+
+#define HQKV_F16 0
+#define HQKV_BF16 1
+#define HQKV_IMPORTANCE_ROWS 64 /* most rows of hqkv_prompt_importance */
+
+/*
+ * Packed sequences: the tokens of all of them one behind another, sequence s holding the queries q_starts[s] ... q_starts[s + 1] - 1
+ * and the keys k_starts[s] ... k_starts[s + 1] - 1 (int32 on the device, not decreasing; what lies outside 0 ... total is taken
+ * as the nearest of the two).  Element (token, head, channel) of a tensor is at token * x_token + head * x_head + channel; strides are in
+ * elements, multiples of 8 and not negative, bases 16-byte aligned.  Every sequence sees all prefix_len tokens of the prefix
+ * before its own keys.  causal: query i of a sequence with Lq queries and Lk keys sees its own keys j <= i + Lk - Lq; else all of them.
+ */
+typedef struct {
+  int32_t dtype;         /* HQKV_F16 or HQKV_BF16: q, k, v, prefix and output */
+  int32_t D;             /* head dim, must be 128 */
+  int32_t nh_q, nh_kv;   /* nh_q a multiple of nh_kv; query heads of one kv head are neighbours */
+  int32_t n_seqs, causal;
+  float scale;           /* multiplies q.k; positive */
+  int64_t total_q, total_k, prefix_len;
+  const void *q, *k, *v, *prefix_k, *prefix_v;
+  int64_t q_token, q_head, k_token, k_head, v_token, v_head;
+  int64_t prefix_k_token, prefix_k_head, prefix_v_token, prefix_v_head;
+  const int32_t *q_starts, *k_starts; /* [n_seqs + 1] */
+} hqkv_prompt_t;
+
+/*
+ * softmax(scale q K^T) V: what the flash-attention branch of the prefill computes (model/llama_hqe.py:141-166), for sequences of any
+ * lengths in one call.  out [total_q, nh_q, D] and lse fp32 [nh_q, total_q] (the log of the softmax's denominator), both dense.
+ * A query that sees no key has output 0 and lse -inf; rows of queries in no sequence are not written.  Scratch (for calls with few rows, whose
+ * keys are shared out) as hqkv_prompt_workspace_bytes says, 256-byte aligned, of any contents; the size depends on sizes alone,
+ * not on the starts.
+ */
+size_t hqkv_prompt_workspace_bytes(const hqkv_prompt_t* prompt_host);
+int hqkv_prompt_attention(const hqkv_prompt_t* prompt_host, void* out, float* lse, void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * Rows that seed the importance ring (the probabilities of a prompt's last queries, model/llama_hqe.py:124, 141-166, summed over
+ * the heads as last_attn_weights.update does, model/public_func.py:247-252): out fp16 [rows, total_k], where
+ *   out[r, k] = sum over the heads of exp(scale q_i.k - lse_i),  i = the r-th of the last t = min(rows, Lq) queries of k's sequence,
+ * summed in fp32 and rounded once; 0 for r >= t and for keys that i does not see.  lse as hqkv_prompt_attention left it, so that a
+ * prefix takes its share.  v, prefix_k and prefix_v are not read.  Columns of keys in no sequence are not written.
+ */
+int hqkv_prompt_importance(const hqkv_prompt_t* prompt_host, const float* lse, int rows, void* out_f16, void* stream);
+
+/*
+ * One decode step of a batch whose sequences share a dense prefix: hqkv_decode_attention over [prefix | own cache].  prefix_k / prefix_v
+ * fp16, element (token, kv head, channel) at token * stride + head * stride + channel (16-byte aligned, strides multiples of 8).
+ * attn_weights fp16 [B, nh_q, 1, L] are the probabilities of the cache's own tokens (they add up to 1 minus the prefix's share).
+ * workspace as for hqkv_decode_attention; prefix_workspace: hqkv_decode_prefix_workspace_bytes, 256-byte aligned, any contents.
+ */
+size_t hqkv_decode_prefix_workspace_bytes(const hqkv_cache_desc_t* cache_host, int64_t prefix_len);
+int hqkv_decode_attention_prefix(const hqkv_cache_desc_t* cache_host, const void* q, const void* prefix_k, const void* prefix_v,
+                                 int64_t prefix_len, int64_t k_token, int64_t k_head, int64_t v_token, int64_t v_head,
+                                 void* attn_weights, void* attn_output, void* workspace, size_t workspace_bytes,
+                                 void* prefix_workspace, size_t prefix_workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
