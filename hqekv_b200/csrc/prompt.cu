@@ -6,6 +6,12 @@
 //                      sequences' own caches)
 #include "prompt.cuh"
 
+#include <cudaTypedefs.h>
+
+#include <type_traits>
+
+#include "tensor.cuh"
+
 namespace hqkv {
 
 template <typename T>
@@ -14,70 +20,444 @@ template <>
 __device__ __forceinline__ float to_float(__half x) { return __half2float(x); }
 template <>
 __device__ __forceinline__ float to_float(__nv_bfloat16 x) { return __bfloat162float(x); }
-template <typename T>
-__device__ __forceinline__ T from_float(float x);
-template <>
-__device__ __forceinline__ __half from_float(float x) { return __float2half_rn(x); }
-template <>
-__device__ __forceinline__ __nv_bfloat16 from_float(float x) { return __float2bfloat16_rn(x); }
 
 __device__ __forceinline__ int start_of(const int* starts, int s, int total) { return min(max(starts[s], 0), total); }
 
-// A warp per query row, four channels per lane, one pass over the keys with the running maximum and sum of the softmax.
-template <typename T>
-__global__ void __launch_bounds__(256) prompt_rows_kernel(const PromptArgs A) {
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
-  const int lane = threadIdx.x & 31;
-  if (row >= static_cast<int64_t>(A.total_q) * A.nh_q) return;
-  const int token = static_cast<int>(row / A.nh_q), head = static_cast<int>(row % A.nh_q), kv = head / (A.nh_q / A.nh_kv);
-  int first = 0, own = 0;
-  if (A.n_seqs > 0) {
-    int s = 0;
-    while (s < A.n_seqs && start_of(A.q_starts, s + 1, A.total_q) <= token) ++s;
-    if (s == A.n_seqs || start_of(A.q_starts, s, A.total_q) > token) return;   // in no sequence
-    first = start_of(A.k_starts, s, A.total_k);
-    own = max(start_of(A.k_starts, s + 1, A.total_k) - first, 0);
-    if (A.causal) own = min(max(token + 1 + own - start_of(A.q_starts, s + 1, A.total_q), 0), own);
-  }
-  auto load = [&](const void* base, int64_t at, float (&v)[4]) {
-    const T* p = static_cast<const T*>(base) + at + 4 * lane;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = to_float(p[i]);
-  };
-  float q[4], o[4] = {0.f, 0.f, 0.f, 0.f}, m = -INFINITY, l = 0.f;
-  load(A.q, token * A.q_token + head * A.q_head, q);
-  const int n = A.prefix_len + own;
-  for (int j = 0; j < n; ++j) {
-    float k[4], v[4];
-    if (j < A.prefix_len) {
-      load(A.pk, j * A.pk_token + kv * A.pk_head, k);
-      load(A.pv, j * A.pv_token + kv * A.pv_head, v);
-    } else {
-      const int64_t t = first + (j - A.prefix_len);
-      load(A.k, t * A.k_token + kv * A.k_head, k);
-      load(A.v, t * A.v_token + kv * A.v_head, v);
-    }
-    float s = q[0] * k[0] + q[1] * k[1] + q[2] * k[2] + q[3] * k[3];
-#pragma unroll
-    for (int b = 16; b; b >>= 1) s += __shfl_xor_sync(0xffffffffu, s, b);
-    s *= A.scale_log2;
-    const float mx = fmaxf(m, s), ref = mx == -INFINITY ? 0.f : mx;
-    const float f = exp2f(m - ref), p = exp2f(s - ref);
-    l = l * f + p;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) o[i] = o[i] * f + p * v[i];
-    m = mx;
-  }
-  if (A.part_o) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) A.part_o[row * 128 + 4 * lane + i] = o[i];
-    if (lane == 0) A.part_ml[row] = make_float2(m, l);
+// ------------------------------------------------------------------------------------------------
+// Attention
+// ------------------------------------------------------------------------------------------------
+// A CTA takes 256 rows of queries - two tiles of 128 rows, a row being a (token, head of the group) - and walks the tiles of 128 keys that
+// any of them sees: first the prefix, then the sequence's own.  One pass, with the running maximum and sum of the softmax.
+//   warps 0-3, 4-7   softmax of the first and second row tile, a row per thread
+//   warp 8           issues the matrix products (one thread)
+//   warp 9           requests the tiles of Q, K and V (one thread)
+//   warp 10          looks after V tiles that not every row sees (below)
+// Tensor memory: S of both row tiles (128 columns each, overwritten by P in the type of V) and O of both.
+constexpr int TILE = 128;                                // keys per tile, rows per row tile
+constexpr int TILE_BYTES = TILE * 128 * 2;               // 64 channels of all its tokens, then the other 64
+constexpr int KV_STAGES = 5;
+constexpr int PROMPT_THREADS = 384;
+constexpr unsigned TMEM_COLUMNS = 512;
+constexpr float RESCALE_AT = 8.f;                        // powers of two that P may exceed 1 by
+
+struct PromptShared {
+  unsigned long long q_full, kv_full[KV_STAGES], kv_empty[KV_STAGES], v_raw[KV_STAGES];
+  unsigned long long s_full[2], p_first[2], p_rest[2], o_full[2], drained;
+  uint32_t tmem;
+  int stop, odd_values;
+  int q0, lq, k0, lk, tile, found;
+};
+constexpr size_t PROMPT_SMEM = 1024 + (2 + KV_STAGES) * static_cast<size_t>(TILE_BYTES) + sizeof(PromptShared);
+static_assert(PROMPT_SMEM <= 227 * 1024, "one CTA per SM");
+
+static __device__ unsigned g_waits_expired;
+
+// What a CTA works on: the t-th block of 256 / group tokens of all sequences (the last block of a sequence, which sees the most
+// keys, first).  One warp.
+__device__ __forceinline__ void find_block(const PromptArgs& A, int t, int tokens, int lane, PromptShared& sh) {
+  if (A.n_seqs == 0) {   // a single sequence without keys of its own
+    if (lane == 0) sh.q0 = 0, sh.lq = A.total_q, sh.k0 = 0, sh.lk = 0, sh.tile = t, sh.found = 1;
     return;
   }
-  const float inv = l == 0.f ? 0.f : 1.f / l;
+  int before = 0;
+  for (int s0 = 0; s0 < A.n_seqs; s0 += 32) {
+    const int s = s0 + lane;
+    int q0 = 0, lq = 0;
+    if (s < A.n_seqs) {
+      q0 = start_of(A.q_starts, s, A.total_q);
+      lq = max(start_of(A.q_starts, s + 1, A.total_q) - q0, 0);
+    }
+    const int blocks = (lq + tokens - 1) / tokens;
+    int sum = blocks;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) static_cast<T*>(A.out)[row * 128 + 4 * lane + i] = from_float<T>(o[i] * inv);
-  if (lane == 0) A.lse[static_cast<int64_t>(head) * A.total_q + token] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
+    for (int d = 1; d < 32; d <<= 1) {
+      const int up = __shfl_up_sync(0xffffffffu, sum, d);
+      if (lane >= d) sum += up;
+    }
+    const unsigned past = __ballot_sync(0xffffffffu, t < before + sum);
+    if (past) {
+      if (lane == __ffs(past) - 1) {
+        sh.q0 = q0, sh.lq = lq;
+        sh.tile = before + sum - 1 - t;
+        sh.k0 = start_of(A.k_starts, s, A.total_k);
+        sh.lk = max(start_of(A.k_starts, s + 1, A.total_k) - sh.k0, 0);
+        sh.found = 1;
+      }
+      return;
+    }
+    before += __shfl_sync(0xffffffffu, sum, 31);
+  }
+}
+
+// own keys that query i of its sequence sees
+__device__ __forceinline__ int keys_seen(const PromptArgs& A, int i, int lq, int lk) {
+  return A.causal ? min(max(i + 1 + lk - lq, 0), lk) : lk;
+}
+
+template <bool BF16>
+__device__ __forceinline__ bool odd_pair(uint32_t v) {   // an infinity or NaN in either half
+  constexpr uint32_t e = BF16 ? 0x7F80u : 0x7C00u;
+  return (v & e) == e || (v >> 16 & e) == e;
+}
+
+template <bool BF16>
+__global__ void __launch_bounds__(PROMPT_THREADS, 1) prompt_kernel(const __grid_constant__ PromptArgs A, const __grid_constant__ PromptMaps M) {
+  using T = std::conditional_t<BF16, __nv_bfloat16, __half>;
+  extern __shared__ unsigned char raw[];
+  unsigned char* const tiles = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  PromptShared& sh = *reinterpret_cast<PromptShared*>(tiles + (2 + KV_STAGES) * TILE_BYTES);
+  const uint32_t q_at = smem_u32(tiles), kv_at = q_at + 2 * TILE_BYTES;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int groups = A.nh_q / A.group;                       // head groups of all kv heads
+  const int t = blockIdx.x / groups, head0 = (blockIdx.x - t * groups) * A.group, kv = head0 / (A.nh_q / A.nh_kv);
+  const int half = TILE / A.group, tokens = 2 * half;        // tokens per row tile and CTA
+  if (threadIdx.x == 0) sh.found = 0;
+  __syncwarp();
+  if (warp == 0) find_block(A, t, tokens, lane, sh);
+  __syncthreads();
+  if (!sh.found) return;
+  const int q0 = sh.q0, lq = sh.lq, k0 = sh.k0, lk = sh.lk, i0 = sh.tile * tokens;   // i0: the CTA's first query in its sequence
+  // tiles of keys: those of the prefix, then the own ones up to the last that a row tile sees; this CTA's are [lo, hi[a])
+  const int before = (A.prefix_len + TILE - 1) / TILE;
+  const int seen_first = keys_seen(A, i0, lq, lk), seen_last = keys_seen(A, min(i0 + tokens, lq) - 1, lq, lk);
+  const int n1 = i0 + half < lq ? before + (seen_last + TILE - 1) / TILE : 0;
+  const int n0 = before + (keys_seen(A, min(i0 + half, lq) - 1, lq, lk) + TILE - 1) / TILE;
+  const int n = max(n0, n1);
+  const int lo = static_cast<int>(static_cast<int64_t>(n) * blockIdx.y / gridDim.y), hi = static_cast<int>(static_cast<int64_t>(n) * (blockIdx.y + 1) / gridDim.y);
+  const int hi0 = min(hi, n0), hi1 = min(hi, n1);
+  volatile int* const stop = &sh.stop;
+  if (warp == 8) tmem_alloc(smem_u32(&sh.tmem), TMEM_COLUMNS);
+  if (threadIdx.x == 0) {
+    sh.stop = 0, sh.odd_values = 0;
+    bar_init(smem_u32(&sh.q_full), 1);
+    bar_init(smem_u32(&sh.drained), 1);
+    for (int i = 0; i < KV_STAGES; ++i) {
+      bar_init(smem_u32(&sh.kv_full[i]), 1);
+      bar_init(smem_u32(&sh.kv_empty[i]), 1);
+      bar_init(smem_u32(&sh.v_raw[i]), 1);
+    }
+    for (int a = 0; a < 2; ++a) {
+      bar_init(smem_u32(&sh.s_full[a]), 1);
+      bar_init(smem_u32(&sh.p_first[a]), 4);
+      bar_init(smem_u32(&sh.p_rest[a]), 4);
+      bar_init(smem_u32(&sh.o_full[a]), 1);
+    }
+    bar_init_fence();
+  }
+  fence_before();
+  __syncthreads();
+  fence_after();
+  const uint32_t tmem = sh.tmem;
+  // Own V tiles that hold keys which some rows of the CTA do not see.  0 x NaN is NaN in a matrix product, so what lies behind
+  // the last key that any row sees is set to 0; an infinity or NaN that only some rows see is set to 0 as well, and those rows
+  // add it at the end.
+  auto partly_seen = [&](int i) { return i >= before && (i - before + 1) * TILE > seen_first; };
+
+  if (warp < 8) {
+    // ---- softmax
+    const int a = warp >> 2, row = threadIdx.x & 127, i = i0 + a * half + row / A.group, head = head0 + row % A.group;
+    const int end = a ? hi1 : hi0, count = max(end - lo, 0);
+    const bool live = i < lq;
+    const int seen = live ? keys_seen(A, i, lq, lk) : lk;
+    const uint32_t lanes = tmem + (static_cast<uint32_t>(warp & 3) << 21);   // (32 lanes a warp, in bits 16 and up)
+    const uint32_t s_at = lanes + a * TILE, o_at = lanes + 2 * TILE + a * 128;
+    float ref = -INFINITY, sum = 0.f;
+    const float scale = A.scale_log2;
+    bool ok = true;
+#pragma unroll 1
+    for (int it = 0; it < count; ++it) {
+      if (!(ok = __all_sync(0xffffffffu, bar_wait(smem_u32(&sh.s_full[a]), it & 1, stop)))) break;
+      fence_after();
+      uint32_t s[TILE];
+#pragma unroll
+      for (int c = 0; c < TILE; c += 32) tmem_load32(s_at + c, s + c);
+      wait_loads();
+      const int tile = lo + it, limit = tile < before ? A.prefix_len - tile * TILE : seen - (tile - before) * TILE;
+      if (__any_sync(0xffffffffu, limit < TILE)) {
+#pragma unroll
+        for (int c = 0; c < TILE; ++c)
+          if (c >= limit) s[c] = 0xFF800000u;   // -inf
+      }
+      float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+      for (int c = 0; c < TILE; c += 8)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) mx[k] = max3(mx[k], __uint_as_float(s[c + 2 * k]), __uint_as_float(s[c + 2 * k + 1]));
+      const float top = fmaxf(max3(mx[0], mx[1], mx[2]), mx[3]) * scale;
+      // O and the sum are scaled to the maximum only where it has grown enough to matter: P stays below 2^8
+      const bool grown = top > ref + RESCALE_AT;
+      if (__any_sync(0xffffffffu, grown)) {
+        const float f = grown ? exp2_approx(ref - top) : 1.f;
+        if (grown) ref = top;
+        sum *= f;
+        if (it > 0) {
+          // (the product with the tile before, which was issued before this S, is complete)
+#pragma unroll 1
+          for (int c = 0; c < 128; c += 32) {
+            uint32_t o[32];
+            tmem_load32(o_at + c, o);
+            wait_loads();
+#pragma unroll
+            for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * f);
+            tmem_store32(o_at + c, o);
+          }
+        }
+      }
+      const float shift = ref == -INFINITY ? 0.f : -ref;
+      const uint64_t scale2 = pair(scale, scale), shift2 = pair(shift, shift);
+      uint64_t sums[2] = {0ull, 0ull};
+#pragma unroll
+      for (int c = 0; c < TILE; c += 32) {
+        uint32_t p[16];
+#pragma unroll
+        for (int k = 0; k < 16; ++k) {
+          float x, y;
+          unpair(pair_fma(pair(__uint_as_float(s[c + 2 * k]), __uint_as_float(s[c + 2 * k + 1])), scale2, shift2), x, y);
+          x = exp2_approx(x), y = exp2_approx(y);
+          sums[k & 1] = pair_add(sums[k & 1], pair(x, y));
+          p[k] = narrow2<BF16>(x, y);
+        }
+        tmem_store16(s_at + c / 2, p);
+        if (c >= TILE - 64) {
+          wait_stores();
+          fence_before();
+          __syncwarp();
+          if (lane == 0) bar_arrive(smem_u32(c == TILE - 64 ? &sh.p_first[a] : &sh.p_rest[a]));
+        }
+      }
+      float x, y;
+      unpair(pair_add(sums[0], sums[1]), x, y);
+      sum += x + y;
+    }
+    // ---- output
+    if (count > 0 && ok) ok = __all_sync(0xffffffffu, bar_wait(smem_u32(&sh.o_full[a]), 0, stop));
+    if (ok) {
+      fence_after();
+      const int64_t at = (static_cast<int64_t>(q0 + i) * A.nh_q + head);
+      const bool odd = *const_cast<volatile int*>(&sh.odd_values) != 0;
+      const float by = A.part_o ? 1.f : sum == 0.f ? 0.f : 1.f / sum;
+      if (live && A.part_o) A.part_ml[static_cast<int64_t>(blockIdx.y) * A.total_q * A.nh_q + at] = make_float2(ref, sum);
+      else if (live) A.lse[static_cast<int64_t>(head) * A.total_q + q0 + i] = sum == 0.f ? -INFINITY : (ref + log2f(sum)) * 0.6931471805599453f;
+#pragma unroll 1
+      for (int c = 0; c < 128; c += 32) {
+        uint32_t o[32];
+        if (count > 0) {
+          tmem_load32(o_at + c, o);
+          wait_loads();
+        } else {
+#pragma unroll
+          for (int k = 0; k < 32; ++k) o[k] = 0u;
+        }
+        if (!live) continue;
+        if (odd) {
+          const int to = min(seen, (end - before) * TILE);
+          for (int j = max(seen_first, (lo - before) * TILE); j < to; ++j) {
+            const T* v = static_cast<const T*>(A.v) + (k0 + j) * A.v_token + kv * A.v_head + c;
+#pragma unroll
+            for (int k = 0; k < 32; ++k) {
+              const float x = to_float(v[k]);
+              if (!isfinite(x)) o[k] = __float_as_uint(__uint_as_float(o[k]) + x);
+            }
+          }
+        }
+        if (A.part_o) {
+          uint4* to = reinterpret_cast<uint4*>(A.part_o + (static_cast<int64_t>(blockIdx.y) * A.total_q * A.nh_q + at) * 128 + c);
+#pragma unroll
+          for (int k = 0; k < 8; ++k) to[k] = make_uint4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]);
+        } else {
+          uint32_t h[16];
+#pragma unroll
+          for (int k = 0; k < 16; ++k) h[k] = narrow2<BF16>(__uint_as_float(o[2 * k]) * by, __uint_as_float(o[2 * k + 1]) * by);
+          uint4* to = reinterpret_cast<uint4*>(static_cast<T*>(A.out) + at * 128 + c);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) to[k] = make_uint4(h[4 * k], h[4 * k + 1], h[4 * k + 2], h[4 * k + 3]);
+        }
+      }
+    }
+  } else if (warp == 8) {
+    // ---- matrix products
+    if (lane == 0 && hi > lo) {
+      constexpr uint32_t kind_s = mma_kind(BF16, TILE, TILE, false), kind_o = mma_kind(BF16, TILE, 128, true);
+      int stage = 0;
+      unsigned phase = 0;
+      auto scores = [&](int a, uint32_t k_at) {   // S = Q K^T, 16 channels at a time
+#pragma unroll
+        for (int c = 0; c < 8; ++c)
+          mma_shared(tmem + a * TILE, operand(q_at + a * TILE_BYTES + (c >> 2) * (TILE_BYTES / 2) + (c & 3) * 32, 16),
+                     operand(k_at + (c >> 2) * (TILE_BYTES / 2) + (c & 3) * 32, 16), kind_s, c > 0);
+        mma_commit(smem_u32(&sh.s_full[a]));
+      };
+      auto advance = [&] {
+        if (++stage == KV_STAGES) stage = 0, phase ^= 1;
+      };
+      bool ok = bar_wait(smem_u32(&sh.q_full), 0, stop) && bar_wait(smem_u32(&sh.kv_full[0]), 0, stop);
+      if (ok) {
+        fence_after();
+        if (lo < hi0) scores(0, kv_at);
+        if (lo < hi1) scores(1, kv_at);
+        mma_commit(smem_u32(&sh.kv_empty[0]));
+        advance();
+      }
+#pragma unroll 1
+      for (int i = lo; ok && i < hi; ++i) {
+        const int v_stage = stage;
+        if (!(ok = bar_wait(smem_u32(&sh.kv_full[stage]), phase, stop))) break;
+        advance();
+        const uint32_t v_at = kv_at + v_stage * TILE_BYTES, k_at = kv_at + stage * TILE_BYTES;
+        bool have_k = false;
+#pragma unroll
+        for (int a = 0; a < 2; ++a) {
+          const int end = a ? hi1 : hi0;
+          if (i < end) {
+            // O += P V, 16 keys at a time, the first three quarters as soon as they are there
+            if (!(ok = bar_wait(smem_u32(&sh.p_first[a]), (i - lo) & 1, stop))) break;
+            fence_after();
+#pragma unroll
+            for (int c = 0; c < 6; ++c)
+              mma_tensor(tmem + 2 * TILE + a * 128, tmem + a * TILE + c * 8, operand(v_at + c * 2048, TILE_BYTES / 2), kind_o, c > 0 || i > lo);
+            if (!(ok = bar_wait(smem_u32(&sh.p_rest[a]), (i - lo) & 1, stop))) break;
+            fence_after();
+#pragma unroll
+            for (int c = 6; c < 8; ++c)
+              mma_tensor(tmem + 2 * TILE + a * 128, tmem + a * TILE + c * 8, operand(v_at + c * 2048, TILE_BYTES / 2), kind_o, true);
+            if (i + 1 == end) mma_commit(smem_u32(&sh.o_full[a]));
+          }
+          if (a == 1) mma_commit(smem_u32(&sh.kv_empty[v_stage]));
+          if (i + 1 < end) {
+            if (!have_k && !(ok = bar_wait(smem_u32(&sh.kv_full[stage]), phase, stop))) break;
+            fence_after();
+            have_k = true;
+            scores(a, k_at);
+          }
+        }
+        if (!ok) break;
+        if (i + 1 < hi) {
+          mma_commit(smem_u32(&sh.kv_empty[stage]));
+          advance();
+        }
+      }
+      if (!ok) {   // products in flight end before the CTA does
+        mma_commit(smem_u32(&sh.drained));
+        for (int k = 0; k < WAIT_TRIES && !bar_try(smem_u32(&sh.drained), 0); ++k) {
+        }
+      }
+    }
+  } else if (warp == 9) {
+    // ---- copies: Q, then K and V of one tile after the other
+    if (lane == 0 && hi > lo) {
+      bar_expect(smem_u32(&sh.q_full), 2 * TILE_BYTES);
+      for (int a = 0; a < 2; ++a)
+        for (int c = 0; c < 2; ++c)
+          copy_box(q_at + a * TILE_BYTES + c * (TILE_BYTES / 2), &M.q, 64 * c, head0, q0 + i0 + a * half, smem_u32(&sh.q_full));
+      int stage = 0;
+      unsigned phase = 1, to_raw = 0, raw_parity = 0, full_parity = 0, used = 0;   // a bit per stage: of the last copy into it
+      bool ok = true;
+#pragma unroll 1
+      for (int i = lo; ok && i < hi; ++i) {
+        const bool own = i >= before;
+        const int token = own ? k0 + (i - before) * TILE : i * TILE;
+#pragma unroll 1
+        for (int side = 0; side < 2; ++side) {
+          if (!(ok = bar_wait(smem_u32(&sh.kv_empty[stage]), phase, stop))) break;
+          const CUtensorMap* map = side ? (own ? &M.v : &M.pv) : (own ? &M.k : &M.pk);
+          const bool raw_first = side && partly_seen(i);
+          const uint32_t bar = smem_u32(raw_first ? &sh.v_raw[stage] : &sh.kv_full[stage]), bit = 1u << stage;
+          if (used & bit) full_parity ^= bit;
+          if (raw_first) raw_parity ^= bit;
+          used |= bit;
+          to_raw = raw_first ? to_raw | bit : to_raw & ~bit;
+          bar_expect(bar, TILE_BYTES);
+          for (int c = 0; c < 2; ++c) copy_box(kv_at + stage * TILE_BYTES + c * (TILE_BYTES / 2), map, 64 * c, kv, token, bar);
+          if (++stage == KV_STAGES) stage = 0, phase ^= 1;
+        }
+      }
+      if (!ok) {   // copies in flight land before the CTA ends
+        auto landed = [&](const unsigned long long& bar, unsigned parity) {
+          for (int k = 0; k < WAIT_TRIES && !bar_try(smem_u32(&bar), parity); ++k) {
+          }
+        };
+        landed(sh.q_full, 0);
+        for (int k = 0; k < KV_STAGES; ++k) {
+          if (!(used >> k & 1)) continue;
+          if (to_raw >> k & 1) landed(sh.v_raw[k], (raw_parity >> k & 1) ^ 1);
+          else landed(sh.kv_full[k], full_parity >> k & 1);
+        }
+      }
+    }
+  } else if (warp == 10) {
+    // ---- V tiles that not every row sees
+    unsigned parity = 0;   // a bit per stage
+#pragma unroll 1
+    for (int i = lo; i < hi; ++i) {
+      if (!partly_seen(i)) continue;
+      const int stage = (2 * (i - lo) + 1) % KV_STAGES, first = (i - before) * TILE;
+      if (!bar_wait(smem_u32(&sh.v_raw[stage]), parity >> stage & 1, stop)) break;
+      parity ^= 1u << stage;
+      unsigned char* const v = tiles + (2 + stage) * TILE_BYTES;
+      bool odd = false;
+      // (which of a row's pieces of 16 bytes comes where does not matter here)
+      for (int k = lane; k < TILE_BYTES / 16; k += 32) {
+        const int token = first + (k >> 3 & (TILE - 1));
+        if (token < seen_first) continue;
+        uint4* const at = reinterpret_cast<uint4*>(v + k * 16);
+        if (token >= seen_last) {
+          *at = make_uint4(0u, 0u, 0u, 0u);
+          continue;
+        }
+        uint4 x = *at;
+        if (odd_pair<BF16>(x.x) || odd_pair<BF16>(x.y) || odd_pair<BF16>(x.z) || odd_pair<BF16>(x.w)) {
+          odd = true;
+          uint32_t* w = &x.x;
+          constexpr uint32_t e = BF16 ? 0x7F80u : 0x7C00u;
+          for (int m = 0; m < 4; ++m) {
+            if ((w[m] & e) == e) w[m] &= 0xFFFF0000u;
+            if ((w[m] >> 16 & e) == e) w[m] &= 0x0000FFFFu;
+          }
+          *at = x;
+        }
+      }
+      if (odd) *const_cast<volatile int*>(&sh.odd_values) = 1;
+      fence_generic_to_async();
+      __syncwarp();
+      if (lane == 0) bar_arrive(smem_u32(&sh.kv_full[stage]));
+    }
+  }
+  __syncwarp();
+  fence_before();
+  __syncthreads();
+  fence_after();
+  if (warp == 8) tmem_free(tmem, TMEM_COLUMNS);
+  if (threadIdx.x == 0 && *stop) atomicAdd(&g_waits_expired, 1u);
+}
+
+// Joins the parts of a row: a warp per row.
+template <bool BF16>
+__global__ void __launch_bounds__(256) prompt_join_kernel(const PromptArgs A, int splits) {
+  using T = std::conditional_t<BF16, __nv_bfloat16, __half>;
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5), rows = static_cast<int64_t>(A.total_q) * A.nh_q;
+  const int lane = threadIdx.x & 31;
+  if (row >= rows) return;
+  const int token = static_cast<int>(row / A.nh_q), head = static_cast<int>(row % A.nh_q);
+  bool in = false;
+  for (int s = lane; s < A.n_seqs; s += 32)
+    in |= token >= start_of(A.q_starts, s, A.total_q) && token < start_of(A.q_starts, s + 1, A.total_q);
+  if (!__any_sync(0xffffffffu, in)) return;
+  float m = -INFINITY, l = 0.f;
+  for (int s = 0; s < splits; ++s) m = fmaxf(m, A.part_ml[s * rows + row].x);
+  const float ref = m == -INFINITY ? 0.f : m;
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int s = 0; s < splits; ++s) {
+    const float2 part = A.part_ml[s * rows + row];
+    if (part.y == 0.f) continue;   // it had no keys that this row sees
+    const float f = exp2_approx(part.x - ref);
+    const float4 v = *reinterpret_cast<const float4*>(A.part_o + (s * rows + row) * 128 + 4 * lane);
+    l += f * part.y;
+    o.x += f * v.x, o.y += f * v.y, o.z += f * v.z, o.w += f * v.w;
+  }
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  *reinterpret_cast<uint2*>(static_cast<T*>(A.out) + row * 128 + 4 * lane) =
+      make_uint2(narrow2<BF16>(o.x * inv, o.y * inv), narrow2<BF16>(o.z * inv, o.w * inv));
+  if (lane == 0) A.lse[static_cast<int64_t>(head) * A.total_q + token] = l == 0.f ? -INFINITY : (ref + log2f(l)) * 0.6931471805599453f;
 }
 
 // A thread per key, the sums over the heads in shared memory.
@@ -113,6 +493,13 @@ __global__ void __launch_bounds__(IMP_KEYS) prompt_importance_kernel(const Promp
 // ------------------------------------------------------------------------------------------------
 // host side
 // ------------------------------------------------------------------------------------------------
+// Query heads that share a row tile: those of one kv head, as many of them as a power of two takes (at most 32: four tokens).
+static int head_group(int nh_q, int nh_kv) {
+  int g = 1;
+  while (g < 32 && nh_q / nh_kv % (2 * g) == 0) g *= 2;
+  return g;
+}
+
 static int prompt_args(const hqkv_prompt_t* p, bool values, PromptArgs& A) {
   HQKV_REQUIRE(p != nullptr, "prompt: null descriptor");
   HQKV_REQUIRE(p->dtype == HQKV_F16 || p->dtype == HQKV_BF16, "prompt: unknown type %d", p->dtype);
@@ -134,11 +521,13 @@ static int prompt_args(const hqkv_prompt_t* p, bool values, PromptArgs& A) {
                                before && values ? p->prefix_v : nullptr};
   const int64_t strides[5][2] = {{p->q_token, p->q_head}, {p->k_token, p->k_head}, {p->v_token, p->v_head},
                                  {p->prefix_k_token, p->prefix_k_head}, {p->prefix_v_token, p->prefix_v_head}};
+  const int64_t entries[5][2] = {{p->total_q, p->nh_q}, {p->total_k, p->nh_kv}, {p->total_k, p->nh_kv}, {p->prefix_len, p->nh_kv}, {p->prefix_len, p->nh_kv}};
   for (int i = 0; i < 5; ++i) {
     if (!base[i]) continue;
     HQKV_REQUIRE(aligned(base[i], 16), "prompt: tensors must be 16-byte aligned");
-    for (int64_t s : strides[i])
-      HQKV_REQUIRE(s >= 0 && s % 8 == 0 && s < (1ll << 38), "prompt: strides must be multiples of 8 elements, and not negative");
+    for (int d = 0; d < 2; ++d)
+      HQKV_REQUIRE(entries[i][d] < 2 || (strides[i][d] > 0 && strides[i][d] % 8 == 0 && strides[i][d] < (1ll << 38)),
+                   "prompt: strides must be multiples of 8 elements, and positive");
   }
   A = PromptArgs();
   A.q = p->q, A.k = p->k, A.v = p->v, A.pk = p->prefix_k, A.pv = p->prefix_v;
@@ -150,41 +539,131 @@ static int prompt_args(const hqkv_prompt_t* p, bool values, PromptArgs& A) {
   A.nh_q = p->nh_q, A.nh_kv = p->nh_kv;
   A.causal = p->causal != 0;
   A.bf16 = p->dtype == HQKV_BF16;
+  A.group = head_group(p->nh_q, p->nh_kv);
   A.scale_log2 = p->scale * 1.4426950408889634f;
   return HQKV_OK;
 }
 
-static int launch_rows(const PromptArgs& A, cudaStream_t st) {
-  const int64_t rows = static_cast<int64_t>(A.total_q) * A.nh_q;
-  const unsigned grid = static_cast<unsigned>(ceil_div(rows, 8));
-  if (A.bf16) prompt_rows_kernel<__nv_bfloat16><<<grid, 256, 0, st>>>(A);
-  else prompt_rows_kernel<__half><<<grid, 256, 0, st>>>(A);
-  HQKV_LAUNCH_CHECK("prompt_rows");
+// Blocks of queries that all sequences together have at most (their lengths are on the device).
+static int64_t most_blocks(const PromptArgs& A) {
+  const int64_t tokens = 2 * TILE / A.group, n = max(1, min(A.n_seqs, A.total_q));
+  return (A.total_q + n * (tokens - 1)) / tokens;
+}
+
+// Where the CTAs do not fill the GPU, the tiles of keys are shared out as well.
+static int prompt_splits(const PromptArgs& A) {
+  const int64_t ctas = most_blocks(A) * (A.nh_q / A.group);
+  const int64_t tiles = ceil_div(A.prefix_len, TILE) + ceil_div(A.total_k / max(1, A.n_seqs), TILE);
+  return static_cast<int>(max(int64_t{1}, min(148 / max(int64_t{1}, ctas), tiles)));
+}
+
+static int tensor_map(CUtensorMap* map, const void* base, bool bf16, int64_t tokens, int heads, int64_t token_stride, int64_t head_stride,
+                      int box_heads, int box_tokens) {
+  static PFN_cuTensorMapEncodeTiled_v12000 encode = nullptr;   // (whoever is first stores what every other thread would)
+  if (!encode) {
+    void* f = nullptr;
+    cudaDriverEntryPointQueryResult found;
+    HQKV_CUDA(cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &f, 12000, cudaEnableDefault, &found));
+    if (found != cudaDriverEntryPointSuccess || !f) return fail(HQKV_E_CUDA, "prompt: the driver has no cuTensorMapEncodeTiled");
+    encode = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(f);
+  }
+  const cuuint64_t size[3] = {128, static_cast<cuuint64_t>(heads), static_cast<cuuint64_t>(tokens)};
+  // (a dimension of one entry may come with any stride)
+  const cuuint64_t stride[2] = {static_cast<cuuint64_t>(heads > 1 ? 2 * head_stride : 256), static_cast<cuuint64_t>(tokens > 1 ? 2 * token_stride : 256)};
+  const cuuint32_t box[3] = {64, static_cast<cuuint32_t>(box_heads), static_cast<cuuint32_t>(box_tokens)}, step[3] = {1, 1, 1};
+  const CUresult rc = encode(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<void*>(base), size, stride,
+                             box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (rc != CUDA_SUCCESS) return fail(HQKV_E_CUDA, "prompt: cuTensorMapEncodeTiled failed (%d)", static_cast<int>(rc));
   return HQKV_OK;
 }
 
-int prefix_splits(const hqkv_prompt_t*) { return 1; }
+static int launch_prompt(const PromptArgs& A, int splits, cudaStream_t st) {
+  PromptMaps M = {};
+  if (int rc = tensor_map(&M.q, A.q, A.bf16, A.total_q, A.nh_q, A.q_token, A.q_head, A.group, TILE / A.group)) return rc;
+  if (A.total_k > 0) {
+    if (int rc = tensor_map(&M.k, A.k, A.bf16, A.total_k, A.nh_kv, A.k_token, A.k_head, 1, TILE)) return rc;
+    if (int rc = tensor_map(&M.v, A.v, A.bf16, A.total_k, A.nh_kv, A.v_token, A.v_head, 1, TILE)) return rc;
+  }
+  if (A.prefix_len > 0) {
+    if (int rc = tensor_map(&M.pk, A.pk, A.bf16, A.prefix_len, A.nh_kv, A.pk_token, A.pk_head, 1, TILE)) return rc;
+    if (int rc = tensor_map(&M.pv, A.pv, A.bf16, A.prefix_len, A.nh_kv, A.pv_token, A.pv_head, 1, TILE)) return rc;
+  }
+  static bool opted_in[64] = {};   // per device
+  int dev = 0;
+  HQKV_CUDA(cudaGetDevice(&dev));
+  if (dev < 0 || dev >= 64 || !opted_in[dev]) {
+    HQKV_CUDA(cudaFuncSetAttribute(prompt_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(PROMPT_SMEM)));
+    HQKV_CUDA(cudaFuncSetAttribute(prompt_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(PROMPT_SMEM)));
+    if (dev >= 0 && dev < 64) opted_in[dev] = true;
+  }
+  const int64_t blocks = most_blocks(A) * (A.nh_q / A.group);
+  HQKV_REQUIRE(blocks < (1ll << 31), "prompt: too many rows");
+  const dim3 grid(static_cast<unsigned>(blocks), splits);
+  (A.bf16 ? prompt_kernel<true> : prompt_kernel<false>)<<<grid, PROMPT_THREADS, PROMPT_SMEM, st>>>(A, M);
+  HQKV_LAUNCH_CHECK("prompt");
+  return HQKV_OK;
+}
 
-int prefix_partial(const hqkv_prompt_t* p, float* part_o, float2* part_ml, int, cudaStream_t st) {
+int prefix_splits(const hqkv_prompt_t* p) {
+  PromptArgs A;
+  A.total_q = static_cast<int>(p->total_q), A.total_k = 0, A.n_seqs = 0, A.prefix_len = static_cast<int>(p->prefix_len);
+  A.nh_q = p->nh_q, A.nh_kv = p->nh_kv, A.group = head_group(p->nh_q, p->nh_kv);
+  return prompt_splits(A);
+}
+
+int prefix_partial(const hqkv_prompt_t* p, float* part_o, float2* part_ml, int splits, cudaStream_t st) {
   PromptArgs A;
   if (int rc = prompt_args(p, true, A)) return rc;
   A.part_o = part_o, A.part_ml = part_ml;
-  return launch_rows(A, st);
+  return launch_prompt(A, splits, st);
+}
+
+static size_t split_bytes(const PromptArgs& A, int splits, size_t* part_ml) {
+  const size_t rows = static_cast<size_t>(A.total_q) * A.nh_q * splits;
+  *part_ml = rows * 128 * sizeof(float);
+  return splits > 1 ? *part_ml + rows * sizeof(float2) : 0;
 }
 
 }  // namespace hqkv
 
 using namespace hqkv;
 
-extern "C" size_t hqkv_prompt_workspace_bytes(const hqkv_prompt_t*) { return 0; }
+extern "C" size_t hqkv_prompt_workspace_bytes(const hqkv_prompt_t* prompt_host) {
+  PromptArgs A;
+  if (prompt_args(prompt_host, true, A) != HQKV_OK || A.total_q == 0 || A.n_seqs == 0) return 0;
+  size_t ml;
+  return split_bytes(A, prompt_splits(A), &ml);
+}
 
-extern "C" int hqkv_prompt_attention(const hqkv_prompt_t* prompt_host, void* out, float* lse, void*, size_t, void* stream) {
+extern "C" int hqkv_prompt_attention(const hqkv_prompt_t* prompt_host, void* out, float* lse, void* workspace, size_t workspace_bytes, void* stream) {
   PromptArgs A;
   if (int rc = prompt_args(prompt_host, true, A)) return rc;
   if (A.total_q == 0 || A.n_seqs == 0) return HQKV_OK;
   HQKV_REQUIRE(out && lse && aligned(out, 16) && aligned(lse, 4), "prompt: the outputs are null or misaligned");
   A.out = out, A.lse = lse;
-  return launch_rows(A, static_cast<cudaStream_t>(stream));
+  const int splits = prompt_splits(A);
+  size_t ml;
+  const size_t need = split_bytes(A, splits, &ml);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (splits == 1) return launch_prompt(A, 1, st);
+  HQKV_REQUIRE(workspace && aligned(workspace, 256), "prompt: the workspace is null or not 256-byte aligned");
+  if (workspace_bytes < need) return fail(HQKV_E_WORKSPACE, "prompt: the workspace holds %zu bytes, %zu needed", workspace_bytes, need);
+  A.part_o = static_cast<float*>(workspace);
+  A.part_ml = reinterpret_cast<float2*>(static_cast<unsigned char*>(workspace) + ml);
+  if (int rc = launch_prompt(A, splits, st)) return rc;
+  const unsigned grid = static_cast<unsigned>(ceil_div(static_cast<int64_t>(A.total_q) * A.nh_q, 8));
+  (A.bf16 ? prompt_join_kernel<true> : prompt_join_kernel<false>)<<<grid, 256, 0, st>>>(A, splits);
+  HQKV_LAUNCH_CHECK("prompt_join");
+  return HQKV_OK;
+}
+
+extern "C" int hqkv_prompt_waits_expired(int reset, unsigned* count_host) {
+  HQKV_REQUIRE(count_host != nullptr, "prompt_waits_expired: null pointer");
+  const unsigned zero = 0;
+  HQKV_CUDA(cudaMemcpyFromSymbol(count_host, hqkv::g_waits_expired, sizeof(unsigned)));
+  if (reset) HQKV_CUDA(cudaMemcpyToSymbol(hqkv::g_waits_expired, &zero, sizeof(unsigned)));
+  return HQKV_OK;
 }
 
 extern "C" int hqkv_prompt_importance(const hqkv_prompt_t* prompt_host, const float* lse, int rows, void* out_f16, void* stream) {

@@ -3,6 +3,8 @@
 
 #include <cuda_bf16.h>
 
+#include <cuda.h>
+
 #include "common.cuh"
 
 namespace hqkv {
@@ -12,12 +14,17 @@ struct PromptArgs {
   int64_t q_token, q_head, k_token, k_head, v_token, v_head, pk_token, pk_head, pv_token, pv_head;
   const int *q_starts, *k_starts;                   // [n_seqs + 1]
   int n_seqs, total_q, total_k, prefix_len, nh_q, nh_kv;
+  int group;                                        // query heads of a kv head that share a row tile
   bool causal, bf16;
   float scale_log2;                                 // scale * log2(e)
   void* out;                                        // [total_q][nh_q][128]
   float* lse;                                       // [nh_q][total_q]
   float* part_o;                                    // [splits][total_q * nh_q][128], not yet normalised (null: out and lse)
   float2* part_ml;                                  // [splits][total_q * nh_q] (maximum, sum), in powers of two
+};
+
+struct PromptMaps {   // the tensors as (channel, head, token), for copies by tiles
+  CUtensorMap q, k, v, pk, pv;
 };
 
 // Attention of p's queries (a token each, no sequences) to its prefix alone: splits parts per row, to be joined.

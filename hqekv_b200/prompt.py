@@ -20,6 +20,11 @@ MAX_ROWS = 64   # HQKV_IMPORTANCE_ROWS
 _DTYPES = {torch.float16: 0, torch.bfloat16: 1}
 
 
+def usable(x):
+    """Whether the kernels read a [tokens, heads, 128] tensor where it is."""
+    return x.stride(2) == 1 and x.data_ptr() % 16 == 0 and all(x.shape[d] < 2 or (x.stride(d) > 0 and x.stride(d) % 8 == 0) for d in (0, 1))
+
+
 def _tensor(name, x, like=None, heads=None, tokens=None):
     """A [tokens, heads, 128] operand as the kernels take it: channels adjacent, 16-byte aligned rows (copied where it is not)."""
     if x.dim() != 3 or x.shape[2] != HEAD_DIM:
@@ -32,8 +37,7 @@ def _tensor(name, x, like=None, heads=None, tokens=None):
         raise ValueError(f"{name} must have {tokens} tokens (got {x.shape[0]})")
     if x.requires_grad and torch.is_grad_enabled():
         raise RuntimeError("the prompt operators have no backward pass: call them under torch.no_grad()")
-    usable = x.stride(2) == 1 and x.data_ptr() % 16 == 0 and x.stride(0) % 8 == 0 and x.stride(1) % 8 == 0
-    return x if usable else x.clone(memory_format=torch.contiguous_format)
+    return x if usable(x) else x.clone(memory_format=torch.contiguous_format)
 
 
 def _starts(name, x, device, n=None):

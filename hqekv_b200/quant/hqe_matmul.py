@@ -8,6 +8,7 @@ from typing import Tuple
 import torch
 
 from .._lib import CODEC_NORMAL, CODEC_UNIFORM, HqkvError, check, decode_workspace, host, lib, ptr, require_cuda, stream_ptr
+from ..prompt import usable
 from ._cache import UNIFORM_STRATEGIES, cached_cache_desc
 
 
@@ -104,8 +105,7 @@ def qkv_matmul_hqe_prefix(q: torch.Tensor, past_key_value: Tuple, prefix: Tuple[
     if pk.shape[0] != pv.shape[0] or pk.shape[0] == 0:
         raise ValueError("the prefix's k and v must hold the same number of tokens, at least one")
     require_cuda(q, pk, pv)
-    pk, pv = (x if x.stride(2) == 1 and x.data_ptr() % 16 == 0 and x.stride(0) % 8 == 0 and x.stride(1) % 8 == 0
-              else x.clone(memory_format=torch.contiguous_format) for x in (pk, pv))
+    pk, pv = (x if usable(x) else x.clone(memory_format=torch.contiguous_format) for x in (pk, pv))
     q = q.contiguous()
     if q.data_ptr() % 16:
         q = q.clone()

@@ -504,7 +504,7 @@ int hqkv_gather_columns_f16(const void* in, int64_t in_stride, int rows, const i
  * Packed sequences: the tokens of all of them one behind another, sequence s holding the queries q_starts[s] ... q_starts[s + 1] - 1
  * and the keys k_starts[s] ... k_starts[s + 1] - 1 (int32 on the device, not decreasing; what lies outside 0 ... total is taken
  * as the nearest of the two).  Element (token, head, channel) of a tensor is at token * x_token + head * x_head + channel; strides are in
- * elements, multiples of 8 and not negative, bases 16-byte aligned.  Every sequence sees all prefix_len tokens of the prefix
+ * elements, multiples of 8 and positive (of any value where there is one token or head), bases 16-byte aligned.  Every sequence sees all prefix_len tokens of the prefix
  * before its own keys.  causal: query i of a sequence with Lq queries and Lk keys sees its own keys j <= i + Lk - Lq; else all of them.
  */
 typedef struct {
@@ -529,6 +529,12 @@ typedef struct {
  */
 size_t hqkv_prompt_workspace_bytes(const hqkv_prompt_t* prompt_host);
 int hqkv_prompt_attention(const hqkv_prompt_t* prompt_host, void* out, float* lse, void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * The kernel's waits for its own copies and products have a limit of some seconds.  A CTA in which one runs out ends without a
+ * result and is counted here: 0 unless the GPU is not working properly.  Waits for the device's work and (optionally) clears the count.
+ */
+int hqkv_prompt_waits_expired(int reset, unsigned* count_host);
 
 /*
  * Rows that seed the importance ring (the probabilities of a prompt's last queries, model/llama_hqe.py:124, 141-166, summed over

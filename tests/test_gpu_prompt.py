@@ -1,12 +1,14 @@
 """GPU tests of the prompt operators (hqekv_b200/prompt.py) and of the decode behind a shared prefix against their formulas in 64 bits.
 
 Tolerances, per element, with u = half a step of the type (2^-11 for fp16, 2^-8 for bf16):
-* output: u sum_j p_j |v_j| for the probabilities rounded before the product with V, u |o| for the output's own rounding, and for fp32 arithmetic
-  2^-18 (|s| + 16) of the sums (a logit s of 128 terms of one sign is off by 2^-17 of it at most, mostly far less, and an exponential by as much).
-  Probabilities below 2^-14 of the largest are subnormal halfs, off by up to 2^-25 of it: 2^-25 p_max sum_j |v_j|.
-  An fp16 output below 2^-14 is off by 2^-25.
-* lse: 2^-18 (|s| + 16) / 16 of fp32 arithmetic.
-* rows of the importance: u of the value, 2^-18 (|s| + 16) for the exponentials, 2^-25.
+* A logit is a sum of 128 products that are exact in fp32.  Every addition of it is off by at most 2^-23 (a unit of the last place: a matrix
+  instruction may cut off instead of rounding) of a partial sum, which is at most t = scale sum |q_i k_i|: 2^-16 t in all.  As much
+  relative to its value is an exponential off, and 2^-20 more for its own argument, value and sum.
+* output: u sum_j p_j |v_j| for the probabilities rounded before the product with V, u |o| for the output's own rounding, and
+  (2^-16 t + 2^-20) sum_j p_j |v_j| for fp32 arithmetic.  Probabilities below 2^-14 of the largest are subnormal halfs, off by up to 2^-25 of it:
+  2^-25 p_max sum_j |v_j|.  An fp16 output below 2^-14 is off by 2^-25.
+* lse: 2^-16 t + 2^-22 (1 + |lse|).
+* rows of the importance: u of the value, 2^-16 t + 2^-20 of it for the exponentials, 2^-25.
 """
 import math
 
@@ -41,6 +43,11 @@ def starts(lengths, first=0):
     return torch.tensor(np.cumsum([first] + list(lengths)), dtype=torch.int32, device="cuda")
 
 
+def terms(q, k, scale):
+    """The largest sum of a logit's terms without their signs."""
+    return float(torch.einsum("nhd,mhd->hnm", q.abs(), k.abs()).amax()) * scale if k.numel() and q.numel() else 0.0
+
+
 def reference(q, k, v, prefix, causal, scale):
     """One sequence in 64 bits: (out, lse, bound of the output's error, largest |s|)."""
     n, nh = q.shape[0], q.shape[1]
@@ -56,11 +63,11 @@ def reference(q, k, v, prefix, causal, scale):
     lse = torch.logsumexp(s, -1)
     p = torch.exp(s - torch.where(lse.isinf(), 0.0, lse)[..., None])
     out = torch.einsum("hnm,mhd->nhd", p, v)
-    top = torch.where(s.isinf(), 0.0, s.abs()).amax() if s.numel() else torch.zeros((), device="cuda")
+    top = terms(q, k, scale)
     a = torch.einsum("hnm,mhd->nhd", p, v.abs())
     peak = p.amax(-1).T[..., None] if p.shape[-1] else torch.zeros(n, nh, 1, device="cuda", dtype=torch.float64)
-    bound = u * (a + out.abs()) + 2.0 ** -18 * (top + 16) * a + 2.0 ** -25 * (1 + peak * v.abs().sum(0)) * (1 + 2.0 ** -8)
-    return out, lse, bound, float(top)
+    bound = u * (a + out.abs()) + (2.0 ** -16 * top + 2.0 ** -20) * a + 2.0 ** -25 * (1 + peak * v.abs().sum(0)) * (1 + 2.0 ** -8)
+    return out, lse, bound, top
 
 
 def check(ops, q, k, v, q_len, k_len, prefix=None, causal=True, scale=None, call=None):
@@ -74,7 +81,7 @@ def check(ops, q, k, v, q_len, k_len, prefix=None, causal=True, scale=None, call
             assert float(over.max()) <= 1, f"output off by {float(over.max()):.3g} of what it may be (lengths {n}, {m})"
             got, none = lse[:, a:a + n].double(), l.isinf()
             assert torch.equal(got.isinf(), none) and bool((got[none] < 0).all())
-            assert float((got - l)[~none].abs().max() if bool((~none).any()) else 0) <= 2.0 ** -18 * (top + 16) / 16
+            assert bool(((got - l).abs() <= 2.0 ** -16 * top + 2.0 ** -22 * (1 + l.abs()))[~none].all())
             assert bool((out[a:a + n].transpose(0, 1)[none] == 0).all())
         a, b = a + n, b + m
     return out, lse
@@ -304,7 +311,8 @@ def test_importance(ops, heads, rows):
             for n, m in zip(q_len, k_len):
                 want = importance_reference(q[a:a + n], k[b:b + m], lse[:, a:a + n], rows, causal)
                 err = (got[:, b:b + m].double() - want).abs()
-                assert bool((err <= (2.0 ** -11 + 2.0 ** -18 * 24) * want + 2.0 ** -25).all())
+                top = terms(q[a:a + n].double(), k[b:b + m].double().repeat_interleave(nh // nkv, 1), D ** -0.5)
+                assert bool((err <= (2.0 ** -11 + 2.0 ** -16 * top + 2.0 ** -20) * want + 2.0 ** -25).all())
                 a, b = a + n, b + m
 
 
@@ -343,14 +351,14 @@ def check_prefix(ops, q, cache, prefix, group=32, strategy="uniform_group", call
     V = torch.cat((prefix[1].double().transpose(0, 1).expand(B, -1, -1, -1), V), 2).repeat_interleave(rep, 1)
     s = torch.matmul(q.double(), K.transpose(2, 3)) * D ** -0.5
     p = torch.softmax(s, -1)
-    out, a, top = torch.matmul(p, V), torch.matmul(p, V.abs()), float(s.abs().max())
+    out, a, top = torch.matmul(p, V), torch.matmul(p, V.abs()), float(torch.matmul(q.double().abs(), K.abs().transpose(2, 3)).max()) * D ** -0.5
     own = p[..., P:].sum(-1, keepdim=True)
     lost = 2.0 ** -25 * (1 + own * V[:, :, P:].abs().sum(2, keepdim=True) + p.amax(-1, keepdim=True) * V.abs().sum(2, keepdim=True))
-    over = (o.double() - out).abs() / (2.0 ** -11 * (a + out.abs()) + 2.0 ** -18 * (top + 16) * a + lost)
+    over = (o.double() - out).abs() / (2.0 ** -11 * (a + out.abs()) + (2.0 ** -16 * top + 2.0 ** -20) * a + lost)
     assert w.shape == (B, q.shape[1], 1, L) and w.dtype == o.dtype == torch.float16 and o.shape == q.shape
     assert float(over.max()) <= 1, f"output off by {float(over.max()):.3g} of what it may be"
     err = (w.double() - p[..., P:]).abs()
-    assert bool((err <= (2.0 ** -11 + 2.0 ** -18 * (top + 16)) * p[..., P:] + 2.0 ** -25).all())
+    assert bool((err <= (2.0 ** -11 + 2.0 ** -16 * top + 2.0 ** -20) * p[..., P:] + 2.0 ** -25).all())
     return w, o
 
 

@@ -111,7 +111,7 @@ def good_prompt():
     ("nh_q", 1 << 17, "too many heads"), ("n_seqs", -1, "negative"), ("total_q", -1, "negative"), ("prefix_len", -1, "negative"),
     ("total_k", 1 << 30, "too many"), ("n_seqs", 1 << 24, "too many"), ("scale", 0.0, "scale"), ("scale", float("nan"), "scale"),
     ("q", None, "null"), ("k", None, "null"), ("v", None, "null"), ("prefix_len", 3, "null"), ("q_starts", None, "starts"),
-    ("k_starts", 2, "starts"), ("q", 8 + (1 << 20), "16-byte"), ("k_token", 12, "multiples of 8"), ("v_head", -8, "multiples of 8"),
+    ("k_starts", 2, "starts"), ("q", 8 + (1 << 20), "16-byte"), ("k_token", 12, "multiples of 8"), ("v_head", -8, "multiples of 8"), ("k_head", 0, "multiples of 8"),
 ])
 def test_c_abi_refuses_prompts(field, value, text):
     p = good_prompt()
