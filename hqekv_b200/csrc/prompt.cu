@@ -40,53 +40,59 @@ constexpr int PROMPT_THREADS = 384;
 constexpr unsigned TMEM_COLUMNS = 512;
 constexpr float RESCALE_AT = 8.f;                        // powers of two that P may exceed 1 by
 
+struct PromptWork {   // a block of a sequence, and where the sequence's queries and keys are
+  int q0, lq, k0, lk, tile, found;
+};
 struct PromptShared {
   unsigned long long q_full, kv_full[KV_STAGES], kv_empty[KV_STAGES], v_raw[KV_STAGES];
   unsigned long long s_full[2], p_first[2], p_rest[2], o_full[2], drained;
   uint32_t tmem;
   int stop, odd_values;
-  int q0, lq, k0, lk, tile, found;
+  PromptWork work;
 };
 constexpr size_t PROMPT_SMEM = 1024 + (2 + KV_STAGES) * static_cast<size_t>(TILE_BYTES) + sizeof(PromptShared);
 static_assert(PROMPT_SMEM <= 227 * 1024, "one CTA per SM");
 
 static __device__ unsigned g_waits_expired;
 
-// What a CTA works on: the t-th block of 256 / group tokens of all sequences (the last block of a sequence, which sees the most
-// keys, first).  One warp.
-__device__ __forceinline__ void find_block(const PromptArgs& A, int t, int tokens, int lane, PromptShared& sh) {
-  if (A.n_seqs == 0) {   // a single sequence without keys of its own
-    if (lane == 0) sh.q0 = 0, sh.lq = A.total_q, sh.k0 = 0, sh.lk = 0, sh.tile = t, sh.found = 1;
-    return;
-  }
+// The t-th block of `tokens` queries or keys of all sequences (`starts` says whose), the last block of a sequence first: in a causal
+// prompt it sees the most keys.  Lane `first` of the warp's result holds it; -1: there are not as many.
+struct Block {
+  int lane, seq, tile;
+};
+__device__ __forceinline__ Block find_block(const int* starts, int total, int n_seqs, int t, int tokens, int lane) {
   int before = 0;
-  for (int s0 = 0; s0 < A.n_seqs; s0 += 32) {
+  for (int s0 = 0; s0 < n_seqs; s0 += 32) {
     const int s = s0 + lane;
-    int q0 = 0, lq = 0;
-    if (s < A.n_seqs) {
-      q0 = start_of(A.q_starts, s, A.total_q);
-      lq = max(start_of(A.q_starts, s + 1, A.total_q) - q0, 0);
-    }
-    const int blocks = (lq + tokens - 1) / tokens;
-    int sum = blocks;
+    const int length = s < n_seqs ? max(start_of(starts, s + 1, total) - start_of(starts, s, total), 0) : 0;
+    int sum = (length + tokens - 1) / tokens;
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
       const int up = __shfl_up_sync(0xffffffffu, sum, d);
       if (lane >= d) sum += up;
     }
     const unsigned past = __ballot_sync(0xffffffffu, t < before + sum);
-    if (past) {
-      if (lane == __ffs(past) - 1) {
-        sh.q0 = q0, sh.lq = lq;
-        sh.tile = before + sum - 1 - t;
-        sh.k0 = start_of(A.k_starts, s, A.total_k);
-        sh.lk = max(start_of(A.k_starts, s + 1, A.total_k) - sh.k0, 0);
-        sh.found = 1;
-      }
-      return;
-    }
+    if (past) return {__ffs(past) - 1, s, before + sum - 1 - t};
     before += __shfl_sync(0xffffffffu, sum, 31);
   }
+  return {-1, 0, 0};
+}
+// What the CTA works on, into its shared memory.
+__device__ __forceinline__ void find_work(const PromptArgs& A, const int* starts, int total, int t, int tokens, int lane, PromptWork& w) {
+  if (lane == 0) w.found = 0;
+  __syncwarp();
+  if (A.n_seqs == 0) {   // a single sequence without keys of its own
+    if (lane == 0) w.q0 = 0, w.lq = A.total_q, w.k0 = 0, w.lk = 0, w.tile = t, w.found = 1;
+    return;
+  }
+  const Block b = find_block(starts, total, A.n_seqs, t, tokens, lane);
+  if (lane != b.lane) return;
+  w.q0 = start_of(A.q_starts, b.seq, A.total_q);
+  w.lq = max(start_of(A.q_starts, b.seq + 1, A.total_q) - w.q0, 0);
+  w.k0 = start_of(A.k_starts, b.seq, A.total_k);
+  w.lk = max(start_of(A.k_starts, b.seq + 1, A.total_k) - w.k0, 0);
+  w.tile = b.tile;
+  w.found = 1;
 }
 
 // own keys that query i of its sequence sees
@@ -111,12 +117,10 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1) prompt_kernel(const __grid_
   const int groups = A.nh_q / A.group;                       // head groups of all kv heads
   const int t = blockIdx.x / groups, head0 = (blockIdx.x - t * groups) * A.group, kv = head0 / (A.nh_q / A.nh_kv);
   const int half = TILE / A.group, tokens = 2 * half;        // tokens per row tile and CTA
-  if (threadIdx.x == 0) sh.found = 0;
-  __syncwarp();
-  if (warp == 0) find_block(A, t, tokens, lane, sh);
+  if (warp == 0) find_work(A, A.q_starts, A.total_q, t, tokens, lane, sh.work);
   __syncthreads();
-  if (!sh.found) return;
-  const int q0 = sh.q0, lq = sh.lq, k0 = sh.k0, lk = sh.lk, i0 = sh.tile * tokens;   // i0: the CTA's first query in its sequence
+  if (!sh.work.found) return;
+  const int q0 = sh.work.q0, lq = sh.work.lq, k0 = sh.work.k0, lk = sh.work.lk, i0 = sh.work.tile * tokens;   // i0: the CTA's first query in its sequence
   // tiles of keys: those of the prefix, then the own ones up to the last that a row tile sees; this CTA's are [lo, hi[a])
   const int before = (A.prefix_len + TILE - 1) / TILE;
   const int seen_first = keys_seen(A, i0, lq, lk), seen_last = keys_seen(A, min(i0 + tokens, lq) - 1, lq, lk);
@@ -460,34 +464,163 @@ __global__ void __launch_bounds__(256) prompt_join_kernel(const PromptArgs A, in
   if (lane == 0) A.lse[static_cast<int64_t>(head) * A.total_q + token] = l == 0.f ? -INFINITY : (ref + log2f(l)) * 0.6931471805599453f;
 }
 
-// A thread per key, the sums over the heads in shared memory.
-constexpr int IMP_KEYS = 64;
-template <typename T>
-__global__ void __launch_bounds__(IMP_KEYS) prompt_importance_kernel(const PromptArgs A, const float* lse, int rows, __half* out) {
-  extern __shared__ float acc[];   // [rows][IMP_KEYS]
-  const int64_t key = static_cast<int64_t>(blockIdx.x) * IMP_KEYS + threadIdx.x;
-  if (key >= A.total_k) return;
-  for (int r = 0; r < rows; ++r) acc[r * IMP_KEYS + threadIdx.x] = 0.f;
-  int s = 0;
-  while (s < A.n_seqs && start_of(A.k_starts, s + 1, A.total_k) <= key) ++s;
-  const bool in = s < A.n_seqs && start_of(A.k_starts, s, A.total_k) <= key;
-  if (!in) return;
-  const int k0 = start_of(A.k_starts, s, A.total_k), k1 = start_of(A.k_starts, s + 1, A.total_k);
-  const int q0 = start_of(A.q_starts, s, A.total_q), q1 = start_of(A.q_starts, s + 1, A.total_q);
-  const int t = min(rows, max(q1 - q0, 0)), rep = A.nh_q / A.nh_kv;
-  for (int kv = 0; kv < A.nh_kv; ++kv) {
-    const T* k = static_cast<const T*>(A.k) + key * A.k_token + kv * A.k_head;
-    for (int h = kv * rep; h < (kv + 1) * rep; ++h)
-      for (int r = 0; r < t; ++r) {
-        const int i = q1 - t + r;
-        if (A.causal && key - k0 > i + (k1 - k0) - q1) continue;
-        const T* q = static_cast<const T*>(A.q) + i * A.q_token + h * A.q_head;
-        float x = 0.f;
-        for (int d = 0; d < 128; ++d) x = fmaf(to_float(q[d]), to_float(k[d]), x);
-        acc[r * IMP_KEYS + threadIdx.x] += exp2f(x * A.scale_log2 - lse[static_cast<int64_t>(h) * A.total_q + i] * 1.4426950408889634f);
-      }
+// ------------------------------------------------------------------------------------------------
+// Importance
+// ------------------------------------------------------------------------------------------------
+// A CTA takes a tile of keys of one sequence and all heads, HB query heads of a kv head at a time: S^T = K Q^T with the keys as the
+// matrix's rows, so that a thread holds all queries and heads of its key and the sum over the heads needs no other thread.
+//   warps 0-3, 4-7   exponentials and sums, a key per thread, every other eight columns (column = query * HB + head) each
+//   warp 8           matrix products;  warp 9  copies (K of a kv head and the last queries of the HB heads)
+constexpr int IMP_THREADS = 320, IMP_COLUMNS = 128;   // columns: most per product
+struct ImportanceShared {
+  unsigned long long full[4], empty[4], s_full[2], s_empty[2], drained;
+  uint32_t tmem;
+  int stop;
+  PromptWork work;
+  alignas(16) float lse[2][IMP_COLUMNS];
+};
+struct ImportanceShape {
+  int rows, keys, columns, stages;   // keys per tile; columns: rows * HB in whole 16
+};
+__host__ __device__ constexpr int imp_stage_bytes(const ImportanceShape& g) { return TILE_BYTES + g.columns * 256; }
+static size_t imp_smem(const ImportanceShape& g) {
+  return 1024 + g.stages * static_cast<size_t>(imp_stage_bytes(g)) + sizeof(float) * g.rows * TILE + sizeof(ImportanceShared);
+}
+
+template <bool BF16, int HB>
+__global__ void __launch_bounds__(IMP_THREADS) importance_kernel(const __grid_constant__ PromptArgs A, const __grid_constant__ PromptMaps M,
+                                                                 const ImportanceShape G, const float* lse, __half* out) {
+  extern __shared__ unsigned char raw[];
+  unsigned char* const tiles = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  const int stage_bytes = imp_stage_bytes(G);
+  float* const acc = reinterpret_cast<float*>(tiles + G.stages * stage_bytes);   // [rows][key]
+  ImportanceShared& sh = *reinterpret_cast<ImportanceShared*>(acc + G.rows * TILE);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (warp == 0) find_work(A, A.k_starts, A.total_k, blockIdx.x, G.keys, lane, sh.work);
+  __syncthreads();
+  if (!sh.work.found) return;
+  const int q0 = sh.work.q0, lq = sh.work.lq, k0 = sh.work.k0, lk = sh.work.lk, j0 = sh.work.tile * G.keys;
+  const int t = min(G.rows, lq), first = q0 + lq - t;   // the queries
+  const int per_kv = A.nh_q / A.nh_kv / HB, items = t > 0 ? A.nh_kv * per_kv : 0;
+  volatile int* const stop = &sh.stop;
+  if (warp == 8) tmem_alloc(smem_u32(&sh.tmem), 2 * IMP_COLUMNS);
+  if (threadIdx.x == 0) {
+    sh.stop = 0;
+    bar_init(smem_u32(&sh.drained), 1);
+    for (int i = 0; i < 4; ++i) {
+      bar_init(smem_u32(&sh.full[i]), 1);
+      bar_init(smem_u32(&sh.empty[i]), 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      bar_init(smem_u32(&sh.s_full[i]), 1);
+      bar_init(smem_u32(&sh.s_empty[i]), 8);
+    }
+    bar_init_fence();
   }
-  for (int r = 0; r < rows; ++r) out[r * A.total_k + key] = __float2half_rn(acc[r * IMP_KEYS + threadIdx.x]);
+  fence_before();
+  __syncthreads();
+  fence_after();
+  const uint32_t tmem = sh.tmem;
+  if (warp < 8) {
+    const int side = warp >> 2, key = threadIdx.x & 127, j = j0 + key;
+    // the first of the t queries that sees this key
+    const int sees = A.causal ? j - (lk - t) : 0;
+    for (int r = side; r < G.rows; r += 2) acc[r * TILE + key] = 0.f;
+    const float scale = A.scale_log2;
+    const int column = threadIdx.x & 127, col_row = column / HB, col_head = column % HB;
+    auto denominator = [&](int item) {   // of the column that this thread looks after: log2, 0 where there is none
+      if (item >= items || col_row >= t) return 0.f;
+      return 1.4426950408889634f * __ldg(lse + static_cast<int64_t>(item * HB + col_head) * A.total_q + first + col_row);
+    };
+    bool ok = true;
+    float next = denominator(0);
+#pragma unroll 1
+    for (int item = 0; item < items; ++item) {
+      float* const den = sh.lse[item & 1];
+      if (side == 0) den[column] = next;
+      asm volatile("bar.sync 1, 256;" ::: "memory");   // (a buffer is written again two items later: everyone has passed the barrier between)
+      next = denominator(item + 1);
+      ok = ok && __all_sync(0xffffffffu, bar_wait(smem_u32(&sh.s_full[item & 1]), item >> 1 & 1, stop));
+      if (!ok) continue;   // (every warp comes to every barrier)
+      fence_after();
+      const uint32_t at = tmem + (static_cast<uint32_t>(warp & 3) << 21) + (item & 1) * IMP_COLUMNS;
+#pragma unroll 1
+      for (int c = 8 * side; c < G.columns; c += 16) {
+        uint32_t s[8];
+        tmem_load8(at + c, s);
+        const float4 d0 = *reinterpret_cast<const float4*>(den + c), d1 = *reinterpret_cast<const float4*>(den + c + 4);
+        const float d[8] = {d0.x, d0.y, d0.z, d0.w, d1.x, d1.y, d1.z, d1.w};
+        wait_loads();
+#pragma unroll
+        for (int k = 0; k < 8; k += HB) {
+          float sum = 0.f;
+#pragma unroll
+          for (int h = 0; h < HB; ++h) sum += exp2_approx(fmaf(__uint_as_float(s[k + h]), scale, -d[k + h]));
+          const int r = (c + k) / HB;
+          if (r < t && r >= sees) acc[r * TILE + key] += sum;
+        }
+      }
+      fence_before();
+      __syncwarp();
+      if (lane == 0) bar_arrive(smem_u32(&sh.s_empty[item & 1]));
+    }
+    asm volatile("bar.sync 1, 256;" ::: "memory");
+    if (ok && j < lk && key < G.keys)
+      for (int r = side; r < G.rows; r += 2) out[static_cast<int64_t>(r) * A.total_k + k0 + j] = __float2half_rn(acc[r * TILE + key]);
+  } else if (warp == 8) {
+    if (lane == 0) {
+      const uint32_t kind = mma_kind(BF16, TILE, G.columns, false), tiles_at = smem_u32(tiles), q_half = G.columns * 128;
+      bool ok = true;
+      int stage = 0;
+      unsigned phase = 0;
+#pragma unroll 1
+      for (int item = 0; item < items; ++item) {
+        if (!(ok = bar_wait(smem_u32(&sh.full[stage]), phase, stop) &&
+                   bar_wait(smem_u32(&sh.s_empty[item & 1]), (item >> 1 & 1) ^ 1, stop))) break;
+        fence_after();
+        const uint32_t k_at = tiles_at + stage * stage_bytes, q_at = k_at + TILE_BYTES;
+#pragma unroll
+        for (int c = 0; c < 8; ++c)
+          mma_shared(tmem + (item & 1) * IMP_COLUMNS, operand(k_at + (c >> 2) * (TILE_BYTES / 2) + (c & 3) * 32, 16),
+                     operand(q_at + (c >> 2) * q_half + (c & 3) * 32, 16), kind, c > 0);
+        mma_commit(smem_u32(&sh.s_full[item & 1]));
+        mma_commit(smem_u32(&sh.empty[stage]));
+        if (++stage == G.stages) stage = 0, phase ^= 1;
+      }
+      if (!ok) {   // products in flight end before the CTA does
+        mma_commit(smem_u32(&sh.drained));
+        for (int k = 0; k < WAIT_TRIES && !bar_try(smem_u32(&sh.drained), 0); ++k) {
+        }
+      }
+    }
+  } else if (lane == 0) {
+    const uint32_t tiles_at = smem_u32(tiles);
+    const unsigned bytes = 256u * (G.keys + G.rows * HB);
+    bool ok = true;
+    int stage = 0, item = 0;
+    unsigned phase = 1;
+#pragma unroll 1
+    for (; item < items; ++item) {
+      if (!(ok = bar_wait(smem_u32(&sh.empty[stage]), phase, stop))) break;
+      const uint32_t k_at = tiles_at + stage * stage_bytes, q_at = k_at + TILE_BYTES, bar = smem_u32(&sh.full[stage]);
+      bar_expect(bar, bytes);
+      for (int c = 0; c < 2; ++c) {
+        copy_box(k_at + c * (TILE_BYTES / 2), &M.k, 64 * c, item / per_kv, k0 + j0, bar);
+        copy_box(q_at + c * G.columns * 128, &M.q, 64 * c, item * HB, first, bar);
+      }
+      if (++stage == G.stages) stage = 0, phase ^= 1;
+    }
+    if (!ok)   // copies in flight land before the CTA ends
+      for (int i = max(0, item - G.stages); i < item; ++i)
+        for (int k = 0; k < WAIT_TRIES && !bar_try(smem_u32(&sh.full[i % G.stages]), i / G.stages & 1); ++k) {
+        }
+  }
+  __syncwarp();
+  fence_before();
+  __syncthreads();
+  fence_after();
+  if (warp == 8) tmem_free(tmem, 2 * IMP_COLUMNS);
+  if (threadIdx.x == 0 && *stop) atomicAdd(&g_waits_expired, 1u);
 }
 
 // ------------------------------------------------------------------------------------------------
@@ -605,6 +738,44 @@ static int launch_prompt(const PromptArgs& A, int splits, cudaStream_t st) {
   return HQKV_OK;
 }
 
+template <bool BF16, int HB>
+static int launch_importance(const PromptArgs& A, const PromptMaps& M, const ImportanceShape& G, const float* lse, __half* out, cudaStream_t st) {
+  static bool opted_in[64] = {};   // per device
+  int dev = 0;
+  HQKV_CUDA(cudaGetDevice(&dev));
+  if (dev < 0 || dev >= 64 || !opted_in[dev]) {
+    HQKV_CUDA(cudaFuncSetAttribute(importance_kernel<BF16, HB>, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024));
+    if (dev >= 0 && dev < 64) opted_in[dev] = true;
+  }
+  const int64_t n = max(1, min(A.n_seqs, A.total_k)), blocks = (A.total_k + n * (G.keys - 1)) / G.keys;
+  importance_kernel<BF16, HB><<<static_cast<unsigned>(blocks), IMP_THREADS, imp_smem(G), st>>>(A, M, G, lse, out);
+  HQKV_LAUNCH_CHECK("importance");
+  return HQKV_OK;
+}
+
+static int launch_importance(const PromptArgs& A, const float* lse, int rows, __half* out, cudaStream_t st) {
+  int hb = 1;   // query heads per product
+  while (hb < 8 && A.nh_q / A.nh_kv % (2 * hb) == 0 && 2 * hb * rows <= IMP_COLUMNS) hb *= 2;
+  ImportanceShape G;
+  G.rows = rows;
+  G.columns = (rows * hb + 15) / 16 * 16;
+  // as many tiles as two CTAs per SM take at once, of 64 to 128 keys
+  const int64_t waves = ceil_div(A.total_k, 296 * TILE), keys = ceil_div(ceil_div(A.total_k, 296 * waves), 8) * 8;
+  G.keys = static_cast<int>(max(int64_t{64}, min(int64_t{TILE}, keys)));
+  G.stages = 4;
+  while (G.stages > 2 && imp_smem(G) > 113 * 1024) --G.stages;
+  PromptMaps M = {};
+  if (A.total_q > 0)
+    if (int rc = tensor_map(&M.q, A.q, A.bf16, A.total_q, A.nh_q, A.q_token, A.q_head, hb, rows)) return rc;
+  if (int rc = tensor_map(&M.k, A.k, A.bf16, A.total_k, A.nh_kv, A.k_token, A.k_head, 1, G.keys)) return rc;
+  switch (hb) {
+    case 1: return A.bf16 ? launch_importance<true, 1>(A, M, G, lse, out, st) : launch_importance<false, 1>(A, M, G, lse, out, st);
+    case 2: return A.bf16 ? launch_importance<true, 2>(A, M, G, lse, out, st) : launch_importance<false, 2>(A, M, G, lse, out, st);
+    case 4: return A.bf16 ? launch_importance<true, 4>(A, M, G, lse, out, st) : launch_importance<false, 4>(A, M, G, lse, out, st);
+    default: return A.bf16 ? launch_importance<true, 8>(A, M, G, lse, out, st) : launch_importance<false, 8>(A, M, G, lse, out, st);
+  }
+}
+
 int prefix_splits(const hqkv_prompt_t* p) {
   PromptArgs A;
   A.total_q = static_cast<int>(p->total_q), A.total_k = 0, A.n_seqs = 0, A.prefix_len = static_cast<int>(p->prefix_len);
@@ -673,11 +844,5 @@ extern "C" int hqkv_prompt_importance(const hqkv_prompt_t* prompt_host, const fl
   if (A.total_k == 0 || A.n_seqs == 0) return HQKV_OK;
   HQKV_REQUIRE(out_f16 && aligned(out_f16, 2), "prompt_importance: the output is null or misaligned");
   HQKV_REQUIRE(A.total_q == 0 || (lse && aligned(lse, 4)), "prompt_importance: lse is null or misaligned");
-  const unsigned grid = static_cast<unsigned>(ceil_div(A.total_k, IMP_KEYS));
-  const size_t smem = sizeof(float) * rows * IMP_KEYS;
-  cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (A.bf16) prompt_importance_kernel<__nv_bfloat16><<<grid, IMP_KEYS, smem, st>>>(A, lse, rows, static_cast<__half*>(out_f16));
-  else prompt_importance_kernel<__half><<<grid, IMP_KEYS, smem, st>>>(A, lse, rows, static_cast<__half*>(out_f16));
-  HQKV_LAUNCH_CHECK("prompt_importance");
-  return HQKV_OK;
+  return launch_importance(A, lse, rows, static_cast<__half*>(out_f16), static_cast<cudaStream_t>(stream));
 }
