@@ -163,7 +163,8 @@ def _load_host():
                   ("hqkv_decode_workspace_bytes", "hqkv_decode_attention", "hqkv_decode_attention_headsum",
                    "hqkv_quantize_pack", "hqkv_dequantize_unpack", "hqkv_head_sum", "hqkv_token_importance", "hqkv_block_rank",
                    "hqkv_flush_workspace_bytes", "hqkv_flush_prepare", "hqkv_flush_join", "hqkv_flush_tiers_beside",
-                   "hqkv_flush_finish", "hqkv_flush_evict")],
+                   "hqkv_flush_finish", "hqkv_flush_evict", "hqkv_prompt_workspace_bytes", "hqkv_prompt_attention",
+                   "hqkv_prompt_importance", "hqkv_decode_prefix_workspace_bytes", "hqkv_decode_attention_prefix")],
                 decode_workspace)
     return module
 

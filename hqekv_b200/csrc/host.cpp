@@ -11,6 +11,7 @@
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <ATen/ATen.h>
+#include <c10/core/GradMode.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 
@@ -42,6 +43,11 @@ struct Lib {
   decltype(&hqkv_flush_tiers_beside) flush_tiers_beside;
   decltype(&hqkv_flush_finish) flush_finish;
   decltype(&hqkv_flush_evict) flush_evict;
+  decltype(&hqkv_prompt_workspace_bytes) prompt_workspace_bytes;
+  decltype(&hqkv_prompt_attention) prompt_attention;
+  decltype(&hqkv_prompt_importance) prompt_importance;
+  decltype(&hqkv_decode_prefix_workspace_bytes) decode_prefix_workspace_bytes;
+  decltype(&hqkv_decode_attention_prefix) decode_attention_prefix;
 } L;
 PyObject* g_workspace_fn = nullptr;  // _lib.decode_workspace(device, bytes, stream): owns the scratch buffers
 bool g_bound = false;
@@ -67,10 +73,10 @@ inline void* ptr(const at::Tensor* t) { return t ? t->data_ptr() : nullptr; }
 PyObject* none() { Py_RETURN_NONE; }
 
 PyObject* bind(PyObject*, PyObject* args) {
-  unsigned long long a[14];
+  unsigned long long a[19];
   PyObject* fn;
-  if (!PyArg_ParseTuple(args, "KKKKKKKKKKKKKKO", &a[0], &a[1], &a[2], &a[3], &a[4], &a[5], &a[6], &a[7], &a[8], &a[9], &a[10],
-                        &a[11], &a[12], &a[13], &fn))
+  if (!PyArg_ParseTuple(args, "KKKKKKKKKKKKKKKKKKKO", &a[0], &a[1], &a[2], &a[3], &a[4], &a[5], &a[6], &a[7], &a[8], &a[9], &a[10],
+                        &a[11], &a[12], &a[13], &a[14], &a[15], &a[16], &a[17], &a[18], &fn))
     return nullptr;
   int i = 0;
   auto take = [&](auto& f) { f = reinterpret_cast<std::decay_t<decltype(f)>>(a[i++]); };
@@ -88,6 +94,11 @@ PyObject* bind(PyObject*, PyObject* args) {
   take(L.flush_tiers_beside);
   take(L.flush_finish);
   take(L.flush_evict);
+  take(L.prompt_workspace_bytes);
+  take(L.prompt_attention);
+  take(L.prompt_importance);
+  take(L.decode_prefix_workspace_bytes);
+  take(L.decode_attention_prefix);
   Py_INCREF(fn);
   Py_XDECREF(g_workspace_fn);
   g_workspace_fn = fn;
@@ -152,21 +163,19 @@ PyObject* pack(std::initializer_list<at::Tensor> ts) {
   return out;
 }
 
-// decode(q, cache, block_size, group_size, low_codec, head_sum_row | None) -> (attn_weights, attn_output) | None
-PyObject* decode(PyObject*, PyObject* const* a, Py_ssize_t na) {
-  HANDLE_TH_ERRORS
-  if (!g_bound || na != 6 || !THPVariable_Check(a[0]) || !PyTuple_Check(a[1]) || PyTuple_GET_SIZE(a[1]) != kSlots)
-    return none();
-  const at::Tensor& q_in = THPVariable_Unpack(a[0]);
-  if (!q_in.is_cuda() || q_in.scalar_type() != at::kHalf || q_in.dim() != 4 || q_in.size(2) != 1) return none();
-  PyObject* cache = a[1];
-  hqkv_cache_desc_t d = {};
-  d.group_k = static_cast<int32_t>(PyLong_AsLong(a[2]));
-  d.group_v = static_cast<int32_t>(PyLong_AsLong(a[3]));
-  const int low_codec = static_cast<int>(PyLong_AsLong(a[4]));
+// What the decode calls have in common: the library's description of a cache tuple for these queries, and its length.
+bool describe_cache(PyObject* q_obj, PyObject* cache, PyObject* block_size, PyObject* group_size, PyObject* codec, hqkv_cache_desc_t& d,
+                    int64_t& len) {
+  if (!g_bound || !THPVariable_Check(q_obj) || !PyTuple_Check(cache) || PyTuple_GET_SIZE(cache) != kSlots) return false;
+  const at::Tensor& q_in = THPVariable_Unpack(q_obj);
+  if (!q_in.is_cuda() || q_in.scalar_type() != at::kHalf || q_in.dim() != 4 || q_in.size(2) != 1) return false;
+  d = {};
+  d.group_k = static_cast<int32_t>(PyLong_AsLong(block_size));
+  d.group_v = static_cast<int32_t>(PyLong_AsLong(group_size));
+  const int low_codec = static_cast<int>(PyLong_AsLong(codec));
   if (PyErr_Occurred()) {
     PyErr_Clear();
-    return none();
+    return false;
   }
   int64_t B = 0, H = 0, D = 0, n_k = 0;
   const at::Tensor* where = nullptr;
@@ -175,12 +184,12 @@ PyObject* decode(PyObject*, PyObject* const* a, Py_ssize_t na) {
     const int parts = t == 0 ? 2 : 4;
     for (int i = 0; i < parts; ++i)
       if (!slot(PyTuple_GET_ITEM(cache, kSlotK[t] + i), &k[i]) || !slot(PyTuple_GET_ITEM(cache, kSlotV[t] + i), &v[i]))
-        return none();
+        return false;
     hqkv_tier_t& T = d.tier[t];
     T.bits = kBits[t];
     T.codec = kBits[t] == 1 ? low_codec : 0;
     for (const at::Tensor* idx : {k[1], v[1]})
-      if (idx && idx->scalar_type() != at::kLong) return none();
+      if (idx && idx->scalar_type() != at::kLong) return false;
     T.n_k = k[1] ? static_cast<int32_t>(k[1]->numel()) : 0;
     T.n_v = v[1] ? static_cast<int32_t>(v[1]->numel()) : 0;
     n_k += T.n_k;
@@ -193,7 +202,7 @@ PyObject* decode(PyObject*, PyObject* const* a, Py_ssize_t na) {
     T.v_scale = ptr(v[2]);
     T.v_zero = ptr(v[3]);
     if (v[0]) {
-      if (v[0]->dim() != 4) return none();
+      if (v[0]->dim() != 4) return false;
       B = v[0]->size(0);
       H = v[0]->size(1);
       D = v[0]->size(3) * (t == 0 ? 1 : 32 / kBits[t]);
@@ -201,24 +210,35 @@ PyObject* decode(PyObject*, PyObject* const* a, Py_ssize_t na) {
     }
   }
   const at::Tensor *nk, *nv;
-  if (!slot(PyTuple_GET_ITEM(cache, kSlotNewK), &nk) || !slot(PyTuple_GET_ITEM(cache, kSlotNewV), &nv)) return none();
+  if (!slot(PyTuple_GET_ITEM(cache, kSlotNewK), &nk) || !slot(PyTuple_GET_ITEM(cache, kSlotNewV), &nv)) return false;
   if (nv) {
-    if (nv->dim() != 4 || (where && (nv->size(0) != B || nv->size(1) != H || nv->size(3) != D))) return none();
+    if (nv->dim() != 4 || (where && (nv->size(0) != B || nv->size(1) != H || nv->size(3) != D))) return false;
     B = nv->size(0);
     H = nv->size(1);
     D = nv->size(3);
     d.n_new = static_cast<int32_t>(nv->size(2));
     where = nv;
   }
-  if (!where || where->device() != q_in.device() || q_in.size(0) != B || q_in.size(3) != D) return none();
+  if (!where || where->device() != q_in.device() || q_in.size(0) != B || q_in.size(3) != D) return false;
   d.new_k = ptr(nk);
   d.new_v = ptr(nv);
-  const int64_t nh_q = q_in.size(1), len = n_k + d.n_new;
+  const int64_t nh_q = q_in.size(1);
+  len = n_k + d.n_new;
   d.B = static_cast<int32_t>(B);
   d.H = static_cast<int32_t>(H);
   d.D = static_cast<int32_t>(D);
   d.nh_q = static_cast<int32_t>(nh_q);
   d.softmax_scale = static_cast<float>(1.0 / std::sqrt(static_cast<double>(D)));
+  return true;
+}
+
+// decode(q, cache, block_size, group_size, low_codec, head_sum_row | None) -> (attn_weights, attn_output) | None
+PyObject* decode(PyObject*, PyObject* const* a, Py_ssize_t na) {
+  HANDLE_TH_ERRORS
+  hqkv_cache_desc_t d;
+  int64_t len;
+  if (na != 6 || !describe_cache(a[0], a[1], a[2], a[3], a[4], d, len)) return none();
+  const at::Tensor& q_in = THPVariable_Unpack(a[0]);
   void* row = nullptr;
   if (a[5] != Py_None) {
     if (!THPVariable_Check(a[5])) return none();
@@ -235,14 +255,150 @@ PyObject* decode(PyObject*, PyObject* const* a, Py_ssize_t na) {
   size_t ws_bytes;
   if (!scratch(q_in.device().index(), st, need, a[0], &ws, &ws_bytes)) return nullptr;
   const at::Tensor q = q_in.contiguous();
-  at::Tensor weights = at::empty({B, nh_q, 1, len}, q.options());
-  at::Tensor out = at::empty({B, nh_q, 1, D}, q.options());
+  at::Tensor weights = at::empty({d.B, d.nh_q, 1, len}, q.options());
+  at::Tensor out = at::empty({d.B, d.nh_q, 1, d.D}, q.options());
   int rc;
   Py_BEGIN_ALLOW_THREADS
   rc = row ? L.decode_attention_headsum(&d, q.data_ptr(), weights.data_ptr(), out.data_ptr(), row, ws, ws_bytes, st)
            : L.decode_attention(&d, q.data_ptr(), weights.data_ptr(), out.data_ptr(), ws, ws_bytes, st);
   Py_END_ALLOW_THREADS
   return rc ? none() : pack({weights, out});
+  END_HANDLE_TH_ERRORS
+}
+
+// a [tokens, heads, 128] operand that the prompt kernels read where it is
+inline bool packed(const at::Tensor& x) {
+  if (!x.is_cuda() || x.dim() != 3 || x.size(2) != 128 || x.stride(2) != 1 || reinterpret_cast<uintptr_t>(x.data_ptr()) % 16) return false;
+  for (int d = 0; d < 2; ++d)
+    if (x.size(d) > 1 && (x.stride(d) <= 0 || x.stride(d) % 8)) return false;
+  return !(x.requires_grad() && c10::GradMode::is_enabled());
+}
+
+// decode_prefix(q, cache, prefix_k, prefix_v, block_size, group_size, low_codec) -> (attn_weights, attn_output) | None
+PyObject* decode_prefix(PyObject*, PyObject* const* a, Py_ssize_t na) {
+  HANDLE_TH_ERRORS
+  hqkv_cache_desc_t d;
+  int64_t len;
+  if (na != 7 || !THPVariable_Check(a[2]) || !THPVariable_Check(a[3]) || !describe_cache(a[0], a[1], a[4], a[5], a[6], d, len)) return none();
+  const at::Tensor &q = THPVariable_Unpack(a[0]), &pk = THPVariable_Unpack(a[2]), &pv = THPVariable_Unpack(a[3]);
+  for (const at::Tensor* x : {&pk, &pv})
+    if (!packed(*x) || x->scalar_type() != at::kHalf || x->device() != q.device() || x->size(1) != d.H || x->size(2) != d.D ||
+        x->size(0) != pk.size(0) || x->size(0) == 0)
+      return none();
+  if (!q.is_contiguous() || reinterpret_cast<uintptr_t>(q.data_ptr()) % 16 || (q.requires_grad() && c10::GradMode::is_enabled())) return none();
+  const size_t need = L.decode_workspace_bytes(&d), more = L.decode_prefix_workspace_bytes(&d, pk.size(0));
+  if (need == 0 || more == 0) return none();
+  const c10::cuda::OptionalCUDAGuard guard(q.device());
+  const cudaStream_t st = current_stream(q);
+  void* ws;
+  size_t ws_bytes;
+  if (!scratch(q.device().index(), st, need, a[0], &ws, &ws_bytes)) return nullptr;
+  at::Tensor weights = at::empty({d.B, d.nh_q, 1, len}, q.options());
+  at::Tensor out = at::empty({d.B, d.nh_q, 1, d.D}, q.options());
+  at::Tensor parts = at::empty({static_cast<int64_t>(more)}, q.options().dtype(at::kByte));
+  int rc;
+  Py_BEGIN_ALLOW_THREADS
+  rc = L.decode_attention_prefix(&d, q.data_ptr(), pk.data_ptr(), pv.data_ptr(), pk.size(0), pk.stride(0), pk.stride(1), pv.stride(0),
+                                 pv.stride(1), weights.data_ptr(), out.data_ptr(), ws, ws_bytes, parts.data_ptr(), more, st);
+  Py_END_ALLOW_THREADS
+  return rc ? none() : pack({weights, out});
+  END_HANDLE_TH_ERRORS
+}
+
+// the arguments that the prompt operators share: q, k, v | None, seq_starts, kv_starts | None, prefix_k | None, prefix_v | None, causal,
+// scale | None
+bool describe_prompt(PyObject* const* a, hqkv_prompt_t& p) {
+  const at::Tensor* x[7] = {};
+  for (int i = 0; i < 7; ++i) {
+    if (a[i] == Py_None) continue;
+    if (!THPVariable_Check(a[i])) return false;
+    x[i] = &THPVariable_Unpack(a[i]);
+  }
+  const at::Tensor *q = x[0], *k = x[1], *v = x[2], *qs = x[3], *ks = x[4] ? x[4] : x[3], *pk = x[5], *pv = x[6];
+  if (!g_bound || !q || !k || !qs || !pk != !pv || (!x[4] && q->dim() == 3 && k->dim() == 3 && q->size(0) != k->size(0))) return false;
+  const auto type = q->scalar_type();
+  if ((type != at::kHalf && type != at::kBFloat16)) return false;
+  for (const at::Tensor* t : {q, k, v, pk, pv})
+    if (t && (!packed(*t) || t->scalar_type() != type || t->device() != q->device() || (t != q && t->size(1) != k->size(1)))) return false;
+  if ((v && v->size(0) != k->size(0)) || (pk && pk->size(0) != pv->size(0)) || k->size(1) == 0 || q->size(1) == 0 || q->size(1) % k->size(1))
+    return false;
+  for (const at::Tensor* t : {qs, ks})
+    if (t->device() != q->device() || t->scalar_type() != at::kInt || t->dim() != 1 || t->numel() < 1 || t->numel() != qs->numel() ||
+        !t->is_contiguous())
+      return false;
+  const int causal = PyObject_IsTrue(a[7]);
+  const double scale = a[8] == Py_None ? 1.0 / std::sqrt(128.0) : PyFloat_AsDouble(a[8]);
+  if (PyErr_Occurred()) {
+    PyErr_Clear();
+    return false;
+  }
+  p = {};
+  p.dtype = type == at::kHalf ? HQKV_F16 : HQKV_BF16;
+  p.D = 128;
+  p.nh_q = static_cast<int32_t>(q->size(1));
+  p.nh_kv = static_cast<int32_t>(k->size(1));
+  p.n_seqs = static_cast<int32_t>(qs->numel() - 1);
+  p.causal = causal;
+  p.scale = static_cast<float>(scale);
+  p.total_q = q->size(0);
+  p.total_k = k->size(0);
+  auto take = [](const at::Tensor* t, const void*& at, int64_t& token, int64_t& head) {
+    if (t) at = t->data_ptr(), token = t->stride(0), head = t->stride(1);
+  };
+  take(q, p.q, p.q_token, p.q_head);
+  take(k, p.k, p.k_token, p.k_head);
+  take(v, p.v, p.v_token, p.v_head);
+  take(pk, p.prefix_k, p.prefix_k_token, p.prefix_k_head);
+  take(pv, p.prefix_v, p.prefix_v_token, p.prefix_v_head);
+  if (pk) p.prefix_len = pk->size(0);
+  p.q_starts = static_cast<const int32_t*>(qs->data_ptr());
+  p.k_starts = static_cast<const int32_t*>(ks->data_ptr());
+  return true;
+}
+
+// prompt_attention(the nine arguments above) -> (out, lse) | None
+PyObject* prompt_attention(PyObject*, PyObject* const* a, Py_ssize_t na) {
+  HANDLE_TH_ERRORS
+  hqkv_prompt_t p;
+  if (na != 9 || a[2] == Py_None || !describe_prompt(a, p)) return none();
+  const at::Tensor& q = THPVariable_Unpack(a[0]);
+  const c10::cuda::OptionalCUDAGuard guard(q.device());
+  at::Tensor out = at::empty({p.total_q, p.nh_q, p.D}, q.options());
+  at::Tensor lse = at::empty({p.nh_q, p.total_q}, q.options().dtype(at::kFloat)), parts;
+  const size_t need = L.prompt_workspace_bytes(&p);
+  if (need) parts = at::empty({static_cast<int64_t>(need)}, q.options().dtype(at::kByte));
+  const cudaStream_t st = current_stream(q);
+  int rc;
+  Py_BEGIN_ALLOW_THREADS
+  rc = L.prompt_attention(&p, out.data_ptr(), static_cast<float*>(lse.data_ptr()), need ? parts.data_ptr() : nullptr, need, st);
+  Py_END_ALLOW_THREADS
+  return rc ? none() : pack({out, lse});
+  END_HANDLE_TH_ERRORS
+}
+
+// prompt_importance(the nine arguments above, lse, rows) -> rows | None
+PyObject* prompt_importance(PyObject*, PyObject* const* a, Py_ssize_t na) {
+  HANDLE_TH_ERRORS
+  hqkv_prompt_t p;
+  const at::Tensor* lse;
+  if (na != 11 || !describe_prompt(a, p) || !slot(a[9], &lse) || !lse) return none();
+  const int64_t rows = PyLong_AsLong(a[10]);
+  if (PyErr_Occurred()) {
+    PyErr_Clear();
+    return none();
+  }
+  const at::Tensor& q = THPVariable_Unpack(a[0]);
+  if (lse->scalar_type() != at::kFloat || lse->device() != q.device() || lse->dim() != 2 || lse->size(0) != p.nh_q || lse->size(1) != p.total_q ||
+      rows < 1 || rows > HQKV_IMPORTANCE_ROWS)
+    return none();
+  const c10::cuda::OptionalCUDAGuard guard(q.device());
+  at::Tensor out = at::empty({rows, p.total_k}, q.options().dtype(at::kHalf));
+  const cudaStream_t st = current_stream(q);
+  int rc;
+  Py_BEGIN_ALLOW_THREADS
+  rc = L.prompt_importance(&p, static_cast<const float*>(lse->data_ptr()), static_cast<int>(rows), out.data_ptr(), st);
+  Py_END_ALLOW_THREADS
+  return rc ? none() : THPVariable_Wrap(out);
   END_HANDLE_TH_ERRORS
 }
 
@@ -585,6 +741,9 @@ PyMethodDef methods[] = {
     {"bind", bind, METH_VARARGS, "addresses of the library's entry points, and the owner of the decode scratch"},
     {"build_id", build_id, METH_NOARGS, "hash of the sources this module was compiled from"},
     {"decode", fast(decode), METH_FASTCALL, nullptr},
+    {"decode_prefix", fast(decode_prefix), METH_FASTCALL, nullptr},
+    {"prompt_attention", fast(prompt_attention), METH_FASTCALL, nullptr},
+    {"prompt_importance", fast(prompt_importance), METH_FASTCALL, nullptr},
     {"quantize_pack", fast(quantize_pack), METH_FASTCALL, nullptr},
     {"dequantize_unpack", fast(dequantize_unpack), METH_FASTCALL, nullptr},
     {"head_sum", fast(head_sum), METH_FASTCALL, nullptr},

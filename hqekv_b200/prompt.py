@@ -13,7 +13,7 @@ import ctypes as C
 
 import torch
 
-from ._lib import Prompt, check, lib, ptr, require_cuda, stream_ptr
+from ._lib import Prompt, check, host, lib, ptr, require_cuda, stream_ptr
 
 HEAD_DIM = 128
 MAX_ROWS = 64   # HQKV_IMPORTANCE_ROWS
@@ -104,6 +104,12 @@ def prompt_attention(q, k, v, seq_starts, kv_starts=None, *, prefix=None, causal
     Rows of queries in no sequence (behind the last start, or before the first) are not written: in ``out`` they stay as they were,
     in results allocated here they are undefined.  What a query does not see has no influence on its output, whatever it holds.  Probabilities are
     rounded to the type of v before the product with it; sums, maxima and the output's accumulator are fp32."""
+    if out is None:
+        pk, pv = prefix or (None, None)
+        done = host.prompt_attention(q, k, v, seq_starts, kv_starts, pk, pv, causal, scale)
+        if done is not None:
+            return done
+    # what the native path does not take as it is: operands to be copied, and everything that is an error
     p, keep = _describe(q, k, v, seq_starts, kv_starts, prefix, causal, scale)
     q = keep[0]
     if out is None:
@@ -128,6 +134,10 @@ def prompt_importance(q, k, lse, seq_starts, kv_starts=None, *, rows=20, causal=
     a result allocated here they are undefined."""
     if isinstance(rows, bool) or not isinstance(rows, int) or not 1 <= rows <= MAX_ROWS:
         raise ValueError(f"rows must be an integer from 1 to {MAX_ROWS}")
+    if out is None:
+        done = host.prompt_importance(q, k, None, seq_starts, kv_starts, None, None, causal, scale, lse, rows)
+        if done is not None:
+            return done
     p, keep = _describe(q, k, None, seq_starts, kv_starts, None, causal, scale)
     q, k = keep[0], keep[1]
     if lse.shape != (q.shape[1], q.shape[0]) or lse.dtype != torch.float32 or lse.device != q.device:

@@ -92,6 +92,9 @@ def qkv_matmul_hqe_prefix(q: torch.Tensor, past_key_value: Tuple, prefix: Tuple[
         raise ValueError("invalid past_key_value")
     low_codec = CODEC_UNIFORM if quant_strategy == "uniform_group" else CODEC_NORMAL
     pk, pv = prefix
+    done = host.decode_prefix(q, past_key_value, pk, pv, block_size, group_size, low_codec)
+    if done is not None:
+        return done
     if q.dtype != torch.float16 or q.dim() != 4 or q.shape[2] != 1:
         raise ValueError("q must be float16 of shape [B, nh_q, 1, head_dim]")
     if torch.is_grad_enabled() and (q.requires_grad or pk.requires_grad or pv.requires_grad):
