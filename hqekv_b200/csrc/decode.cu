@@ -2533,7 +2533,7 @@ extern "C" size_t hqkv_decode_prefix_workspace_bytes(const hqkv_cache_desc_t* ca
   if (build_params(cache_host, P, lay) != HQKV_OK || prefix_len < 1 || prefix_len >= (1ll << 30)) return 0;
   const hqkv_prompt_t p = prefix_of(cache_host, prefix_len);
   size_t o, ml;
-  return join_bytes(cache_host, prefix_splits(&p), &o, &ml);
+  return join_bytes(cache_host, prefix_shares(&p), &o, &ml);
 }
 
 extern "C" int hqkv_decode_attention_prefix(const hqkv_cache_desc_t* cache_host, const void* q, const void* prefix_k, const void* prefix_v,
@@ -2550,14 +2550,14 @@ extern "C" int hqkv_decode_attention_prefix(const hqkv_cache_desc_t* cache_host,
   p.q = q, p.prefix_k = prefix_k, p.prefix_v = prefix_v;
   p.prefix_k_token = k_token, p.prefix_k_head = k_head, p.prefix_v_token = v_token, p.prefix_v_head = v_head;
   JoinParams J = {};
-  J.splits = prefix_splits(&p);
+  J.splits = prefix_shares(&p);
   size_t o, ml;
   const size_t need = join_bytes(cache_host, J.splits, &o, &ml);
   if (prefix_workspace_bytes < need)
     return fail(HQKV_E_WORKSPACE, "decode_prefix: the prefix workspace holds %zu bytes, %zu needed", prefix_workspace_bytes, need);
   unsigned char* pw = static_cast<unsigned char*>(prefix_workspace);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (int rc = prefix_partial(&p, reinterpret_cast<float*>(pw + o), reinterpret_cast<float2*>(pw + ml), J.splits, st)) return rc;
+  if (int rc = prefix_partial(&p, reinterpret_cast<float*>(pw + o), reinterpret_cast<float2*>(pw + ml), st)) return rc;
   if (int rc = decode_launch(cache_host, q, attn_weights, attn_output, workspace, workspace_bytes, 3, hqkv::PeerArgs(), stream, nullptr, nullptr, 0, 0,
                              nullptr, reinterpret_cast<float*>(pw)))
     return rc;

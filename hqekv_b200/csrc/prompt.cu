@@ -26,84 +26,155 @@ __device__ __forceinline__ int start_of(const int* starts, int s, int total) { r
 // ------------------------------------------------------------------------------------------------
 // Attention
 // ------------------------------------------------------------------------------------------------
-// A CTA takes 256 rows of queries - two tiles of 128 rows, a row being a (token, head of the group) - and walks the tiles of 128 keys that
-// any of them sees: first the prefix, then the sequence's own.  One pass, with the running maximum and sum of the softmax.
-//   warps 0-3, 4-7   softmax of the first and second row tile, a row per thread
-//   warp 8           issues the matrix products (one thread)
+// A CTA takes blocks of 256 rows of queries - two tiles of 128 rows, a row being a (token, head of the group) - and walks the tiles of 128
+// keys that any of them sees: first the prefix, then the sequence's own.  One pass, with the running maximum and sum of the softmax.
+//   warps 0-3, 4-7   softmax and output of the first and second row tile, a row per thread
+//   warps 8, 11      issue the matrix products of the first and second row tile
 //   warp 9           requests the tiles of Q, K and V (one thread)
 //   warp 10          looks after V tiles that not every row sees (below)
 // Tensor memory: S of both row tiles (128 columns each, overwritten by P in the type of V) and O of both.
+// There is one CTA per SM.  It takes an item - a block of queries, a head group and a share of the keys - after the other, and every
+// warp goes through the same items by itself: the first S of an item is there when the output of the one before is written.
 constexpr int TILE = 128;                                // keys per tile, rows per row tile
 constexpr int TILE_BYTES = TILE * 128 * 2;               // 64 channels of all its tokens, then the other 64
 constexpr int KV_STAGES = 5;
 constexpr int PROMPT_THREADS = 384;
+constexpr int PROMPT_CTAS = 148;                         // one per SM
 constexpr unsigned TMEM_COLUMNS = 512;
 constexpr float RESCALE_AT = 8.f;                        // powers of two that P may exceed 1 by
+constexpr int BY_POLYNOMIAL = 0;                         // of 16 pairs of exponentials
 
-struct PromptWork {   // a block of a sequence, and where the sequence's queries and keys are
-  int q0, lq, k0, lk, tile, found;
-};
 struct PromptShared {
-  unsigned long long q_full, kv_full[KV_STAGES], kv_empty[KV_STAGES], v_raw[KV_STAGES];
-  unsigned long long s_full[2], p_first[2], p_rest[2], o_full[2], drained;
+  unsigned long long q_full, q_empty, kv_full[KV_STAGES], kv_empty[KV_STAGES], v_raw[KV_STAGES];
+  unsigned long long s_full[2], p_first[2], p_rest[2], o_full[2], o_empty[2], turn[2], drained[2];
   uint32_t tmem;
-  int stop, odd_values;
-  PromptWork work;
+  int stop, odd[4];   // odd: the last item (by its number, of those with the same two low bits) in which warp 10 found infinities or NaN
 };
 constexpr size_t PROMPT_SMEM = 1024 + (2 + KV_STAGES) * static_cast<size_t>(TILE_BYTES) + sizeof(PromptShared);
 static_assert(PROMPT_SMEM <= 227 * 1024, "one CTA per SM");
 
 static __device__ unsigned g_waits_expired;
 
-// The t-th block of `tokens` queries or keys of all sequences (`starts` says whose), the last block of a sequence first: in a causal
-// prompt it sees the most keys.  Lane `first` of the warp's result holds it; -1: there are not as many.
-struct Block {
-  int lane, seq, tile;
-};
-__device__ __forceinline__ Block find_block(const int* starts, int total, int n_seqs, int t, int tokens, int lane) {
-  int before = 0;
-  for (int s0 = 0; s0 < n_seqs; s0 += 32) {
-    const int s = s0 + lane;
-    const int length = s < n_seqs ? max(start_of(starts, s + 1, total) - start_of(starts, s, total), 0) : 0;
-    int sum = (length + tokens - 1) / tokens;
-#pragma unroll
-    for (int d = 1; d < 32; d <<= 1) {
-      const int up = __shfl_up_sync(0xffffffffu, sum, d);
-      if (lane >= d) sum += up;
-    }
-    const unsigned past = __ballot_sync(0xffffffffu, t < before + sum);
-    if (past) return {__ffs(past) - 1, s, before + sum - 1 - t};
-    before += __shfl_sync(0xffffffffu, sum, 31);
-  }
-  return {-1, 0, 0};
-}
-// What the CTA works on, into its shared memory.
-__device__ __forceinline__ void find_work(const PromptArgs& A, const int* starts, int total, int t, int tokens, int lane, PromptWork& w) {
-  if (lane == 0) w.found = 0;
-  __syncwarp();
-  if (A.n_seqs == 0) {   // a single sequence without keys of its own
-    if (lane == 0) w.q0 = 0, w.lq = A.total_q, w.k0 = 0, w.lk = 0, w.tile = t, w.found = 1;
-    return;
-  }
-  const Block b = find_block(starts, total, A.n_seqs, t, tokens, lane);
-  if (lane != b.lane) return;
-  w.q0 = start_of(A.q_starts, b.seq, A.total_q);
-  w.lq = max(start_of(A.q_starts, b.seq + 1, A.total_q) - w.q0, 0);
-  w.k0 = start_of(A.k_starts, b.seq, A.total_k);
-  w.lk = max(start_of(A.k_starts, b.seq + 1, A.total_k) - w.k0, 0);
-  w.tile = b.tile;
-  w.found = 1;
-}
-
 // own keys that query i of its sequence sees
 __device__ __forceinline__ int keys_seen(const PromptArgs& A, int i, int lq, int lk) {
   return A.causal ? min(max(i + 1 + lk - lq, 0), lk) : lk;
 }
+__device__ __forceinline__ int tiles_of(int keys) { return (keys + TILE - 1) / TILE; }
+// shares that the keys of a sequence's blocks are divided into
+__device__ __forceinline__ int shares_of(const PromptArgs& A, int lq, int lk) {
+  return max(1, (tiles_of(A.prefix_len) + tiles_of(keys_seen(A, lq - 1, lq, lk)) + A.per_share - 1) / A.per_share);
+}
+
+// Walks the sequences in order, 32 at a time (a lane each), to the one that holds an item; items are asked for in rising order.
+struct Place {   // a block of a sequence, and where the sequence's queries and keys are
+  int q0, lq, k0, lk, block, rest;   // rest: head group and share
+};
+template <typename Count>
+struct Walk {
+  const PromptArgs& A;
+  Count count;   // items of (lq, lk), and those of one block
+  int lane, at = 0, q0 = 0, lq = 0, k0 = 0, lk = 0;
+  long long before = 0, sum = 0;   // (what starts that are not in order add up to may be anything)
+  __device__ __forceinline__ Walk(const PromptArgs& args, Count c) : A(args), count(c), lane(threadIdx.x & 31) { look(); }
+  __device__ __forceinline__ void look() {
+    const int s = at + lane;
+    q0 = lq = k0 = lk = 0;
+    if (A.n_seqs == 0) lq = lane == 0 ? A.total_q : 0;   // a single sequence without keys of its own
+    else if (s < A.n_seqs) {
+      q0 = start_of(A.q_starts, s, A.total_q), k0 = start_of(A.k_starts, s, A.total_k);
+      lq = max(start_of(A.q_starts, s + 1, A.total_q) - q0, 0), lk = max(start_of(A.k_starts, s + 1, A.total_k) - k0, 0);
+    }
+    sum = static_cast<long long>(count.blocks(lq, lk)) * count.each(lq, lk);
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const long long up = __shfl_up_sync(0xffffffffu, sum, d);
+      if (lane >= d) sum += up;
+    }
+  }
+  // The last block of a sequence, which sees the most keys, comes first.  False: there are not as many items.
+  __device__ __forceinline__ bool find(int item, Place& p) {
+    unsigned past;
+    while (!(past = __ballot_sync(0xffffffffu, item < before + sum))) {
+      before += __shfl_sync(0xffffffffu, sum, 31);
+      at += 32;
+      if (at >= A.n_seqs) {
+        sum = 0;   // (whoever asks again gets the same answer)
+        return false;
+      }
+      look();
+    }
+    const int from = __ffs(past) - 1;
+    auto get = [&](int v) { return __shfl_sync(0xffffffffu, v, from); };
+    p.q0 = get(q0), p.lq = get(lq), p.k0 = get(k0), p.lk = get(lk);
+    const int each = count.each(p.lq, p.lk), blocks = count.blocks(p.lq, p.lk);
+    const int i = item - static_cast<int>(before + __shfl_sync(0xffffffffu, sum, from) - static_cast<long long>(blocks) * each);
+    p.block = blocks - 1 - i / each, p.rest = i % each;
+    return true;
+  }
+};
 
 template <bool BF16>
 __device__ __forceinline__ bool odd_pair(uint32_t v) {   // an infinity or NaN in either half
   constexpr uint32_t e = BF16 ? 0x7F80u : 0x7C00u;
   return (v & e) == e || (v >> 16 & e) == e;
+}
+
+// 2^x of two numbers without the special function unit, which would otherwise take as long as the matrix products: x = n + f with
+// |f| <= 1/2, a polynomial of degree 5 in f with the least largest relative error (7.5e-8; coefficients by Remez's exchange), n added
+// to the exponent.  x is at most 8 here; below -126 the result is 2^-126.
+__device__ __forceinline__ void exp2_polynomial(uint64_t x2, float& a, float& b) {
+  unpair(x2, a, b);
+  x2 = pair(fmaxf(a, -126.f), fmaxf(b, -126.f));
+  const uint64_t whole = pair(12582912.f, 12582912.f), minus = pair(-12582912.f, -12582912.f), sign = pair(-1.f, -1.f);   // 1.5 * 2^23
+  const uint64_t t = pair_add(x2, whole), f = pair_fma(pair_add(t, minus), sign, x2);
+  auto c = [](float v) { return pair(v, v); };
+  uint64_t p = pair_fma(c(0.00132764724f), f, c(0.00967554096f));
+  p = pair_fma(p, f, c(0.0555071309f));
+  p = pair_fma(p, f, c(0.240221202f));
+  p = pair_fma(p, f, c(0.693146944f));
+  p = pair_fma(p, f, c(1.00000012f));
+  float n, m;
+  unpair(t, n, m);
+  unpair(p, a, b);
+  a = __int_as_float(__float_as_int(a) + (__float_as_int(n) << 23));
+  b = __int_as_float(__float_as_int(b) + (__float_as_int(m) << 23));
+}
+
+// an item of the attention kernel
+struct Item {
+  Place at;
+  int head0, kv, share, shares, i0;        // i0: the block's first query in its sequence
+  int before, seen_first, seen_last;       // tiles of the prefix; own keys that the block's first and last query see
+  int lo, hi, hi0, hi1;                    // tiles of keys: [lo, hi), of which the row tiles see those below hi0 and hi1
+  // Own V tiles that hold keys which some rows of the block do not see.  0 x NaN is NaN in a matrix product, so what lies behind
+  // the last key that any row sees is set to 0; an infinity or NaN that only some rows see is set to 0 as well, and those rows
+  // add it at the end.
+  __device__ __forceinline__ bool partly_seen(int tile) const { return tile >= before && (tile - before + 1) * TILE > seen_first; }
+};
+struct ItemCount {
+  const PromptArgs& A;
+  __device__ __forceinline__ int blocks(int lq, int) const { return (lq + 2 * TILE / A.group - 1) / (2 * TILE / A.group); }
+  __device__ __forceinline__ int each(int lq, int lk) const { return A.nh_q / A.group * shares_of(A, lq, lk); }
+};
+__device__ __forceinline__ bool next_item(const PromptArgs& A, Walk<ItemCount>& walk, int round, Item& w) {
+  // (every other round backwards: the first items of a causal prompt are the longest)
+  const int item = round * static_cast<int>(gridDim.x) + (round & 1 ? static_cast<int>(gridDim.x - 1 - blockIdx.x) : static_cast<int>(blockIdx.x));
+  if (item >= A.items || !walk.find(item, w.at)) return false;   // (more than there can be: the starts are not in order)
+  const int lq = w.at.lq, lk = w.at.lk, half = TILE / A.group, groups = A.nh_q / A.group, group = w.at.rest % groups;
+  w.shares = shares_of(A, lq, lk);
+  w.share = w.at.rest / groups;
+  w.head0 = group * A.group;
+  w.kv = w.head0 / (A.nh_q / A.nh_kv);
+  w.i0 = w.at.block * 2 * half;
+  w.before = tiles_of(A.prefix_len);
+  w.seen_first = keys_seen(A, w.i0, lq, lk);
+  w.seen_last = keys_seen(A, min(w.i0 + 2 * half, lq) - 1, lq, lk);
+  const int n0 = w.before + tiles_of(keys_seen(A, min(w.i0 + half, lq) - 1, lq, lk));
+  const int n1 = w.i0 + half < lq ? w.before + tiles_of(w.seen_last) : 0;
+  w.lo = min(w.share * A.per_share, max(n0, n1));
+  w.hi = min(w.lo + A.per_share, max(n0, n1));
+  w.hi0 = min(w.hi, n0), w.hi1 = min(w.hi, n1);
+  return true;
 }
 
 template <bool BF16>
@@ -113,31 +184,18 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1) prompt_kernel(const __grid_
   unsigned char* const tiles = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~static_cast<uintptr_t>(1023));
   PromptShared& sh = *reinterpret_cast<PromptShared*>(tiles + (2 + KV_STAGES) * TILE_BYTES);
   const uint32_t q_at = smem_u32(tiles), kv_at = q_at + 2 * TILE_BYTES;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int groups = A.nh_q / A.group;                       // head groups of all kv heads
-  const int t = blockIdx.x / groups, head0 = (blockIdx.x - t * groups) * A.group, kv = head0 / (A.nh_q / A.nh_kv);
-  const int half = TILE / A.group, tokens = 2 * half;        // tokens per row tile and CTA
-  if (warp == 0) find_work(A, A.q_starts, A.total_q, t, tokens, lane, sh.work);
-  __syncthreads();
-  if (!sh.work.found) return;
-  const int q0 = sh.work.q0, lq = sh.work.lq, k0 = sh.work.k0, lk = sh.work.lk, i0 = sh.work.tile * tokens;   // i0: the CTA's first query in its sequence
-  // tiles of keys: those of the prefix, then the own ones up to the last that a row tile sees; this CTA's are [lo, hi[a])
-  const int before = (A.prefix_len + TILE - 1) / TILE;
-  const int seen_first = keys_seen(A, i0, lq, lk), seen_last = keys_seen(A, min(i0 + tokens, lq) - 1, lq, lk);
-  const int n1 = i0 + half < lq ? before + (seen_last + TILE - 1) / TILE : 0;
-  const int n0 = before + (keys_seen(A, min(i0 + half, lq) - 1, lq, lk) + TILE - 1) / TILE;
-  const int n = max(n0, n1);
-  const int lo = static_cast<int>(static_cast<int64_t>(n) * blockIdx.y / gridDim.y), hi = static_cast<int>(static_cast<int64_t>(n) * (blockIdx.y + 1) / gridDim.y);
-  const int hi0 = min(hi, n0), hi1 = min(hi, n1);
+  const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
+  const int half = TILE / A.group;   // tokens per row tile
   volatile int* const stop = &sh.stop;
   if (warp == 8) tmem_alloc(smem_u32(&sh.tmem), TMEM_COLUMNS);
   if (threadIdx.x == 0) {
-    sh.stop = 0, sh.odd_values = 0;
+    sh.stop = 0;
+    for (int& o : sh.odd) o = -1;
     bar_init(smem_u32(&sh.q_full), 1);
-    bar_init(smem_u32(&sh.drained), 1);
+    bar_init(smem_u32(&sh.q_empty), 2);
     for (int i = 0; i < KV_STAGES; ++i) {
       bar_init(smem_u32(&sh.kv_full[i]), 1);
-      bar_init(smem_u32(&sh.kv_empty[i]), 1);
+      bar_init(smem_u32(&sh.kv_empty[i]), 2);
       bar_init(smem_u32(&sh.v_raw[i]), 1);
     }
     for (int a = 0; a < 2; ++a) {
@@ -145,118 +203,149 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1) prompt_kernel(const __grid_
       bar_init(smem_u32(&sh.p_first[a]), 4);
       bar_init(smem_u32(&sh.p_rest[a]), 4);
       bar_init(smem_u32(&sh.o_full[a]), 1);
+      bar_init(smem_u32(&sh.o_empty[a]), 4);
+      bar_init(smem_u32(&sh.turn[a]), 1);
+      bar_init(smem_u32(&sh.drained[a]), 1);
     }
     bar_init_fence();
   }
+  Walk<ItemCount> walk(A, ItemCount{A});
+  Item w;
   fence_before();
   __syncthreads();
   fence_after();
-  const uint32_t tmem = sh.tmem;
-  // Own V tiles that hold keys which some rows of the CTA do not see.  0 x NaN is NaN in a matrix product, so what lies behind
-  // the last key that any row sees is set to 0; an infinity or NaN that only some rows see is set to 0 as well, and those rows
-  // add it at the end.
-  auto partly_seen = [&](int i) { return i >= before && (i - before + 1) * TILE > seen_first; };
+  const uint32_t tmem = uniform(sh.tmem);
 
+  // 384 threads are launched with 168 registers each: 2 x 128 x 208 + 128 x 88 = 384 x 168
+  if (warp < 8) more_registers<208>();
+  else fewer_registers<88>();
   if (warp < 8) {
     // ---- softmax
-    const int a = warp >> 2, row = threadIdx.x & 127, i = i0 + a * half + row / A.group, head = head0 + row % A.group;
-    const int end = a ? hi1 : hi0, count = max(end - lo, 0);
-    const bool live = i < lq;
-    const int seen = live ? keys_seen(A, i, lq, lk) : lk;
+    const int a = warp >> 2, row = threadIdx.x & 127, token = a * half + row / A.group;
     const uint32_t lanes = tmem + (static_cast<uint32_t>(warp & 3) << 21);   // (32 lanes a warp, in bits 16 and up)
     const uint32_t s_at = lanes + a * TILE, o_at = lanes + 2 * TILE + a * 128;
-    float ref = -INFINITY, sum = 0.f;
     const float scale = A.scale_log2;
+    unsigned s_phase = 0, o_phase = 0;
     bool ok = true;
 #pragma unroll 1
-    for (int it = 0; it < count; ++it) {
-      if (!(ok = __all_sync(0xffffffffu, bar_wait(smem_u32(&sh.s_full[a]), it & 1, stop)))) break;
-      fence_after();
-      uint32_t s[TILE];
-#pragma unroll
-      for (int c = 0; c < TILE; c += 32) tmem_load32(s_at + c, s + c);
-      wait_loads();
-      const int tile = lo + it, limit = tile < before ? A.prefix_len - tile * TILE : seen - (tile - before) * TILE;
-      if (__any_sync(0xffffffffu, limit < TILE)) {
-#pragma unroll
-        for (int c = 0; c < TILE; ++c)
-          if (c >= limit) s[c] = 0xFF800000u;   // -inf
-      }
-      float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-      for (int c = 0; c < TILE; c += 8)
-#pragma unroll
-        for (int k = 0; k < 4; ++k) mx[k] = max3(mx[k], __uint_as_float(s[c + 2 * k]), __uint_as_float(s[c + 2 * k + 1]));
-      const float top = fmaxf(max3(mx[0], mx[1], mx[2]), mx[3]) * scale;
-      // O and the sum are scaled to the maximum only where it has grown enough to matter: P stays below 2^8
-      const bool grown = top > ref + RESCALE_AT;
-      if (__any_sync(0xffffffffu, grown)) {
-        const float f = grown ? exp2_approx(ref - top) : 1.f;
-        if (grown) ref = top;
-        sum *= f;
-        if (it > 0) {
-          // (the product with the tile before, which was issued before this S, is complete)
+    for (int round = 0; ok && next_item(A, walk, round, w); ++round) {
+      const int i = w.i0 + token, head = w.head0 + row % A.group, end = a ? w.hi1 : w.hi0;
+      const bool live = i < w.at.lq;
+      const int seen = live ? keys_seen(A, i, w.at.lq, w.at.lk) : w.at.lk;
+      float ref = -INFINITY, sum = 0.f;
 #pragma unroll 1
-          for (int c = 0; c < 128; c += 32) {
-            uint32_t o[32];
-            tmem_load32(o_at + c, o);
-            wait_loads();
+      for (int tile = w.lo; tile < end; ++tile) {
+        if (!(ok = __all_sync(0xffffffffu, bar_wait(smem_u32(&sh.s_full[a]), s_phase, stop)))) break;
+        s_phase ^= 1;
+        fence_after();
+        uint32_t s[TILE];
 #pragma unroll
-            for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * f);
-            tmem_store32(o_at + c, o);
+        for (int c = 0; c < TILE; c += 32) tmem_load32(s_at + c, s + c);
+        wait_loads(s);
+        const int limit = tile < w.before ? A.prefix_len - tile * TILE : seen - (tile - w.before) * TILE;
+        if (__any_sync(0xffffffffu, limit < TILE)) {
+#pragma unroll
+          for (int c = 0; c < TILE; ++c)
+            if (c >= limit) s[c] = 0xFF800000u;   // -inf
+        }
+        float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int c = 0; c < TILE; c += 8)
+#pragma unroll
+          for (int k = 0; k < 4; ++k) mx[k] = max3(mx[k], __uint_as_float(s[c + 2 * k]), __uint_as_float(s[c + 2 * k + 1]));
+        const float top = max3(max3(mx[0], mx[1], mx[2]), mx[3], mx[3]) * scale;   // NaN if any S is
+        // O and the sum are scaled to the maximum only where it has grown enough to matter: P stays below 2^8
+        const bool grown = !(top <= ref + RESCALE_AT);
+        if (__any_sync(0xffffffffu, grown)) {
+          const float f = grown ? exp2_approx(ref - top) : 1.f;
+          if (grown) ref = top;
+          sum *= f;
+          if (tile > w.lo) {
+            // (the product with the tile before, which was issued before this S, is complete)
+#pragma unroll 1
+            for (int c = 0; c < 128; c += 32) {
+              uint32_t o[32];
+              tmem_load32(o_at + c, o);
+              wait_loads(o);
+#pragma unroll
+              for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * f);
+              tmem_store32(o_at + c, o);
+            }
           }
         }
-      }
-      const float shift = ref == -INFINITY ? 0.f : -ref;
-      const uint64_t scale2 = pair(scale, scale), shift2 = pair(shift, shift);
-      uint64_t sums[2] = {0ull, 0ull};
+        // (a row of which an S is infinite or NaN is NaN, as inf - inf is)
+        const float shift = ref == -INFINITY ? 0.f : fmaf(0.f, ref, -ref);
+        const uint64_t scale2 = pair(scale, scale), shift2 = pair(shift, shift);
+        uint64_t sums[2] = {0ull, 0ull};
 #pragma unroll
-      for (int c = 0; c < TILE; c += 32) {
-        uint32_t p[16];
+        for (int c = 0; c < TILE; c += 32) {
+          uint32_t p[16];
 #pragma unroll
-        for (int k = 0; k < 16; ++k) {
-          float x, y;
-          unpair(pair_fma(pair(__uint_as_float(s[c + 2 * k]), __uint_as_float(s[c + 2 * k + 1])), scale2, shift2), x, y);
-          x = exp2_approx(x), y = exp2_approx(y);
-          sums[k & 1] = pair_add(sums[k & 1], pair(x, y));
-          p[k] = narrow2<BF16>(x, y);
+          for (int k = 0; k < 16; ++k) {
+            float x, y;
+            const uint64_t e = pair_fma(pair(__uint_as_float(s[c + 2 * k]), __uint_as_float(s[c + 2 * k + 1])), scale2, shift2);
+            if (k * BY_POLYNOMIAL % 16 < BY_POLYNOMIAL) {
+              exp2_polynomial(e, x, y);
+            } else {
+              unpair(e, x, y);
+              x = exp2_approx(x), y = exp2_approx(y);
+            }
+            sums[k & 1] = pair_add(sums[k & 1], pair(x, y));
+            p[k] = narrow2<BF16>(x, y);
+            if (c == TILE - 32 && k == 7) {
+              wait_stores();
+              fence_before();
+              __syncwarp();
+              if (lane == 0) bar_arrive(smem_u32(&sh.p_first[a]));
+            }
+          }
+          tmem_store16(s_at + c / 2, p);
+          if (c == TILE - 32) {
+            wait_stores();
+            fence_before();
+            __syncwarp();
+            if (lane == 0) bar_arrive(smem_u32(&sh.p_rest[a]));
+          }
         }
-        tmem_store16(s_at + c / 2, p);
-        if (c >= TILE - 64) {
-          wait_stores();
-          fence_before();
-          __syncwarp();
-          if (lane == 0) bar_arrive(smem_u32(c == TILE - 64 ? &sh.p_first[a] : &sh.p_rest[a]));
-        }
+        float x, y;
+        unpair(pair_add(sums[0], sums[1]), x, y);
+        sum += x + y;
       }
-      float x, y;
-      unpair(pair_add(sums[0], sums[1]), x, y);
-      sum += x + y;
-    }
-    // ---- output
-    if (count > 0 && ok) ok = __all_sync(0xffffffffu, bar_wait(smem_u32(&sh.o_full[a]), 0, stop));
-    if (ok) {
-      fence_after();
-      const int64_t at = (static_cast<int64_t>(q0 + i) * A.nh_q + head);
-      const bool odd = *const_cast<volatile int*>(&sh.odd_values) != 0;
-      const float by = A.part_o ? 1.f : sum == 0.f ? 0.f : 1.f / sum;
-      if (live && A.part_o) A.part_ml[static_cast<int64_t>(blockIdx.y) * A.total_q * A.nh_q + at] = make_float2(ref, sum);
-      else if (live) A.lse[static_cast<int64_t>(head) * A.total_q + q0 + i] = sum == 0.f ? -INFINITY : (ref + log2f(sum)) * 0.6931471805599453f;
+      if (!ok) break;
+      // ---- output
+      const bool any = end > w.lo, part = A.partial || w.shares > 1;
+      const int64_t at = static_cast<int64_t>(w.at.q0 + i) * A.nh_q + head, rows = static_cast<int64_t>(A.total_q) * A.nh_q;
+      const float by = part ? 1.f : sum == 0.f ? 0.f : 1.f / sum;
+      if (live && part) A.part_ml[w.share * rows + at] = make_float2(ref, sum);
+      else if (live) A.lse[static_cast<int64_t>(head) * A.total_q + w.at.q0 + i] = sum == 0.f ? -INFINITY : (ref + log2f(sum)) * 0.6931471805599453f;
+      if (any) {
+        if (!(ok = __all_sync(0xffffffffu, bar_wait(smem_u32(&sh.o_full[a]), o_phase, stop)))) break;
+        o_phase ^= 1;
+        fence_after();
+      } else if (part) {
+        continue;   // (nobody reads a part whose sum is 0)
+      }
+      const bool odd = *const_cast<volatile int*>(&sh.odd[round & 3]) == round;
 #pragma unroll 1
       for (int c = 0; c < 128; c += 32) {
         uint32_t o[32];
-        if (count > 0) {
+        if (any) {
           tmem_load32(o_at + c, o);
-          wait_loads();
+          wait_loads(o);
+          if (c == 96) {
+            fence_before();
+            __syncwarp();
+            if (lane == 0) bar_arrive(smem_u32(&sh.o_empty[a]));
+          }
         } else {
 #pragma unroll
           for (int k = 0; k < 32; ++k) o[k] = 0u;
         }
         if (!live) continue;
         if (odd) {
-          const int to = min(seen, (end - before) * TILE);
-          for (int j = max(seen_first, (lo - before) * TILE); j < to; ++j) {
-            const T* v = static_cast<const T*>(A.v) + (k0 + j) * A.v_token + kv * A.v_head + c;
+          const int to = min(seen, (end - w.before) * TILE);
+          for (int j = max(w.seen_first, (w.lo - w.before) * TILE); j < to; ++j) {
+            const T* v = static_cast<const T*>(A.v) + (w.at.k0 + j) * A.v_token + w.kv * A.v_head + c;
 #pragma unroll
             for (int k = 0; k < 32; ++k) {
               const float x = to_float(v[k]);
@@ -264,8 +353,8 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1) prompt_kernel(const __grid_
             }
           }
         }
-        if (A.part_o) {
-          uint4* to = reinterpret_cast<uint4*>(A.part_o + (static_cast<int64_t>(blockIdx.y) * A.total_q * A.nh_q + at) * 128 + c);
+        if (part) {
+          uint4* to = reinterpret_cast<uint4*>(A.part_o + (w.share * rows + at) * 128 + c);
 #pragma unroll
           for (int k = 0; k < 8; ++k) to[k] = make_uint4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]);
         } else {
@@ -278,152 +367,187 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1) prompt_kernel(const __grid_
         }
       }
     }
-  } else if (warp == 8) {
-    // ---- matrix products
-    if (lane == 0 && hi > lo) {
-      constexpr uint32_t kind_s = mma_kind(BF16, TILE, TILE, false), kind_o = mma_kind(BF16, TILE, 128, true);
-      int stage = 0;
-      unsigned phase = 0;
-      auto scores = [&](int a, uint32_t k_at) {   // S = Q K^T, 16 channels at a time
+  } else if (warp == 8 || warp == 11) {
+    // ---- matrix products of a row tile.  One warp for both was busy all the time with waiting (some 150 cycles for a barrier that is
+    //      complete already) and issuing, and either softmax waited for it: 8 k tokens, all seen: 866 us with one, 832 with two.
+    constexpr uint32_t kind_s = mma_kind(BF16, TILE, TILE, false), kind_o = mma_kind(BF16, TILE, 128, true);
+    const int a = warp == 8 ? 0 : 1;
+    const uint64_t q_operand = operand(q_at + a * TILE_BYTES, 16), k_operand = operand(kv_at, 16), v_operand = operand(kv_at, TILE_BYTES / 2);
+    const uint32_t s_at = tmem + a * TILE, o_at = tmem + 2 * TILE + a * 128;
+    const uint32_t s_full = smem_u32(&sh.s_full[a]), p_first = smem_u32(&sh.p_first[a]), p_rest = smem_u32(&sh.p_rest[a]), o_empty = smem_u32(&sh.o_empty[a]);
+    int stage = 0;
+    unsigned kv_phase = 0, q_phase = 0, p_phase = 0, o_phase = 1, turn = a ^ 1;
+    bool ok = true;
+    auto wait = [&](uint32_t bar, unsigned parity) { return ok = ok && bar_wait(bar, parity, stop); };
+    auto scores = [&] {   // S = Q K^T, 16 channels at a time
+      if (elect_one()) {
 #pragma unroll
-        for (int c = 0; c < 8; ++c)
-          mma_shared(tmem + a * TILE, operand(q_at + a * TILE_BYTES + (c >> 2) * (TILE_BYTES / 2) + (c & 3) * 32, 16),
-                     operand(k_at + (c >> 2) * (TILE_BYTES / 2) + (c & 3) * 32, 16), kind_s, c > 0);
-        mma_commit(smem_u32(&sh.s_full[a]));
-      };
-      auto advance = [&] {
-        if (++stage == KV_STAGES) stage = 0, phase ^= 1;
-      };
-      bool ok = bar_wait(smem_u32(&sh.q_full), 0, stop) && bar_wait(smem_u32(&sh.kv_full[0]), 0, stop);
-      if (ok) {
-        fence_after();
-        if (lo < hi0) scores(0, kv_at);
-        if (lo < hi1) scores(1, kv_at);
-        mma_commit(smem_u32(&sh.kv_empty[0]));
-        advance();
-      }
-#pragma unroll 1
-      for (int i = lo; ok && i < hi; ++i) {
-        const int v_stage = stage;
-        if (!(ok = bar_wait(smem_u32(&sh.kv_full[stage]), phase, stop))) break;
-        advance();
-        const uint32_t v_at = kv_at + v_stage * TILE_BYTES, k_at = kv_at + stage * TILE_BYTES;
-        bool have_k = false;
-#pragma unroll
-        for (int a = 0; a < 2; ++a) {
-          const int end = a ? hi1 : hi0;
-          if (i < end) {
-            // O += P V, 16 keys at a time, the first three quarters as soon as they are there
-            if (!(ok = bar_wait(smem_u32(&sh.p_first[a]), (i - lo) & 1, stop))) break;
-            fence_after();
-#pragma unroll
-            for (int c = 0; c < 6; ++c)
-              mma_tensor(tmem + 2 * TILE + a * 128, tmem + a * TILE + c * 8, operand(v_at + c * 2048, TILE_BYTES / 2), kind_o, c > 0 || i > lo);
-            if (!(ok = bar_wait(smem_u32(&sh.p_rest[a]), (i - lo) & 1, stop))) break;
-            fence_after();
-#pragma unroll
-            for (int c = 6; c < 8; ++c)
-              mma_tensor(tmem + 2 * TILE + a * 128, tmem + a * TILE + c * 8, operand(v_at + c * 2048, TILE_BYTES / 2), kind_o, true);
-            if (i + 1 == end) mma_commit(smem_u32(&sh.o_full[a]));
-          }
-          if (a == 1) mma_commit(smem_u32(&sh.kv_empty[v_stage]));
-          if (i + 1 < end) {
-            if (!have_k && !(ok = bar_wait(smem_u32(&sh.kv_full[stage]), phase, stop))) break;
-            fence_after();
-            have_k = true;
-            scores(a, k_at);
-          }
+        for (int c = 0; c < 8; ++c) {
+          const int at = ((c >> 2) * (TILE_BYTES / 2) + (c & 3) * 32) >> 4;
+          mma_shared(s_at, q_operand + at, k_operand + (stage * TILE_BYTES >> 4) + at, kind_s, c > 0);
         }
-        if (!ok) break;
+        mma_commit(s_full);
+      }
+    };
+    auto commit = [&](unsigned long long& bar) {
+      if (elect_one()) mma_commit(smem_u32(&bar));
+    };
+    auto advance = [&] {
+      if (++stage == KV_STAGES) stage = 0, kv_phase ^= 1;
+    };
+#pragma unroll 1
+    for (int round = 0; ok && next_item(A, walk, round, w); ++round) {
+      const int lo = uniform(w.lo), hi = uniform(w.hi), end = uniform(a ? w.hi1 : w.hi0), both = uniform(min(w.hi0, w.hi1));
+      if (hi <= lo) continue;
+      if (!wait(smem_u32(&sh.q_full), q_phase) || !wait(smem_u32(&sh.kv_full[stage]), kv_phase)) break;
+      q_phase ^= 1;
+      if (lo < end) scores();
+      commit(sh.kv_empty[stage]);
+      if (lo + 1 >= end) commit(sh.q_empty);
+      advance();
+#pragma unroll 1
+      for (int i = lo; i < hi; ++i) {   // (tiles that the other row tile alone sees are let go)
+        const int v_stage = stage;
+        if (!wait(smem_u32(&sh.kv_full[stage]), kv_phase)) break;
+        advance();
+        if (i + 1 < hi && !wait(smem_u32(&sh.kv_full[stage]), kv_phase)) break;
+        if (i < end) {
+          // O += P V, 16 keys at a time, the first three quarters as soon as they are there
+          auto product = [&](int c) {
+            mma_tensor(o_at, s_at + c * 8, v_operand + (v_stage * TILE_BYTES >> 4) + c * (2048 >> 4), kind_o, c > 0 || i > lo);
+          };
+          if (i == lo) {   // (the output of the item before has been read)
+            if (!wait(o_empty, o_phase)) break;
+            o_phase ^= 1;
+          }
+          // The row tiles take turns.  Left alone they fall into step, and the tensor cores wait for both softmaxes, which share
+          // the special function units: 4280 cycles a tile instead of 3300 (8 k tokens, all seen: 1132 us, 832).
+          if (i < both) {
+            if (!wait(smem_u32(&sh.turn[a]), turn)) break;
+            turn ^= 1;
+          }
+          if (!wait(p_first, p_phase)) break;
+          fence_after();
+          if (elect_one()) {
+#pragma unroll
+            for (int c = 0; c < 6; ++c) product(c);
+          }
+          if (!wait(p_rest, p_phase)) break;
+          p_phase ^= 1;
+          fence_after();
+          if (elect_one()) {
+#pragma unroll
+            for (int c = 6; c < 8; ++c) product(c);
+          }
+          if (i + 1 < end) scores();
+          else commit(sh.o_full[a]);
+          if (i < both && elect_one()) bar_arrive(smem_u32(&sh.turn[a ^ 1]));
+        }
+        commit(sh.kv_empty[v_stage]);
         if (i + 1 < hi) {
-          mma_commit(smem_u32(&sh.kv_empty[stage]));
+          commit(sh.kv_empty[stage]);
+          if (i + 2 == end) commit(sh.q_empty);
           advance();
         }
       }
-      if (!ok) {   // products in flight end before the CTA does
-        mma_commit(smem_u32(&sh.drained));
-        for (int k = 0; k < WAIT_TRIES && !bar_try(smem_u32(&sh.drained), 0); ++k) {
-        }
+    }
+    if (!ok && lane == 0) {   // products in flight end before the CTA does
+      mma_commit(smem_u32(&sh.drained[a]));
+      for (int k = 0; k < WAIT_TRIES && !bar_try(smem_u32(&sh.drained[a]), 0); ++k) {
       }
     }
   } else if (warp == 9) {
-    // ---- copies: Q, then K and V of one tile after the other
-    if (lane == 0 && hi > lo) {
-      bar_expect(smem_u32(&sh.q_full), 2 * TILE_BYTES);
-      for (int a = 0; a < 2; ++a)
-        for (int c = 0; c < 2; ++c)
-          copy_box(q_at + a * TILE_BYTES + c * (TILE_BYTES / 2), &M.q, 64 * c, head0, q0 + i0 + a * half, smem_u32(&sh.q_full));
-      int stage = 0;
-      unsigned phase = 1, to_raw = 0, raw_parity = 0, full_parity = 0, used = 0;   // a bit per stage: of the last copy into it
-      bool ok = true;
+    // ---- copies: of every item Q, then K and V of one tile after the other
+    int stage = 0;
+    unsigned kv_phase = 1, q_phase = 1, to_raw = 0, raw_parity = 0, full_parity = 0, used = 0;   // a bit per stage: of the last copy into it
+    bool ok = true;
 #pragma unroll 1
-      for (int i = lo; ok && i < hi; ++i) {
-        const bool own = i >= before;
-        const int token = own ? k0 + (i - before) * TILE : i * TILE;
+    for (int round = 0; next_item(A, walk, round, w); ++round) {
+      if (w.hi <= w.lo) continue;
+      if (lane == 0) {
+        if ((ok = bar_wait(smem_u32(&sh.q_empty), q_phase, stop))) {
+          q_phase ^= 1;
+          bar_expect(smem_u32(&sh.q_full), 2 * TILE_BYTES);
+          for (int a = 0; a < 2; ++a)
+            for (int c = 0; c < 2; ++c)
+              copy_box(q_at + a * TILE_BYTES + c * (TILE_BYTES / 2), &M.q, 64 * c, w.head0, w.at.q0 + w.i0 + a * half, smem_u32(&sh.q_full));
+        }
 #pragma unroll 1
-        for (int side = 0; side < 2; ++side) {
-          if (!(ok = bar_wait(smem_u32(&sh.kv_empty[stage]), phase, stop))) break;
-          const CUtensorMap* map = side ? (own ? &M.v : &M.pv) : (own ? &M.k : &M.pk);
-          const bool raw_first = side && partly_seen(i);
-          const uint32_t bar = smem_u32(raw_first ? &sh.v_raw[stage] : &sh.kv_full[stage]), bit = 1u << stage;
-          if (used & bit) full_parity ^= bit;
-          if (raw_first) raw_parity ^= bit;
-          used |= bit;
-          to_raw = raw_first ? to_raw | bit : to_raw & ~bit;
-          bar_expect(bar, TILE_BYTES);
-          for (int c = 0; c < 2; ++c) copy_box(kv_at + stage * TILE_BYTES + c * (TILE_BYTES / 2), map, 64 * c, kv, token, bar);
-          if (++stage == KV_STAGES) stage = 0, phase ^= 1;
+        for (int i = w.lo; ok && i < w.hi; ++i) {
+          const bool own = i >= w.before;
+          const int token = own ? w.at.k0 + (i - w.before) * TILE : i * TILE;
+#pragma unroll 1
+          for (int side = 0; side < 2; ++side) {
+            if (!(ok = bar_wait(smem_u32(&sh.kv_empty[stage]), kv_phase, stop))) break;
+            const CUtensorMap* map = side ? (own ? &M.v : &M.pv) : (own ? &M.k : &M.pk);
+            const bool raw_first = side && w.partly_seen(i);
+            const uint32_t bar = smem_u32(raw_first ? &sh.v_raw[stage] : &sh.kv_full[stage]), bit = 1u << stage;
+            if (used & bit) full_parity ^= bit;
+            if (raw_first) raw_parity ^= bit;
+            used |= bit;
+            to_raw = raw_first ? to_raw | bit : to_raw & ~bit;
+            bar_expect(bar, TILE_BYTES);
+            for (int c = 0; c < 2; ++c) copy_box(kv_at + stage * TILE_BYTES + c * (TILE_BYTES / 2), map, 64 * c, w.kv, token, bar);
+            if (++stage == KV_STAGES) stage = 0, kv_phase ^= 1;
+          }
         }
       }
-      if (!ok) {   // copies in flight land before the CTA ends
-        auto landed = [&](const unsigned long long& bar, unsigned parity) {
-          for (int k = 0; k < WAIT_TRIES && !bar_try(smem_u32(&bar), parity); ++k) {
-          }
-        };
-        landed(sh.q_full, 0);
-        for (int k = 0; k < KV_STAGES; ++k) {
-          if (!(used >> k & 1)) continue;
-          if (to_raw >> k & 1) landed(sh.v_raw[k], (raw_parity >> k & 1) ^ 1);
-          else landed(sh.kv_full[k], full_parity >> k & 1);
+      if (__any_sync(0xffffffffu, !ok)) break;
+    }
+    if (lane == 0 && !ok) {   // copies in flight land before the CTA ends
+      auto landed = [&](const unsigned long long& bar, unsigned parity) {
+        for (int k = 0; k < WAIT_TRIES && !bar_try(smem_u32(&bar), parity); ++k) {
         }
+      };
+      if (used) landed(sh.q_full, q_phase);
+      for (int k = 0; k < KV_STAGES; ++k) {
+        if (!(used >> k & 1)) continue;
+        if (to_raw >> k & 1) landed(sh.v_raw[k], (raw_parity >> k & 1) ^ 1);
+        else landed(sh.kv_full[k], full_parity >> k & 1);
       }
     }
   } else if (warp == 10) {
     // ---- V tiles that not every row sees
-    unsigned parity = 0;   // a bit per stage
+    unsigned parity = 0, fills = 0;   // a bit per stage; copies into stages before this item's
+    bool ok = true;
 #pragma unroll 1
-    for (int i = lo; i < hi; ++i) {
-      if (!partly_seen(i)) continue;
-      const int stage = (2 * (i - lo) + 1) % KV_STAGES, first = (i - before) * TILE;
-      if (!bar_wait(smem_u32(&sh.v_raw[stage]), parity >> stage & 1, stop)) break;
-      parity ^= 1u << stage;
-      unsigned char* const v = tiles + (2 + stage) * TILE_BYTES;
-      bool odd = false;
-      // (which of a row's pieces of 16 bytes comes where does not matter here)
-      for (int k = lane; k < TILE_BYTES / 16; k += 32) {
-        const int token = first + (k >> 3 & (TILE - 1));
-        if (token < seen_first) continue;
-        uint4* const at = reinterpret_cast<uint4*>(v + k * 16);
-        if (token >= seen_last) {
-          *at = make_uint4(0u, 0u, 0u, 0u);
-          continue;
-        }
-        uint4 x = *at;
-        if (odd_pair<BF16>(x.x) || odd_pair<BF16>(x.y) || odd_pair<BF16>(x.z) || odd_pair<BF16>(x.w)) {
-          odd = true;
-          uint32_t* w = &x.x;
-          constexpr uint32_t e = BF16 ? 0x7F80u : 0x7C00u;
-          for (int m = 0; m < 4; ++m) {
-            if ((w[m] & e) == e) w[m] &= 0xFFFF0000u;
-            if ((w[m] >> 16 & e) == e) w[m] &= 0x0000FFFFu;
+    for (int round = 0; ok && next_item(A, walk, round, w); ++round) {
+#pragma unroll 1
+      for (int i = max(w.lo, w.before + w.seen_first / TILE); i < w.hi; ++i) {
+        const int stage = (fills + 2 * (i - w.lo) + 1) % KV_STAGES, first = (i - w.before) * TILE;
+        if (!w.partly_seen(i)) continue;
+        if (!(ok = __all_sync(0xffffffffu, bar_wait(smem_u32(&sh.v_raw[stage]), parity >> stage & 1, stop)))) break;
+        parity ^= 1u << stage;
+        unsigned char* const v = tiles + (2 + stage) * TILE_BYTES;
+        bool odd = false;
+        // (which of a row's pieces of 16 bytes comes where does not matter here)
+        for (int k = lane; k < TILE_BYTES / 16; k += 32) {
+          const int j = first + (k >> 3 & (TILE - 1));
+          if (j < w.seen_first) continue;
+          uint4* const at = reinterpret_cast<uint4*>(v + k * 16);
+          if (j >= w.seen_last) {
+            *at = make_uint4(0u, 0u, 0u, 0u);
+            continue;
           }
-          *at = x;
+          uint4 x = *at;
+          if (odd_pair<BF16>(x.x) || odd_pair<BF16>(x.y) || odd_pair<BF16>(x.z) || odd_pair<BF16>(x.w)) {
+            odd = true;
+            uint32_t* word = &x.x;
+            constexpr uint32_t e = BF16 ? 0x7F80u : 0x7C00u;
+            for (int m = 0; m < 4; ++m) {
+              if ((word[m] & e) == e) word[m] &= 0xFFFF0000u;
+              if ((word[m] >> 16 & e) == e) word[m] &= 0x0000FFFFu;
+            }
+            *at = x;
+          }
         }
+        if (odd) *const_cast<volatile int*>(&sh.odd[round & 3]) = round;
+        fence_generic_to_async();
+        __syncwarp();
+        if (lane == 0) bar_arrive(smem_u32(&sh.kv_full[stage]));
       }
-      if (odd) *const_cast<volatile int*>(&sh.odd_values) = 1;
-      fence_generic_to_async();
-      __syncwarp();
-      if (lane == 0) bar_arrive(smem_u32(&sh.kv_full[stage]));
+      fills += 2 * max(w.hi - w.lo, 0);
+      fills %= KV_STAGES;
     }
   }
   __syncwarp();
@@ -436,16 +560,20 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1) prompt_kernel(const __grid_
 
 // Joins the parts of a row: a warp per row.
 template <bool BF16>
-__global__ void __launch_bounds__(256) prompt_join_kernel(const PromptArgs A, int splits) {
+__global__ void __launch_bounds__(256) prompt_join_kernel(const PromptArgs A) {
   using T = std::conditional_t<BF16, __nv_bfloat16, __half>;
   const int64_t row = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5), rows = static_cast<int64_t>(A.total_q) * A.nh_q;
   const int lane = threadIdx.x & 31;
   if (row >= rows) return;
   const int token = static_cast<int>(row / A.nh_q), head = static_cast<int>(row % A.nh_q);
-  bool in = false;
-  for (int s = lane; s < A.n_seqs; s += 32)
-    in |= token >= start_of(A.q_starts, s, A.total_q) && token < start_of(A.q_starts, s + 1, A.total_q);
-  if (!__any_sync(0xffffffffu, in)) return;
+  int splits = 0;   // of the token's sequence; rows in no sequence have none
+  for (int s = lane; s < A.n_seqs; s += 32) {
+    const int q0 = start_of(A.q_starts, s, A.total_q), q1 = start_of(A.q_starts, s + 1, A.total_q);
+    if (token >= q0 && token < q1)
+      splits = shares_of(A, q1 - q0, max(start_of(A.k_starts, s + 1, A.total_k) - start_of(A.k_starts, s, A.total_k), 0));
+  }
+  splits = __reduce_max_sync(0xffffffffu, splits);
+  if (splits < 2) return;   // (written as a whole)
   float m = -INFINITY, l = 0.f;
   for (int s = 0; s < splits; ++s) m = fmaxf(m, A.part_ml[s * rows + row].x);
   const float ref = m == -INFINITY ? 0.f : m;
@@ -476,7 +604,6 @@ struct ImportanceShared {
   unsigned long long full[4], empty[4], s_full[2], s_empty[2], drained;
   uint32_t tmem;
   int stop;
-  PromptWork work;
   alignas(16) float lse[2][IMP_COLUMNS];
 };
 struct ImportanceShape {
@@ -487,6 +614,12 @@ static size_t imp_smem(const ImportanceShape& g) {
   return 1024 + g.stages * static_cast<size_t>(imp_stage_bytes(g)) + sizeof(float) * g.rows * TILE + sizeof(ImportanceShared);
 }
 
+struct KeyCount {
+  int keys;
+  __device__ __forceinline__ int blocks(int, int lk) const { return (lk + keys - 1) / keys; }
+  __device__ __forceinline__ int each(int, int) const { return 1; }
+};
+
 template <bool BF16, int HB>
 __global__ void __launch_bounds__(IMP_THREADS) importance_kernel(const __grid_constant__ PromptArgs A, const __grid_constant__ PromptMaps M,
                                                                  const ImportanceShape G, const float* lse, __half* out) {
@@ -496,10 +629,9 @@ __global__ void __launch_bounds__(IMP_THREADS) importance_kernel(const __grid_co
   float* const acc = reinterpret_cast<float*>(tiles + G.stages * stage_bytes);   // [rows][key]
   ImportanceShared& sh = *reinterpret_cast<ImportanceShared*>(acc + G.rows * TILE);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  if (warp == 0) find_work(A, A.k_starts, A.total_k, blockIdx.x, G.keys, lane, sh.work);
-  __syncthreads();
-  if (!sh.work.found) return;
-  const int q0 = sh.work.q0, lq = sh.work.lq, k0 = sh.work.k0, lk = sh.work.lk, j0 = sh.work.tile * G.keys;
+  Place w;
+  if (!Walk<KeyCount>(A, KeyCount{G.keys}).find(blockIdx.x, w)) return;
+  const int q0 = w.q0, lq = w.lq, k0 = w.k0, lk = w.lk, j0 = w.block * G.keys;
   const int t = min(G.rows, lq), first = q0 + lq - t;   // the queries
   const int per_kv = A.nh_q / A.nh_kv / HB, items = t > 0 ? A.nh_kv * per_kv : 0;
   volatile int* const stop = &sh.stop;
@@ -550,7 +682,7 @@ __global__ void __launch_bounds__(IMP_THREADS) importance_kernel(const __grid_co
         tmem_load8(at + c, s);
         const float4 d0 = *reinterpret_cast<const float4*>(den + c), d1 = *reinterpret_cast<const float4*>(den + c + 4);
         const float d[8] = {d0.x, d0.y, d0.z, d0.w, d1.x, d1.y, d1.z, d1.w};
-        wait_loads();
+        wait_loads(s);
 #pragma unroll
         for (int k = 0; k < 8; k += HB) {
           float sum = 0.f;
@@ -683,11 +815,20 @@ static int64_t most_blocks(const PromptArgs& A) {
   return (A.total_q + n * (tokens - 1)) / tokens;
 }
 
-// Where the CTAs do not fill the GPU, the tiles of keys are shared out as well.
-static int prompt_splits(const PromptArgs& A) {
-  const int64_t ctas = most_blocks(A) * (A.nh_q / A.group);
-  const int64_t tiles = ceil_div(A.prefix_len, TILE) + ceil_div(A.total_k / max(1, A.n_seqs), TILE);
-  return static_cast<int>(max(int64_t{1}, min(148 / max(int64_t{1}, ctas), tiles)));
+// Tiles of keys per share, and the shares that a block has at most.  Where the blocks do not fill the GPU, their keys are shared out:
+// for one sequence so that there is an item for every CTA, for several - of unknown lengths - into shares of which a CTA gets about three.
+static int prompt_shares(PromptArgs& A) {
+  const int64_t blocks = most_blocks(A) * (A.nh_q / A.group), n = max(1, A.n_seqs);
+  const int64_t most = ceil_div(A.prefix_len, TILE) + ceil_div(A.total_k, TILE);
+  int64_t per = max(int64_t{1}, most);
+  if (blocks < PROMPT_CTAS && most > 1) {
+    const int64_t average = ceil_div(A.prefix_len, TILE) + ceil_div(A.total_k, TILE * n);
+    if (n == 1) per = ceil_div(most, PROMPT_CTAS / blocks);
+    else per = max(int64_t{4}, ceil_div(blocks * average, 3 * PROMPT_CTAS));
+    per = max(per, ceil_div(most, max(int64_t{1}, 8 * PROMPT_CTAS / blocks)));   // (the parts take memory)
+  }
+  A.per_share = static_cast<int>(per);
+  return static_cast<int>(max(int64_t{1}, ceil_div(most, per)));
 }
 
 static int tensor_map(CUtensorMap* map, const void* base, bool bf16, int64_t tokens, int heads, int64_t token_stride, int64_t head_stride,
@@ -711,7 +852,7 @@ static int tensor_map(CUtensorMap* map, const void* base, bool bf16, int64_t tok
   return HQKV_OK;
 }
 
-static int launch_prompt(const PromptArgs& A, int splits, cudaStream_t st) {
+static int launch_prompt(PromptArgs& A, int shares, cudaStream_t st) {
   PromptMaps M = {};
   if (int rc = tensor_map(&M.q, A.q, A.bf16, A.total_q, A.nh_q, A.q_token, A.q_head, A.group, TILE / A.group)) return rc;
   if (A.total_k > 0) {
@@ -730,10 +871,10 @@ static int launch_prompt(const PromptArgs& A, int splits, cudaStream_t st) {
     HQKV_CUDA(cudaFuncSetAttribute(prompt_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(PROMPT_SMEM)));
     if (dev >= 0 && dev < 64) opted_in[dev] = true;
   }
-  const int64_t blocks = most_blocks(A) * (A.nh_q / A.group);
-  HQKV_REQUIRE(blocks < (1ll << 31), "prompt: too many rows");
-  const dim3 grid(static_cast<unsigned>(blocks), splits);
-  (A.bf16 ? prompt_kernel<true> : prompt_kernel<false>)<<<grid, PROMPT_THREADS, PROMPT_SMEM, st>>>(A, M);
+  const int64_t items = most_blocks(A) * (A.nh_q / A.group) * shares;
+  HQKV_REQUIRE(items < (1ll << 30), "prompt: too many rows");
+  A.items = static_cast<int>(items);
+  (A.bf16 ? prompt_kernel<true> : prompt_kernel<false>)<<<static_cast<unsigned>(min(items, int64_t{PROMPT_CTAS})), PROMPT_THREADS, PROMPT_SMEM, st>>>(A, M);
   HQKV_LAUNCH_CHECK("prompt");
   return HQKV_OK;
 }
@@ -776,24 +917,26 @@ static int launch_importance(const PromptArgs& A, const float* lse, int rows, __
   }
 }
 
-int prefix_splits(const hqkv_prompt_t* p) {
+int prefix_shares(const hqkv_prompt_t* p) {
   PromptArgs A;
   A.total_q = static_cast<int>(p->total_q), A.total_k = 0, A.n_seqs = 0, A.prefix_len = static_cast<int>(p->prefix_len);
   A.nh_q = p->nh_q, A.nh_kv = p->nh_kv, A.group = head_group(p->nh_q, p->nh_kv);
-  return prompt_splits(A);
+  return prompt_shares(A);
 }
 
-int prefix_partial(const hqkv_prompt_t* p, float* part_o, float2* part_ml, int splits, cudaStream_t st) {
+int prefix_partial(const hqkv_prompt_t* p, float* part_o, float2* part_ml, cudaStream_t st) {
   PromptArgs A;
   if (int rc = prompt_args(p, true, A)) return rc;
   A.part_o = part_o, A.part_ml = part_ml;
-  return launch_prompt(A, splits, st);
+  A.partial = true;
+  const int shares = prompt_shares(A);
+  return launch_prompt(A, shares, st);
 }
 
-static size_t split_bytes(const PromptArgs& A, int splits, size_t* part_ml) {
-  const size_t rows = static_cast<size_t>(A.total_q) * A.nh_q * splits;
+static size_t split_bytes(const PromptArgs& A, int shares, size_t* part_ml) {
+  const size_t rows = static_cast<size_t>(A.total_q) * A.nh_q * shares;
   *part_ml = rows * 128 * sizeof(float);
-  return splits > 1 ? *part_ml + rows * sizeof(float2) : 0;
+  return shares > 1 ? *part_ml + rows * sizeof(float2) : 0;
 }
 
 }  // namespace hqkv
@@ -804,7 +947,8 @@ extern "C" size_t hqkv_prompt_workspace_bytes(const hqkv_prompt_t* prompt_host) 
   PromptArgs A;
   if (prompt_args(prompt_host, true, A) != HQKV_OK || A.total_q == 0 || A.n_seqs == 0) return 0;
   size_t ml;
-  return split_bytes(A, prompt_splits(A), &ml);
+  const int shares = prompt_shares(A);
+  return split_bytes(A, shares, &ml);
 }
 
 extern "C" int hqkv_prompt_attention(const hqkv_prompt_t* prompt_host, void* out, float* lse, void* workspace, size_t workspace_bytes, void* stream) {
@@ -813,18 +957,18 @@ extern "C" int hqkv_prompt_attention(const hqkv_prompt_t* prompt_host, void* out
   if (A.total_q == 0 || A.n_seqs == 0) return HQKV_OK;
   HQKV_REQUIRE(out && lse && aligned(out, 16) && aligned(lse, 4), "prompt: the outputs are null or misaligned");
   A.out = out, A.lse = lse;
-  const int splits = prompt_splits(A);
+  const int shares = prompt_shares(A);
   size_t ml;
-  const size_t need = split_bytes(A, splits, &ml);
+  const size_t need = split_bytes(A, shares, &ml);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (splits == 1) return launch_prompt(A, 1, st);
+  if (shares == 1) return launch_prompt(A, 1, st);
   HQKV_REQUIRE(workspace && aligned(workspace, 256), "prompt: the workspace is null or not 256-byte aligned");
   if (workspace_bytes < need) return fail(HQKV_E_WORKSPACE, "prompt: the workspace holds %zu bytes, %zu needed", workspace_bytes, need);
   A.part_o = static_cast<float*>(workspace);
   A.part_ml = reinterpret_cast<float2*>(static_cast<unsigned char*>(workspace) + ml);
-  if (int rc = launch_prompt(A, splits, st)) return rc;
+  if (int rc = launch_prompt(A, shares, st)) return rc;
   const unsigned grid = static_cast<unsigned>(ceil_div(static_cast<int64_t>(A.total_q) * A.nh_q, 8));
-  (A.bf16 ? prompt_join_kernel<true> : prompt_join_kernel<false>)<<<grid, 256, 0, st>>>(A, splits);
+  (A.bf16 ? prompt_join_kernel<true> : prompt_join_kernel<false>)<<<grid, 256, 0, st>>>(A);
   HQKV_LAUNCH_CHECK("prompt_join");
   return HQKV_OK;
 }

@@ -15,20 +15,22 @@ struct PromptArgs {
   const int *q_starts, *k_starts;                   // [n_seqs + 1]
   int n_seqs, total_q, total_k, prefix_len, nh_q, nh_kv;
   int group;                                        // query heads of a kv head that share a row tile
-  bool causal, bf16;
+  int items;                                        // most blocks x head groups x shares
+  int per_share;                                    // tiles of keys per share of a block's
+  bool causal, bf16, partial;                       // partial: part_o and part_ml are the result
   float scale_log2;                                 // scale * log2(e)
   void* out;                                        // [total_q][nh_q][128]
   float* lse;                                       // [nh_q][total_q]
-  float* part_o;                                    // [splits][total_q * nh_q][128], not yet normalised (null: out and lse)
-  float2* part_ml;                                  // [splits][total_q * nh_q] (maximum, sum), in powers of two
+  float* part_o;                                    // [shares][total_q * nh_q][128], not yet normalised
+  float2* part_ml;                                  // [shares][total_q * nh_q] (maximum, sum), in powers of two
 };
 
 struct PromptMaps {   // the tensors as (channel, head, token), for copies by tiles
   CUtensorMap q, k, v, pk, pv;
 };
 
-// Attention of p's queries (a token each, no sequences) to its prefix alone: splits parts per row, to be joined.
-int prefix_splits(const hqkv_prompt_t* p);
-int prefix_partial(const hqkv_prompt_t* p, float* part_o, float2* part_ml, int splits, cudaStream_t st);
+// Attention of p's queries (a token each, no sequences) to its prefix alone: `shares` parts per row, to be joined.
+int prefix_shares(const hqkv_prompt_t* p);
+int prefix_partial(const hqkv_prompt_t* p, float* part_o, float2* part_ml, cudaStream_t st);
 
 }  // namespace hqkv

@@ -8,8 +8,17 @@ namespace hqkv {
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
 
-// ---- mbarriers.  Every wait has a limit (some seconds); what runs out sets `stop`, which ends the waits of all roles of the CTA.
-constexpr int WAIT_TRIES = 1 << 20;
+// One thread of a warp that is here as a whole.  Around a tcgen05 instruction the compiler then keeps its operands in uniform
+// registers; issued from `if (lane == 0)` each of them took some 100 cycles.
+__device__ __forceinline__ bool elect_one() {
+  unsigned chosen;
+  asm volatile("{\n.reg .pred p;\nelect.sync _|p, 0xFFFFFFFF;\nselp.u32 %0, 1, 0, p;\n}" : "=r"(chosen));
+  return chosen != 0;
+}
+__device__ __forceinline__ int uniform(int v) { return __shfl_sync(0xffffffffu, v, 0); }
+
+// ---- mbarriers.  Every wait has a limit (a second or so); what runs out sets `stop`, which ends the waits of all roles of the CTA.
+constexpr int WAIT_TRIES = 1 << 24;
 __device__ __forceinline__ void bar_init(uint32_t bar, unsigned count) {
   asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory");
 }
@@ -22,13 +31,14 @@ __device__ __forceinline__ void bar_expect(uint32_t bar, unsigned bytes) {
 }
 __device__ __forceinline__ bool bar_try(uint32_t bar, unsigned parity) {
   unsigned ok;
-  asm volatile("{\n.reg .pred p;\nmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, 2000;\nselp.u32 %0, 1, 0, p;\n}"
+  asm volatile("{\n.reg .pred p;\nmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\nselp.u32 %0, 1, 0, p;\n}"
                : "=r"(ok)
                : "r"(bar), "r"(parity)
                : "memory");
   return ok != 0;
 }
-static __device__ __noinline__ bool bar_wait_long(uint32_t bar, unsigned parity, volatile int* stop) {
+__device__ __forceinline__ bool bar_wait(uint32_t bar, unsigned parity, volatile int* stop) {
+#pragma unroll 1
   for (int i = 0; i < WAIT_TRIES; ++i) {
     if (bar_try(bar, parity)) return true;
     if (*stop) return false;
@@ -36,9 +46,12 @@ static __device__ __noinline__ bool bar_wait_long(uint32_t bar, unsigned parity,
   *stop = 1;
   return false;
 }
-__device__ __forceinline__ bool bar_wait(uint32_t bar, unsigned parity, volatile int* stop) {
-  return bar_try(bar, parity) || bar_wait_long(bar, parity, stop);
-}
+
+// registers per thread of a warpgroup (four warps, all of which come here)
+template <int N>
+__device__ __forceinline__ void more_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N>
+__device__ __forceinline__ void fewer_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
 
 // ---- tensor copies: a box of a (channel, head, token) map, rows of 128 bytes swizzled
 __device__ __forceinline__ void copy_box(uint32_t dst, const CUtensorMap* map, int channel, int head, int token, uint32_t bar) {
@@ -59,7 +72,14 @@ __device__ __forceinline__ void tmem_free(uint32_t at, unsigned columns) {
 }
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void wait_loads() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+// the loads' registers pass through the wait, so that nothing that reads them comes before it
+template <int N>
+__device__ __forceinline__ void wait_loads(uint32_t (&v)[N]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+  for (int i = 0; i < N; i += 8)
+    asm volatile("" : "+r"(v[i]), "+r"(v[i + 1]), "+r"(v[i + 2]), "+r"(v[i + 3]), "+r"(v[i + 4]), "+r"(v[i + 5]), "+r"(v[i + 6]), "+r"(v[i + 7]));
+}
 __device__ __forceinline__ void wait_stores() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void mma_commit(uint32_t bar) {
   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
@@ -142,9 +162,10 @@ __device__ __forceinline__ float exp2_approx(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+// NaN if one of them is
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float d;
-  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
   return d;
 }
 template <bool BF16>
