@@ -595,25 +595,27 @@ __global__ void __launch_bounds__(256) prompt_join_kernel(const PromptArgs A) {
 // ------------------------------------------------------------------------------------------------
 // Importance
 // ------------------------------------------------------------------------------------------------
-// A CTA takes a tile of keys of one sequence and all heads, HB query heads of a kv head at a time: S^T = K Q^T with the keys as the
-// matrix's rows, so that a thread holds all queries and heads of its key and the sum over the heads needs no other thread.
+// A tile of keys of one sequence and all heads, HB query heads of a kv head at a time: S^T = K Q^T with the keys as the matrix's rows,
+// so that a thread holds all queries and heads of its key and the sum over the heads needs no other thread.  One CTA per SM goes
+// from tile to tile; what it works on next is on its way meanwhile.
 //   warps 0-3, 4-7   exponentials and sums, a key per thread, every other eight columns (column = query * HB + head) each
-//   warp 8           matrix products;  warp 9  copies (K of a kv head and the last queries of the HB heads)
-constexpr int IMP_THREADS = 320, IMP_COLUMNS = 128;   // columns: most per product
+//   warp 8           matrix products, into one of four places in tensor memory
+//   warp 9           copies (K of a kv head and the last queries of the HB heads)
+//   warp 10          the columns' denominators
+constexpr int IMP_THREADS = 384, IMP_COLUMNS = 128, IMP_SLOTS = 4, IMP_STAGES = 4;   // columns: most per product; slots: products in flight
 struct ImportanceShared {
-  unsigned long long full[4], empty[4], s_full[2], s_empty[2], drained;
+  unsigned long long full[IMP_STAGES], empty[IMP_STAGES], s_full[IMP_SLOTS], s_empty[IMP_SLOTS], drained;
   uint32_t tmem;
   int stop;
-  alignas(16) float lse[2][IMP_COLUMNS];
+  alignas(16) float log_sum[IMP_SLOTS][IMP_COLUMNS];
 };
 struct ImportanceShape {
-  int rows, keys, columns, stages;   // keys per tile; columns: rows * HB in whole 16
+  int rows, keys, columns, stages, tiles;   // keys per tile; columns: rows * HB in whole 16; tiles: as many as there can be
 };
-__host__ __device__ constexpr int imp_stage_bytes(const ImportanceShape& g) { return TILE_BYTES + g.columns * 256; }
-static size_t imp_smem(const ImportanceShape& g) {
-  return 1024 + g.stages * static_cast<size_t>(imp_stage_bytes(g)) + sizeof(float) * g.rows * TILE + sizeof(ImportanceShared);
+__host__ __device__ constexpr int imp_stage_bytes(const ImportanceShape& g) { return (g.keys + g.columns) * 256; }
+static size_t imp_smem(const ImportanceShape& g) {   // (a product reads 128 rows of K, the last of them beyond a short tile)
+  return 1024 + g.stages * static_cast<size_t>(imp_stage_bytes(g)) + (TILE - g.keys) * 128 + sizeof(ImportanceShared);
 }
-
 struct KeyCount {
   int keys;
   __device__ __forceinline__ int blocks(int, int lk) const { return (lk + keys - 1) / keys; }
@@ -621,137 +623,187 @@ struct KeyCount {
 };
 
 template <bool BF16, int HB>
-__global__ void __launch_bounds__(IMP_THREADS) importance_kernel(const __grid_constant__ PromptArgs A, const __grid_constant__ PromptMaps M,
-                                                                 const ImportanceShape G, const float* lse, __half* out) {
+__global__ void __launch_bounds__(IMP_THREADS, 1) importance_kernel(const __grid_constant__ PromptArgs A, const __grid_constant__ PromptMaps M,
+                                                                    const ImportanceShape G, const float* lse, __half* out) {
   extern __shared__ unsigned char raw[];
   unsigned char* const tiles = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~static_cast<uintptr_t>(1023));
-  const int stage_bytes = imp_stage_bytes(G);
-  float* const acc = reinterpret_cast<float*>(tiles + G.stages * stage_bytes);   // [rows][key]
-  ImportanceShared& sh = *reinterpret_cast<ImportanceShared*>(acc + G.rows * TILE);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  Place w;
-  if (!Walk<KeyCount>(A, KeyCount{G.keys}).find(blockIdx.x, w)) return;
-  const int q0 = w.q0, lq = w.lq, k0 = w.k0, lk = w.lk, j0 = w.block * G.keys;
-  const int t = min(G.rows, lq), first = q0 + lq - t;   // the queries
-  const int per_kv = A.nh_q / A.nh_kv / HB, items = t > 0 ? A.nh_kv * per_kv : 0;
+  const int stage_bytes = imp_stage_bytes(G), k_half = G.keys * 128;
+  ImportanceShared& sh = *reinterpret_cast<ImportanceShared*>(tiles + G.stages * stage_bytes + (TILE - G.keys) * 128);
+  const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
+  const int per_kv = A.nh_q / A.nh_kv / HB, items = A.nh_kv * per_kv;   // products per tile
   volatile int* const stop = &sh.stop;
-  if (warp == 8) tmem_alloc(smem_u32(&sh.tmem), 2 * IMP_COLUMNS);
+  if (warp == 8) tmem_alloc(smem_u32(&sh.tmem), IMP_SLOTS * IMP_COLUMNS);
   if (threadIdx.x == 0) {
     sh.stop = 0;
     bar_init(smem_u32(&sh.drained), 1);
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < IMP_STAGES; ++i) {
       bar_init(smem_u32(&sh.full[i]), 1);
       bar_init(smem_u32(&sh.empty[i]), 1);
     }
-    for (int i = 0; i < 2; ++i) {
-      bar_init(smem_u32(&sh.s_full[i]), 1);
+    for (int i = 0; i < IMP_SLOTS; ++i) {
+      bar_init(smem_u32(&sh.s_full[i]), 2);    // the product, the denominators
       bar_init(smem_u32(&sh.s_empty[i]), 8);
     }
     bar_init_fence();
   }
+  Walk<KeyCount> walk(A, KeyCount{G.keys});
+  Place w;
+  auto next = [&](int tile) { return tile < G.tiles && walk.find(tile, w); };   // (never more than the starts allow when in order)
   fence_before();
   __syncthreads();
   fence_after();
-  const uint32_t tmem = sh.tmem;
+  const uint32_t tmem = uniform(sh.tmem);
+  int slot = 0;
+  unsigned slot_phase = 0;
+  auto next_slot = [&] {
+    if (++slot == IMP_SLOTS) slot = 0, slot_phase ^= 1;
+  };
   if (warp < 8) {
-    const int side = warp >> 2, key = threadIdx.x & 127, j = j0 + key;
-    // the first of the t queries that sees this key
-    const int sees = A.causal ? j - (lk - t) : 0;
-    for (int r = side; r < G.rows; r += 2) acc[r * TILE + key] = 0.f;
+    const int side = warp >> 2, key = threadIdx.x & 127;
     const float scale = A.scale_log2;
-    const int column = threadIdx.x & 127, col_row = column / HB, col_head = column % HB;
-    auto denominator = [&](int item) {   // of the column that this thread looks after: log2, 0 where there is none
-      if (item >= items || col_row >= t) return 0.f;
-      return 1.4426950408889634f * __ldg(lse + static_cast<int64_t>(item * HB + col_head) * A.total_q + first + col_row);
-    };
+    const uint32_t lanes = tmem + (static_cast<uint32_t>(warp & 3) << 21) + 8 * side;
+    constexpr int CHUNKS = IMP_COLUMNS / 16, EACH = 8 / HB;   // this side's eights of columns, and the queries in each
     bool ok = true;
-    float next = denominator(0);
 #pragma unroll 1
-    for (int item = 0; item < items; ++item) {
-      float* const den = sh.lse[item & 1];
-      if (side == 0) den[column] = next;
-      asm volatile("bar.sync 1, 256;" ::: "memory");   // (a buffer is written again two items later: everyone has passed the barrier between)
-      next = denominator(item + 1);
-      ok = ok && __all_sync(0xffffffffu, bar_wait(smem_u32(&sh.s_full[item & 1]), item >> 1 & 1, stop));
-      if (!ok) continue;   // (every warp comes to every barrier)
-      fence_after();
-      const uint32_t at = tmem + (static_cast<uint32_t>(warp & 3) << 21) + (item & 1) * IMP_COLUMNS;
+    for (int tile = blockIdx.x; ok && next(tile); tile += gridDim.x) {
+      const int t = min(G.rows, w.lq), j = w.block * G.keys + key;
+      const int sees = A.causal ? j - (w.lk - t) : 0;   // the first of the t queries that sees this key
+      float sum[CHUNKS * EACH];
+#pragma unroll
+      for (int i = 0; i < CHUNKS * EACH; ++i) sum[i] = 0.f;
+      if (t > 0) {
 #pragma unroll 1
-      for (int c = 8 * side; c < G.columns; c += 16) {
-        uint32_t s[8];
-        tmem_load8(at + c, s);
-        const float4 d0 = *reinterpret_cast<const float4*>(den + c), d1 = *reinterpret_cast<const float4*>(den + c + 4);
-        const float d[8] = {d0.x, d0.y, d0.z, d0.w, d1.x, d1.y, d1.z, d1.w};
-        wait_loads(s);
+        for (int item = 0; item < items; ++item) {
+          if (!(ok = __all_sync(0xffffffffu, bar_wait(smem_u32(&sh.s_full[slot]), slot_phase, stop)))) break;
+          fence_after();
+          const uint32_t at = lanes + slot * IMP_COLUMNS;
+          const float* const log_sum = sh.log_sum[slot] + 8 * side;
+          // (chunks of 32 of this side's columns, so that loads and exponentials of several are under way)
 #pragma unroll
-        for (int k = 0; k < 8; k += HB) {
-          float sum = 0.f;
+          for (int c4 = 0; c4 < CHUNKS; c4 += 4) {
+            if (8 * side + 16 * c4 >= G.columns) break;
+            uint32_t s[32];
 #pragma unroll
-          for (int h = 0; h < HB; ++h) sum += exp2_approx(fmaf(__uint_as_float(s[k + h]), scale, -d[k + h]));
-          const int r = (c + k) / HB;
-          if (r < t && r >= sees) acc[r * TILE + key] += sum;
+            for (int c = 0; c < 4; ++c) tmem_load8(at + 16 * (c4 + c), s + 8 * c);   // (what lies behind the columns is not used)
+            wait_loads(s);
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+              if (8 * side + 16 * (c4 + c) >= G.columns) break;
+              const float4 d0 = *reinterpret_cast<const float4*>(log_sum + 16 * (c4 + c)), d1 = *reinterpret_cast<const float4*>(log_sum + 16 * (c4 + c) + 4);
+              const float d[8] = {d0.x, d0.y, d0.z, d0.w, d1.x, d1.y, d1.z, d1.w};
+#pragma unroll
+              for (int k = 0; k < 8; ++k) sum[(c4 + c) * EACH + k / HB] += exp2_approx(fmaf(__uint_as_float(s[8 * c + k]), scale, -d[k]));
+            }
+          }
+          fence_before();
+          __syncwarp();
+          if (lane == 0) bar_arrive(smem_u32(&sh.s_empty[slot]));
+          next_slot();
         }
       }
-      fence_before();
-      __syncwarp();
-      if (lane == 0) bar_arrive(smem_u32(&sh.s_empty[item & 1]));
+      if (ok && key < G.keys && j < w.lk) {
+        __half* const to = out + w.k0 + j;
+#pragma unroll
+        for (int i = 0; i < CHUNKS * EACH; ++i) {
+          const int r = (16 * (i / EACH) + 8 * side) / HB + i % EACH;
+          if (r < G.rows) to[static_cast<int64_t>(r) * A.total_k] = __float2half_rn(r < t && r >= sees ? sum[i] : 0.f);
+        }
+      }
     }
-    asm volatile("bar.sync 1, 256;" ::: "memory");
-    if (ok && j < lk && key < G.keys)
-      for (int r = side; r < G.rows; r += 2) out[static_cast<int64_t>(r) * A.total_k + k0 + j] = __float2half_rn(acc[r * TILE + key]);
   } else if (warp == 8) {
-    if (lane == 0) {
-      const uint32_t kind = mma_kind(BF16, TILE, G.columns, false), tiles_at = smem_u32(tiles), q_half = G.columns * 128;
-      bool ok = true;
-      int stage = 0;
-      unsigned phase = 0;
+    const uint32_t kind = mma_kind(BF16, TILE, G.columns, false);
+    const uint64_t first = operand(smem_u32(tiles), 16);
+    const int q_half = G.columns * 128;
+    bool ok = true;
+    int stage = 0;
+    unsigned phase = 0;
 #pragma unroll 1
-      for (int item = 0; item < items; ++item) {
-        if (!(ok = bar_wait(smem_u32(&sh.full[stage]), phase, stop) &&
-                   bar_wait(smem_u32(&sh.s_empty[item & 1]), (item >> 1 & 1) ^ 1, stop))) break;
+    for (int tile = blockIdx.x; ok && next(tile); tile += gridDim.x) {
+      const int n = uniform(w.lq > 0 ? items : 0);
+#pragma unroll 1
+      for (int item = 0; item < n; ++item) {
+        if (!(ok = bar_wait(smem_u32(&sh.full[stage]), phase, stop) && bar_wait(smem_u32(&sh.s_empty[slot]), slot_phase ^ 1, stop))) break;
         fence_after();
-        const uint32_t k_at = tiles_at + stage * stage_bytes, q_at = k_at + TILE_BYTES;
+        if (elect_one()) {
+          const uint64_t k_at = first + (stage * stage_bytes >> 4), q_at = k_at + (G.keys * 256 >> 4);
 #pragma unroll
-        for (int c = 0; c < 8; ++c)
-          mma_shared(tmem + (item & 1) * IMP_COLUMNS, operand(k_at + (c >> 2) * (TILE_BYTES / 2) + (c & 3) * 32, 16),
-                     operand(q_at + (c >> 2) * q_half + (c & 3) * 32, 16), kind, c > 0);
-        mma_commit(smem_u32(&sh.s_full[item & 1]));
-        mma_commit(smem_u32(&sh.empty[stage]));
-        if (++stage == G.stages) stage = 0, phase ^= 1;
-      }
-      if (!ok) {   // products in flight end before the CTA does
-        mma_commit(smem_u32(&sh.drained));
-        for (int k = 0; k < WAIT_TRIES && !bar_try(smem_u32(&sh.drained), 0); ++k) {
+          for (int c = 0; c < 8; ++c)
+            mma_shared(tmem + slot * IMP_COLUMNS, k_at + (((c >> 2) * k_half + (c & 3) * 32) >> 4), q_at + (((c >> 2) * q_half + (c & 3) * 32) >> 4), kind, c > 0);
+          mma_commit(smem_u32(&sh.s_full[slot]));
+          mma_commit(smem_u32(&sh.empty[stage]));
         }
+        if (++stage == G.stages) stage = 0, phase ^= 1;
+        next_slot();
       }
     }
-  } else if (lane == 0) {
+    if (!ok && lane == 0) {   // products in flight end before the CTA does
+      mma_commit(smem_u32(&sh.drained));
+      for (int k = 0; k < WAIT_TRIES && !bar_try(smem_u32(&sh.drained), 0); ++k) {
+      }
+    }
+  } else if (warp == 9) {
     const uint32_t tiles_at = smem_u32(tiles);
     const unsigned bytes = 256u * (G.keys + G.rows * HB);
     bool ok = true;
-    int stage = 0, item = 0;
+    int stage = 0, used = 0;
     unsigned phase = 1;
 #pragma unroll 1
-    for (; item < items; ++item) {
-      if (!(ok = bar_wait(smem_u32(&sh.empty[stage]), phase, stop))) break;
-      const uint32_t k_at = tiles_at + stage * stage_bytes, q_at = k_at + TILE_BYTES, bar = smem_u32(&sh.full[stage]);
-      bar_expect(bar, bytes);
-      for (int c = 0; c < 2; ++c) {
-        copy_box(k_at + c * (TILE_BYTES / 2), &M.k, 64 * c, item / per_kv, k0 + j0, bar);
-        copy_box(q_at + c * G.columns * 128, &M.q, 64 * c, item * HB, first, bar);
-      }
-      if (++stage == G.stages) stage = 0, phase ^= 1;
-    }
-    if (!ok)   // copies in flight land before the CTA ends
-      for (int i = max(0, item - G.stages); i < item; ++i)
-        for (int k = 0; k < WAIT_TRIES && !bar_try(smem_u32(&sh.full[i % G.stages]), i / G.stages & 1); ++k) {
+    for (int tile = blockIdx.x; ok && next(tile); tile += gridDim.x) {
+      const int n = w.lq > 0 ? items : 0, token = w.k0 + w.block * G.keys, query = w.q0 + w.lq - min(G.rows, w.lq);
+      if (lane == 0)
+#pragma unroll 1
+        for (int item = 0; item < n; ++item) {
+          if (!(ok = bar_wait(smem_u32(&sh.empty[stage]), phase, stop))) break;
+          const uint32_t k_at = tiles_at + stage * stage_bytes, q_at = k_at + G.keys * 256, bar = smem_u32(&sh.full[stage]);
+          bar_expect(bar, bytes);
+          for (int c = 0; c < 2; ++c) {
+            copy_box(k_at + c * k_half, &M.k, 64 * c, item / per_kv, token, bar);
+            copy_box(q_at + c * G.columns * 128, &M.q, 64 * c, item * HB, query, bar);
+          }
+          if (used < G.stages) ++used;
+          if (++stage == G.stages) stage = 0, phase ^= 1;
         }
+      ok = __all_sync(0xffffffffu, ok);
+    }
+    if (!ok && lane == 0)   // copies in flight land before the CTA ends: the last `used` of them, in front of `stage`
+      for (int i = 1; i <= used; ++i) {
+        const int at = (stage - i + G.stages) % G.stages;
+        const unsigned parity = at < stage ? phase ^ 1 : phase;
+        for (int k = 0; k < WAIT_TRIES && !bar_try(smem_u32(&sh.full[at]), parity); ++k) {
+        }
+      }
+  } else if (warp == 10) {
+    bool ok = true;
+#pragma unroll 1
+    for (int tile = blockIdx.x; ok && next(tile); tile += gridDim.x) {
+      const int t = min(G.rows, w.lq), n = w.lq > 0 ? items : 0;
+      const float* const from = lse + w.q0 + w.lq - t;
+      float v[4];
+      auto load = [&](int item) {   // log2; 0 where a column is no query's
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const int column = lane + 32 * k, r = column / HB, head = item * HB + column % HB;
+          v[k] = item < n && r < t ? 1.4426950408889634f * __ldg(from + static_cast<int64_t>(head) * A.total_q + r) : 0.f;
+        }
+      };
+      load(0);
+#pragma unroll 1
+      for (int item = 0; item < n; ++item) {
+        if (!(ok = __all_sync(0xffffffffu, bar_wait(smem_u32(&sh.s_empty[slot]), slot_phase ^ 1, stop)))) break;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) sh.log_sum[slot][lane + 32 * k] = v[k];
+        load(item + 1);
+        __syncwarp();
+        if (lane == 0) bar_arrive(smem_u32(&sh.s_full[slot]));
+        next_slot();
+      }
+    }
   }
   __syncwarp();
   fence_before();
   __syncthreads();
   fence_after();
-  if (warp == 8) tmem_free(tmem, 2 * IMP_COLUMNS);
+  if (warp == 8) tmem_free(tmem, IMP_SLOTS * IMP_COLUMNS);
   if (threadIdx.x == 0 && *stop) atomicAdd(&g_waits_expired, 1u);
 }
 
@@ -888,8 +940,7 @@ static int launch_importance(const PromptArgs& A, const PromptMaps& M, const Imp
     HQKV_CUDA(cudaFuncSetAttribute(importance_kernel<BF16, HB>, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024));
     if (dev >= 0 && dev < 64) opted_in[dev] = true;
   }
-  const int64_t n = max(1, min(A.n_seqs, A.total_k)), blocks = (A.total_k + n * (G.keys - 1)) / G.keys;
-  importance_kernel<BF16, HB><<<static_cast<unsigned>(blocks), IMP_THREADS, imp_smem(G), st>>>(A, M, G, lse, out);
+  importance_kernel<BF16, HB><<<min(G.tiles, PROMPT_CTAS), IMP_THREADS, imp_smem(G), st>>>(A, M, G, lse, out);
   HQKV_LAUNCH_CHECK("importance");
   return HQKV_OK;
 }
@@ -900,11 +951,14 @@ static int launch_importance(const PromptArgs& A, const float* lse, int rows, __
   ImportanceShape G;
   G.rows = rows;
   G.columns = (rows * hb + 15) / 16 * 16;
-  // as many tiles as two CTAs per SM take at once, of 64 to 128 keys
-  const int64_t waves = ceil_div(A.total_k, 296 * TILE), keys = ceil_div(ceil_div(A.total_k, 296 * waves), 8) * 8;
-  G.keys = static_cast<int>(max(int64_t{64}, min(int64_t{TILE}, keys)));
-  G.stages = 4;
-  while (G.stages > 2 && imp_smem(G) > 113 * 1024) --G.stages;
+  // tiles of at most 128 keys, as many as make whole rounds of the CTAs (a sequence's last tile is half empty, on average)
+  const int64_t n = max(1, min(A.n_seqs, A.total_k)), rounds = ceil_div(A.total_k + n * TILE / 2, PROMPT_CTAS * TILE);
+  const int64_t keys = ceil_div(ceil_div(A.total_k, max(int64_t{1}, rounds * PROMPT_CTAS - n / 2)), 8) * 8;
+  G.keys = static_cast<int>(max(int64_t{32}, min(int64_t{TILE}, keys)));
+  const int64_t tiles = (A.total_k + n * (G.keys - 1)) / G.keys;
+  G.tiles = static_cast<int>(tiles);   // (below 2^30 / 32 + 2^24)
+  G.stages = IMP_STAGES;
+  while (G.stages > 2 && imp_smem(G) > 227 * 1024) --G.stages;
   PromptMaps M = {};
   if (A.total_q > 0)
     if (int rc = tensor_map(&M.q, A.q, A.bf16, A.total_q, A.nh_q, A.q_token, A.q_head, hb, rows)) return rc;
