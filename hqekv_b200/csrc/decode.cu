@@ -2453,12 +2453,12 @@ struct JoinParams {
   const float2* k_part;    // the cache's softmax pairs, logits and unrounded outputs, as the two passes leave them
   const float* logits;
   const float* own;
-  const float* part_o;     // [splits][B * nh_q][D], [splits][B * nh_q]
+  const float* part_o;     // [parts][B * nh_q][D], [parts][B * nh_q]
   const float2* part_ml;
   __half *out, *weights;
-  int nk_ctas, r4, L, rows, splits;
+  int nk_ctas, r4, L, rows, parts;
 };
-constexpr int JOIN_THREADS = 128, JOIN_TOKENS = 2048;   // tokens whose weights a CTA writes
+constexpr int JOIN_THREADS = 128, JOIN_TOKENS = 2048, JOIN_PARTS = 148;   // tokens whose weights a CTA writes; most parts
 static_assert(JOIN_THREADS == D, "a thread per channel");
 
 // CTA: a (sequence, query head) and a share of its own tokens.  With M the largest of all logits (base 2) the parts' outputs are
@@ -2466,41 +2466,52 @@ static_assert(JOIN_THREADS == D, "a thread per channel");
 // fp32 logits again: scaling the fp16 probabilities that the V pass has written would round them twice.
 __global__ void __launch_bounds__(JOIN_THREADS) join_prefix_kernel(const __grid_constant__ JoinParams P) {
   const int row = blockIdx.x, tid = threadIdx.x, plane = row / P.r4, head = row - plane * P.r4;
-  __shared__ float2 warp_ml[JOIN_THREADS / 32];
-  // (maximum, sum) of the cache, in base 2
-  float m = -INFINITY, l = 0.f;
+  __shared__ float2 warp_ml[2][JOIN_THREADS / 32];
+  __shared__ float part_f[JOIN_PARTS];
   const float2* pairs = P.k_part + static_cast<int64_t>(row) * P.nk_ctas;
-  auto add = [&](float m2, float l2) {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  // (maximum, sum) of the cache and of the prefix, in base 2
+  float m = -INFINITY, l = 0.f, pm = -INFINITY, pl = 0.f;
+  auto add = [](float& m, float& l, float m2, float l2) {
     const float mx = fmaxf(m, m2), ref = mx == -INFINITY ? 0.f : mx;
     l = l * fast_exp2(m - ref) + l2 * fast_exp2(m2 - ref);
     m = mx;
   };
-  for (int c = tid; c < P.nk_ctas; c += JOIN_THREADS) add(pairs[c].x * LOG2E, pairs[c].y);
+  for (int c = tid; c < P.nk_ctas; c += JOIN_THREADS) add(m, l, pairs[c].x * LOG2E, pairs[c].y);
+  for (int s = tid; s < P.parts; s += JOIN_THREADS) {
+    const float2 part = P.part_ml[static_cast<int64_t>(s) * P.rows + row];
+    add(pm, pl, part.x, part.y);
+    part_f[s] = part.x;
+  }
 #pragma unroll
-  for (int k = 1; k < 32; k <<= 1) add(__shfl_xor_sync(0xffffffffu, m, k), __shfl_xor_sync(0xffffffffu, l, k));
-  if ((tid & 31) == 0) warp_ml[tid >> 5] = make_float2(m, l);
+  for (int k = 1; k < 32; k <<= 1) {
+    add(m, l, __shfl_xor_sync(0xffffffffu, m, k), __shfl_xor_sync(0xffffffffu, l, k));
+    add(pm, pl, __shfl_xor_sync(0xffffffffu, pm, k), __shfl_xor_sync(0xffffffffu, pl, k));
+  }
+  if ((tid & 31) == 0) warp_ml[0][tid >> 5] = make_float2(m, l), warp_ml[1][tid >> 5] = make_float2(pm, pl);
   __syncthreads();
   m = -INFINITY, l = 0.f;
-  for (int w = 0; w < JOIN_THREADS / 32; ++w) add(warp_ml[w].x, warp_ml[w].y);
+#pragma unroll
+  for (int w = 0; w < JOIN_THREADS / 32; ++w) add(m, l, warp_ml[0][w].x, warp_ml[0][w].y);
   const float own_m = m, own_l = l;
-  for (int s = 0; s < P.splits; ++s) {
-    const float2 part = P.part_ml[static_cast<int64_t>(s) * P.rows + row];
-    add(part.x, part.y);
-  }
+#pragma unroll
+  for (int w = 0; w < JOIN_THREADS / 32; ++w) add(m, l, warp_ml[1][w].x, warp_ml[1][w].y);
   const float ref = m == -INFINITY ? 0.f : m, inv = 1.f / l;
   if (blockIdx.y == 0) {
     const int64_t at = static_cast<int64_t>(row) * D + tid;
     float o = own_l * fast_exp2(own_m - ref) * P.own[at];
-    for (int s = 0; s < P.splits; ++s) {
-      const int64_t r = static_cast<int64_t>(s) * P.rows + row;
-      const float2 part = P.part_ml[r];
-      if (part.y != 0.f) o += fast_exp2(part.x - ref) * P.part_o[r * D + tid];   // (a split without tokens has no output)
+    const float* from = P.part_o + at;
+#pragma unroll 8
+    for (int s = 0; s < P.parts; ++s) {   // (every part has tokens, and a row that sees them)
+      o += fast_exp2(part_f[s] - ref) * *from;
+      from += static_cast<int64_t>(P.rows) * D;
     }
     P.out[at] = __float2half_rn(o * inv);
   }
   const float* logits = P.logits + static_cast<int64_t>(plane) * P.r4 * P.L;
   __half* weights = P.weights + static_cast<int64_t>(row) * P.L;
   const int end = min(P.L, (static_cast<int>(blockIdx.y) + 1) * JOIN_TOKENS);
+#pragma unroll 4
   for (int t = blockIdx.y * JOIN_TOKENS + tid; t < end; t += JOIN_THREADS)
     weights[t] = __float2half_rn(fast_exp2(fmaf(logits[logit_at(t, head, P.r4, P.L)], LOG2E, -ref)) * inv);
 }
@@ -2519,11 +2530,11 @@ static hqkv_prompt_t prefix_of(const hqkv_cache_desc_t* c, int64_t prefix_len) {
   p.prefix_len = prefix_len;
   return p;
 }
-static size_t join_bytes(const hqkv_cache_desc_t* c, int splits, size_t* part_o, size_t* part_ml) {
+static size_t join_bytes(const hqkv_cache_desc_t* c, int parts, size_t* part_o, size_t* part_ml) {
   const size_t rows = static_cast<size_t>(c->B) * c->nh_q;
   *part_o = rows * D * sizeof(float);   // (behind the cache's outputs)
-  *part_ml = *part_o + splits * rows * D * sizeof(float);
-  return *part_ml + splits * rows * sizeof(float2);
+  *part_ml = *part_o + parts * rows * D * sizeof(float);
+  return *part_ml + parts * rows * sizeof(float2);
 }
 }  // namespace hqkv
 
@@ -2533,7 +2544,7 @@ extern "C" size_t hqkv_decode_prefix_workspace_bytes(const hqkv_cache_desc_t* ca
   if (build_params(cache_host, P, lay) != HQKV_OK || prefix_len < 1 || prefix_len >= (1ll << 30)) return 0;
   const hqkv_prompt_t p = prefix_of(cache_host, prefix_len);
   size_t o, ml;
-  return join_bytes(cache_host, prefix_shares(&p), &o, &ml);
+  return join_bytes(cache_host, prefix_parts(&p), &o, &ml);
 }
 
 extern "C" int hqkv_decode_attention_prefix(const hqkv_cache_desc_t* cache_host, const void* q, const void* prefix_k, const void* prefix_v,
@@ -2550,9 +2561,9 @@ extern "C" int hqkv_decode_attention_prefix(const hqkv_cache_desc_t* cache_host,
   p.q = q, p.prefix_k = prefix_k, p.prefix_v = prefix_v;
   p.prefix_k_token = k_token, p.prefix_k_head = k_head, p.prefix_v_token = v_token, p.prefix_v_head = v_head;
   JoinParams J = {};
-  J.splits = prefix_shares(&p);
+  J.parts = prefix_parts(&p);
   size_t o, ml;
-  const size_t need = join_bytes(cache_host, J.splits, &o, &ml);
+  const size_t need = join_bytes(cache_host, J.parts, &o, &ml);
   if (prefix_workspace_bytes < need)
     return fail(HQKV_E_WORKSPACE, "decode_prefix: the prefix workspace holds %zu bytes, %zu needed", prefix_workspace_bytes, need);
   unsigned char* pw = static_cast<unsigned char*>(prefix_workspace);
@@ -2570,8 +2581,17 @@ extern "C" int hqkv_decode_attention_prefix(const hqkv_cache_desc_t* cache_host,
   J.out = static_cast<__half*>(attn_output);
   J.weights = static_cast<__half*>(attn_weights);
   J.nk_ctas = P.nk_ctas, J.r4 = P.r4, J.L = P.L, J.rows = P.B * P.nh_q;
-  join_prefix_kernel<<<dim3(J.rows, static_cast<unsigned>(ceil_div(P.L, JOIN_TOKENS))), JOIN_THREADS, 0, st>>>(J);
-  HQKV_LAUNCH_CHECK("join_prefix");
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(P.B * P.nh_q, static_cast<unsigned>(ceil_div(P.L, JOIN_TOKENS)));
+  cfg.blockDim = dim3(JOIN_THREADS);
+  cfg.stream = st;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  HQKV_REQUIRE(J.parts <= JOIN_PARTS, "decode_prefix: too many parts");
+  HQKV_CUDA(cudaLaunchKernelEx(&cfg, join_prefix_kernel, J));
   return HQKV_OK;
 }
 

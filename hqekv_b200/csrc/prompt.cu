@@ -46,11 +46,12 @@ constexpr int BY_POLYNOMIAL = 0;                         // of 16 pairs of expon
 
 struct PromptShared {
   unsigned long long q_full, q_empty, kv_full[KV_STAGES], kv_empty[KV_STAGES], v_raw[KV_STAGES];
-  unsigned long long s_full[2], p_first[2], p_rest[2], o_full[2], o_empty[2], turn[2], drained[2];
+  unsigned long long s_full[2], p_first[2], p_rest[2], o_full[2], o_empty[2], turn[2], drained[2], pair_full[4], pair_done[4];
   uint32_t tmem;
+  float2 pair_ml[2][TILE];   // (maximum, sum) of the rows of a paired item's halves
   int stop, odd[4];   // odd: the last item (by its number, of those with the same two low bits) in which warp 10 found infinities or NaN
 };
-constexpr size_t PROMPT_SMEM = 1024 + (2 + KV_STAGES) * static_cast<size_t>(TILE_BYTES) + sizeof(PromptShared);
+constexpr size_t PROMPT_SMEM = (2 + KV_STAGES) * static_cast<size_t>(TILE_BYTES) + sizeof(PromptShared);
 static_assert(PROMPT_SMEM <= 227 * 1024, "one CTA per SM");
 
 static __device__ unsigned g_waits_expired;
@@ -62,7 +63,7 @@ __device__ __forceinline__ int keys_seen(const PromptArgs& A, int i, int lq, int
 __device__ __forceinline__ int tiles_of(int keys) { return (keys + TILE - 1) / TILE; }
 // shares that the keys of a sequence's blocks are divided into
 __device__ __forceinline__ int shares_of(const PromptArgs& A, int lq, int lk) {
-  return max(1, (tiles_of(A.prefix_len) + tiles_of(keys_seen(A, lq - 1, lq, lk)) + A.per_share - 1) / A.per_share);
+  return A.shares == 1 ? 1 : max(1, (tiles_of(A.prefix_len) + tiles_of(keys_seen(A, lq - 1, lq, lk)) + A.per_share - 1) / A.per_share);
 }
 
 // Walks the sequences in order, 32 at a time (a lane each), to the one that holds an item; items are asked for in rising order.
@@ -107,8 +108,8 @@ struct Walk {
     auto get = [&](int v) { return __shfl_sync(0xffffffffu, v, from); };
     p.q0 = get(q0), p.lq = get(lq), p.k0 = get(k0), p.lk = get(lk);
     const int each = count.each(p.lq, p.lk), blocks = count.blocks(p.lq, p.lk);
-    const int i = item - static_cast<int>(before + __shfl_sync(0xffffffffu, sum, from) - static_cast<long long>(blocks) * each);
-    p.block = blocks - 1 - i / each, p.rest = i % each;
+    const int i = item - static_cast<int>(before + __shfl_sync(0xffffffffu, sum, from) - static_cast<long long>(blocks) * each), at_block = i / each;
+    p.block = blocks - 1 - at_block, p.rest = i - at_block * each;
     return true;
   }
 };
@@ -144,8 +145,13 @@ __device__ __forceinline__ void exp2_polynomial(uint64_t x2, float& a, float& b)
 struct Item {
   Place at;
   int head0, kv, share, shares, i0;        // i0: the block's first query in its sequence
+  bool part, paired;                       // the result is a part of the rows'; one row tile of queries, on which both halves of the CTA work
   int before, seen_first, seen_last;       // tiles of the prefix; own keys that the block's first and last query see
   int lo, hi, hi0, hi1;                    // tiles of keys: [lo, hi), of which the row tiles see those below hi0 and hi1
+  // The tiles that row tile a works on: all that it sees, or of a paired item every other one.
+  __device__ __forceinline__ int first(int a) const { return lo + (paired ? a : 0); }
+  __device__ __forceinline__ int end(int a) const { return a && !paired ? hi1 : hi0; }
+  __device__ __forceinline__ int step() const { return paired ? 2 : 1; }
   // Own V tiles that hold keys which some rows of the block do not see.  0 x NaN is NaN in a matrix product, so what lies behind
   // the last key that any row sees is set to 0; an infinity or NaN that only some rows see is set to 0 as well, and those rows
   // add it at the end.
@@ -153,19 +159,22 @@ struct Item {
 };
 struct ItemCount {
   const PromptArgs& A;
-  __device__ __forceinline__ int blocks(int lq, int) const { return (lq + 2 * TILE / A.group - 1) / (2 * TILE / A.group); }
-  __device__ __forceinline__ int each(int lq, int lk) const { return A.nh_q / A.group * shares_of(A, lq, lk); }
+  __device__ __forceinline__ int blocks(int lq, int) const { return (lq + (1 << A.block_shift) - 1) >> A.block_shift; }
+  __device__ __forceinline__ int each(int lq, int lk) const { return A.groups * shares_of(A, lq, lk); }
 };
 __device__ __forceinline__ bool next_item(const PromptArgs& A, Walk<ItemCount>& walk, int round, Item& w) {
   // (every other round backwards: the first items of a causal prompt are the longest)
   const int item = round * static_cast<int>(gridDim.x) + (round & 1 ? static_cast<int>(gridDim.x - 1 - blockIdx.x) : static_cast<int>(blockIdx.x));
   if (item >= A.items || !walk.find(item, w.at)) return false;   // (more than there can be: the starts are not in order)
-  const int lq = w.at.lq, lk = w.at.lk, half = TILE / A.group, groups = A.nh_q / A.group, group = w.at.rest % groups;
+  const int lq = w.at.lq, lk = w.at.lk, half = 1 << (A.block_shift - 1);
   w.shares = shares_of(A, lq, lk);
-  w.share = w.at.rest / groups;
+  w.share = A.shares == 1 ? 0 : w.at.rest / A.groups;
+  const int group = w.at.rest - w.share * A.groups;
   w.head0 = group * A.group;
-  w.kv = w.head0 / (A.nh_q / A.nh_kv);
-  w.i0 = w.at.block * 2 * half;
+  w.kv = group / A.groups_per_kv;
+  w.i0 = w.at.block << A.block_shift;
+  w.part = A.partial || w.shares > 1;
+  w.paired = w.i0 + half >= lq;
   w.before = tiles_of(A.prefix_len);
   w.seen_first = keys_seen(A, w.i0, lq, lk);
   w.seen_last = keys_seen(A, min(w.i0 + 2 * half, lq) - 1, lq, lk);
@@ -180,12 +189,12 @@ __device__ __forceinline__ bool next_item(const PromptArgs& A, Walk<ItemCount>& 
 template <bool BF16>
 __global__ void __launch_bounds__(PROMPT_THREADS, 1) prompt_kernel(const __grid_constant__ PromptArgs A, const __grid_constant__ PromptMaps M) {
   using T = std::conditional_t<BF16, __nv_bfloat16, __half>;
-  extern __shared__ unsigned char raw[];
-  unsigned char* const tiles = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  extern __shared__ __align__(1024) unsigned char tiles[];
   PromptShared& sh = *reinterpret_cast<PromptShared*>(tiles + (2 + KV_STAGES) * TILE_BYTES);
   const uint32_t q_at = smem_u32(tiles), kv_at = q_at + 2 * TILE_BYTES;
   const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
-  const int half = TILE / A.group;   // tokens per row tile
+  asm volatile("griddepcontrol.launch_dependents;");   // (a kernel behind this one waits for its end before it reads results)
+  const int half = 1 << (A.block_shift - 1);   // tokens per row tile
   volatile int* const stop = &sh.stop;
   if (warp == 8) tmem_alloc(smem_u32(&sh.tmem), TMEM_COLUMNS);
   if (threadIdx.x == 0) {
@@ -207,34 +216,41 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1) prompt_kernel(const __grid_
       bar_init(smem_u32(&sh.turn[a]), 1);
       bar_init(smem_u32(&sh.drained[a]), 1);
     }
+    for (int i = 0; i < 4; ++i) {
+      bar_init(smem_u32(&sh.pair_full[i]), 2);
+      bar_init(smem_u32(&sh.pair_done[i]), 2);
+    }
     bar_init_fence();
   }
-  Walk<ItemCount> walk(A, ItemCount{A});
-  Item w;
+  if (warp == 9 && lane < 5) prefetch_map(lane == 0 ? &M.q : lane == 1 ? &M.k : lane == 2 ? &M.v : lane == 3 ? &M.pk : &M.pv);
   fence_before();
   __syncthreads();
   fence_after();
   const uint32_t tmem = uniform(sh.tmem);
+  // (nothing before this reads or writes what an earlier kernel may still be working on)
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  Walk<ItemCount> walk(A, ItemCount{A});
+  Item w;
 
   // 384 threads are launched with 168 registers each: 2 x 128 x 208 + 128 x 88 = 384 x 168
   if (warp < 8) more_registers<208>();
   else fewer_registers<88>();
   if (warp < 8) {
     // ---- softmax
-    const int a = warp >> 2, row = threadIdx.x & 127, token = a * half + row / A.group;
+    const int a = warp >> 2, row = threadIdx.x & 127, token = row / A.group;
     const uint32_t lanes = tmem + (static_cast<uint32_t>(warp & 3) << 21);   // (32 lanes a warp, in bits 16 and up)
     const uint32_t s_at = lanes + a * TILE, o_at = lanes + 2 * TILE + a * 128;
     const float scale = A.scale_log2;
-    unsigned s_phase = 0, o_phase = 0;
+    unsigned s_phase = 0, o_phase = 0, pair_phase = 0;
     bool ok = true;
 #pragma unroll 1
     for (int round = 0; ok && next_item(A, walk, round, w); ++round) {
-      const int i = w.i0 + token, head = w.head0 + row % A.group, end = a ? w.hi1 : w.hi0;
+      const int i = w.i0 + token + (w.paired ? 0 : a * half), head = w.head0 + row % A.group, first = w.first(a), end = w.end(a), step = w.step();
       const bool live = i < w.at.lq;
       const int seen = live ? keys_seen(A, i, w.at.lq, w.at.lk) : w.at.lk;
       float ref = -INFINITY, sum = 0.f;
 #pragma unroll 1
-      for (int tile = w.lo; tile < end; ++tile) {
+      for (int tile = first; tile < end; tile += step) {
         if (!(ok = __all_sync(0xffffffffu, bar_wait(smem_u32(&sh.s_full[a]), s_phase, stop)))) break;
         s_phase ^= 1;
         fence_after();
@@ -260,7 +276,7 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1) prompt_kernel(const __grid_
           const float f = grown ? exp2_approx(ref - top) : 1.f;
           if (grown) ref = top;
           sum *= f;
-          if (tile > w.lo) {
+          if (tile > first) {
             // (the product with the tile before, which was issued before this S, is complete)
 #pragma unroll 1
             for (int c = 0; c < 128; c += 32) {
@@ -313,37 +329,19 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1) prompt_kernel(const __grid_
       }
       if (!ok) break;
       // ---- output
-      const bool any = end > w.lo, part = A.partial || w.shares > 1;
-      const int64_t at = static_cast<int64_t>(w.at.q0 + i) * A.nh_q + head, rows = static_cast<int64_t>(A.total_q) * A.nh_q;
-      const float by = part ? 1.f : sum == 0.f ? 0.f : 1.f / sum;
-      if (live && part) A.part_ml[w.share * rows + at] = make_float2(ref, sum);
-      else if (live) A.lse[static_cast<int64_t>(head) * A.total_q + w.at.q0 + i] = sum == 0.f ? -INFINITY : (ref + log2f(sum)) * 0.6931471805599453f;
+      const bool any = end > first;
       if (any) {
         if (!(ok = __all_sync(0xffffffffu, bar_wait(smem_u32(&sh.o_full[a]), o_phase, stop)))) break;
         o_phase ^= 1;
         fence_after();
-      } else if (part) {
-        continue;   // (nobody reads a part whose sum is 0)
       }
-      const bool odd = *const_cast<volatile int*>(&sh.odd[round & 3]) == round;
-#pragma unroll 1
-      for (int c = 0; c < 128; c += 32) {
-        uint32_t o[32];
-        if (any) {
-          tmem_load32(o_at + c, o);
-          wait_loads(o);
-          if (c == 96) {
-            fence_before();
-            __syncwarp();
-            if (lane == 0) bar_arrive(smem_u32(&sh.o_empty[a]));
-          }
-        } else {
-#pragma unroll
-          for (int k = 0; k < 32; ++k) o[k] = 0u;
-        }
-        if (!live) continue;
+      const int64_t at = static_cast<int64_t>(w.at.q0 + i) * A.nh_q + head, rows = static_cast<int64_t>(A.total_q) * A.nh_q;
+      bool odd = *const_cast<volatile int*>(&sh.odd[round & 3]) == round;
+      // 32 channels of the row, not yet normalised, from `o`
+      auto store = [&](uint32_t (&o)[32], int c, float by) {
+        if (!live) return;
         if (odd) {
-          const int to = min(seen, (end - w.before) * TILE);
+          const int to = min(seen, (w.hi - w.before) * TILE);
           for (int j = max(w.seen_first, (w.lo - w.before) * TILE); j < to; ++j) {
             const T* v = static_cast<const T*>(A.v) + (w.at.k0 + j) * A.v_token + w.kv * A.v_head + c;
 #pragma unroll
@@ -353,7 +351,7 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1) prompt_kernel(const __grid_
             }
           }
         }
-        if (part) {
+        if (w.part) {
           uint4* to = reinterpret_cast<uint4*>(A.part_o + (w.share * rows + at) * 128 + c);
 #pragma unroll
           for (int k = 0; k < 8; ++k) to[k] = make_uint4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]);
@@ -365,6 +363,64 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1) prompt_kernel(const __grid_
 #pragma unroll
           for (int k = 0; k < 4; ++k) to[k] = make_uint4(h[4 * k], h[4 * k + 1], h[4 * k + 2], h[4 * k + 3]);
         }
+      };
+      auto statistics = [&](float ref, float sum) {
+        if (!live) return;
+        if (w.part) A.part_ml[w.share * rows + at] = make_float2(ref, sum);
+        else A.lse[static_cast<int64_t>(head) * A.total_q + w.at.q0 + i] = sum == 0.f ? -INFINITY : (ref + log2f(sum)) * 0.6931471805599453f;
+      };
+      if (!w.paired) {
+        statistics(ref, sum);
+        if (!any && w.part) continue;   // (nobody reads a part whose sum is 0)
+        const float by = sum == 0.f ? 0.f : 1.f / sum;
+#pragma unroll 1
+        for (int c = 0; c < 128; c += 32) {
+          uint32_t o[32] = {};
+          if (any) {
+            tmem_load32(o_at + c, o);
+            wait_loads(o);
+            if (c == 96) {
+              fence_before();
+              __syncwarp();
+              if (lane == 0) bar_arrive(smem_u32(&sh.o_empty[a]));
+            }
+          }
+          store(o, c, by);
+        }
+      } else {
+        // The halves of the CTA have every other tile of the same rows: a warp of each (which can read the same part of tensor memory)
+        // joins 64 channels of both.
+        const bool others = w.end(a ^ 1) > w.first(a ^ 1);
+        sh.pair_ml[a][row] = make_float2(ref, sum);
+        fence_before();
+        __syncwarp();
+        if (lane == 0) bar_arrive(smem_u32(&sh.pair_full[warp & 3]));
+        if (!(ok = __all_sync(0xffffffffu, bar_wait(smem_u32(&sh.pair_full[warp & 3]), pair_phase, stop)))) break;
+        fence_after();
+        odd = *const_cast<volatile int*>(&sh.odd[round & 3]) == round;   // (found in the other half's tiles, maybe)
+        const float2 other = sh.pair_ml[a ^ 1][row];
+        const float top = fmaxf(ref, other.x), base = top == -INFINITY ? 0.f : top;
+        // (a half without tiles has nothing in tensor memory)
+        const float f = any ? exp2_approx(ref - base) : 0.f, g = others ? exp2_approx(other.x - base) : 0.f, all = f * sum + g * other.y;
+        if (a == 0) statistics(top, all);
+        const float by = all == 0.f ? 0.f : 1.f / all;
+#pragma unroll 1
+        for (int c = 64 * a; c < 64 * a + 64; c += 32) {
+          uint32_t o[32] = {}, x[32] = {};
+          if (any) tmem_load32(o_at + c, o);
+          if (others) tmem_load32(lanes + 2 * TILE + (a ^ 1) * 128 + c, x);
+          wait_loads(o);
+          wait_loads(x);
+#pragma unroll
+          for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(f * __uint_as_float(o[k]) + g * __uint_as_float(x[k]));
+          store(o, c, by);
+        }
+        fence_before();
+        __syncwarp();
+        if (lane == 0) bar_arrive(smem_u32(&sh.pair_done[warp & 3]));
+        if (!(ok = __all_sync(0xffffffffu, bar_wait(smem_u32(&sh.pair_done[warp & 3]), pair_phase, stop)))) break;
+        pair_phase ^= 1;
+        if (any && lane == 0) bar_arrive(smem_u32(&sh.o_empty[a]));
       }
     }
   } else if (warp == 8 || warp == 11) {
@@ -372,9 +428,10 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1) prompt_kernel(const __grid_
     //      complete already) and issuing, and either softmax waited for it: 8 k tokens, all seen: 866 us with one, 832 with two.
     constexpr uint32_t kind_s = mma_kind(BF16, TILE, TILE, false), kind_o = mma_kind(BF16, TILE, 128, true);
     const int a = warp == 8 ? 0 : 1;
-    const uint64_t q_operand = operand(q_at + a * TILE_BYTES, 16), k_operand = operand(kv_at, 16), v_operand = operand(kv_at, TILE_BYTES / 2);
+    const uint64_t k_operand = operand(kv_at, 16), v_operand = operand(kv_at, TILE_BYTES / 2);
     const uint32_t s_at = tmem + a * TILE, o_at = tmem + 2 * TILE + a * 128;
     const uint32_t s_full = smem_u32(&sh.s_full[a]), p_first = smem_u32(&sh.p_first[a]), p_rest = smem_u32(&sh.p_rest[a]), o_empty = smem_u32(&sh.o_empty[a]);
+    uint64_t q_operand = 0;
     int stage = 0;
     unsigned kv_phase = 0, q_phase = 0, p_phase = 0, o_phase = 1, turn = a ^ 1;
     bool ok = true;
@@ -395,14 +452,70 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1) prompt_kernel(const __grid_
     auto advance = [&] {
       if (++stage == KV_STAGES) stage = 0, kv_phase ^= 1;
     };
+    auto release = [&](int at, bool mine) {   // a stage, when the products issued so far have read it
+      if (!elect_one()) return;
+      if (mine) mma_commit(smem_u32(&sh.kv_empty[at]));
+      else bar_arrive(smem_u32(&sh.kv_empty[at]));
+    };
+    // O += P V, 16 keys at a time, the first three quarters as soon as they are there
+    auto values = [&](int v_stage, bool add) {
+      auto product = [&](int c) {
+        mma_tensor(o_at, s_at + c * 8, v_operand + (v_stage * TILE_BYTES >> 4) + c * (2048 >> 4), kind_o, add || c > 0);
+      };
+      if (!add) {   // (the output of the item before has been read)
+        if (!wait(o_empty, o_phase)) return;
+        o_phase ^= 1;
+      }
+      if (!wait(p_first, p_phase)) return;
+      fence_after();
+      if (elect_one()) {
+#pragma unroll
+        for (int c = 0; c < 6; ++c) product(c);
+      }
+      if (!wait(p_rest, p_phase)) return;
+      p_phase ^= 1;
+      fence_after();
+      if (elect_one()) {
+#pragma unroll
+        for (int c = 6; c < 8; ++c) product(c);
+      }
+    };
 #pragma unroll 1
     for (int round = 0; ok && next_item(A, walk, round, w); ++round) {
-      const int lo = uniform(w.lo), hi = uniform(w.hi), end = uniform(a ? w.hi1 : w.hi0), both = uniform(min(w.hi0, w.hi1));
+      const int lo = uniform(w.lo), hi = uniform(w.hi), end = uniform(w.end(a)), both = uniform(min(w.hi0, w.hi1));
       if (hi <= lo) continue;
-      if (!wait(smem_u32(&sh.q_full), q_phase) || !wait(smem_u32(&sh.kv_full[stage]), kv_phase)) break;
+      if (!wait(smem_u32(&sh.q_full), q_phase)) break;
       q_phase ^= 1;
+      if (w.paired) {
+        // tile by tile, and those of the other half of the CTA are let go.  (No turns: copies take longer than products here.)
+        q_operand = operand(q_at, 16);
+        const int first = lo + a;
+        if (first >= end) commit(sh.q_empty);
+#pragma unroll 1
+        for (int i = lo; i < hi; ++i) {
+          const bool mine = (i - first) % 2 == 0;
+          if (!wait(smem_u32(&sh.kv_full[stage]), kv_phase)) break;
+          if (mine) {
+            scores();
+            if (i + 2 >= end) commit(sh.q_empty);
+          }
+          release(stage, mine);
+          advance();
+          if (!wait(smem_u32(&sh.kv_full[stage]), kv_phase)) break;
+          if (mine) {
+            values(stage, i > first);
+            if (!ok) break;
+            if (i + 2 >= end) commit(sh.o_full[a]);
+          }
+          release(stage, mine);
+          advance();
+        }
+        continue;
+      }
+      q_operand = operand(q_at + a * TILE_BYTES, 16);
+      if (!wait(smem_u32(&sh.kv_full[stage]), kv_phase)) break;
       if (lo < end) scores();
-      commit(sh.kv_empty[stage]);
+      release(stage, lo < end);
       if (lo + 1 >= end) commit(sh.q_empty);
       advance();
 #pragma unroll 1
@@ -412,40 +525,21 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1) prompt_kernel(const __grid_
         advance();
         if (i + 1 < hi && !wait(smem_u32(&sh.kv_full[stage]), kv_phase)) break;
         if (i < end) {
-          // O += P V, 16 keys at a time, the first three quarters as soon as they are there
-          auto product = [&](int c) {
-            mma_tensor(o_at, s_at + c * 8, v_operand + (v_stage * TILE_BYTES >> 4) + c * (2048 >> 4), kind_o, c > 0 || i > lo);
-          };
-          if (i == lo) {   // (the output of the item before has been read)
-            if (!wait(o_empty, o_phase)) break;
-            o_phase ^= 1;
-          }
           // The row tiles take turns.  Left alone they fall into step, and the tensor cores wait for both softmaxes, which share
           // the special function units: 4280 cycles a tile instead of 3300 (8 k tokens, all seen: 1132 us, 832).
           if (i < both) {
             if (!wait(smem_u32(&sh.turn[a]), turn)) break;
             turn ^= 1;
           }
-          if (!wait(p_first, p_phase)) break;
-          fence_after();
-          if (elect_one()) {
-#pragma unroll
-            for (int c = 0; c < 6; ++c) product(c);
-          }
-          if (!wait(p_rest, p_phase)) break;
-          p_phase ^= 1;
-          fence_after();
-          if (elect_one()) {
-#pragma unroll
-            for (int c = 6; c < 8; ++c) product(c);
-          }
+          values(v_stage, i > lo);
+          if (!ok) break;
           if (i + 1 < end) scores();
           else commit(sh.o_full[a]);
           if (i < both && elect_one()) bar_arrive(smem_u32(&sh.turn[a ^ 1]));
         }
-        commit(sh.kv_empty[v_stage]);
+        release(v_stage, i < end);
         if (i + 1 < hi) {
-          commit(sh.kv_empty[stage]);
+          release(stage, i < end);
           if (i + 2 == end) commit(sh.q_empty);
           advance();
         }
@@ -467,8 +561,8 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1) prompt_kernel(const __grid_
       if (lane == 0) {
         if ((ok = bar_wait(smem_u32(&sh.q_empty), q_phase, stop))) {
           q_phase ^= 1;
-          bar_expect(smem_u32(&sh.q_full), 2 * TILE_BYTES);
-          for (int a = 0; a < 2; ++a)
+          bar_expect(smem_u32(&sh.q_full), w.paired ? TILE_BYTES : 2 * TILE_BYTES);
+          for (int a = 0; a < (w.paired ? 1 : 2); ++a)
             for (int c = 0; c < 2; ++c)
               copy_box(q_at + a * TILE_BYTES + c * (TILE_BYTES / 2), &M.q, 64 * c, w.head0, w.at.q0 + w.i0 + a * half, smem_u32(&sh.q_full));
         }
@@ -566,25 +660,29 @@ __global__ void __launch_bounds__(256) prompt_join_kernel(const PromptArgs A) {
   const int lane = threadIdx.x & 31;
   if (row >= rows) return;
   const int token = static_cast<int>(row / A.nh_q), head = static_cast<int>(row % A.nh_q);
-  int splits = 0;   // of the token's sequence; rows in no sequence have none
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  int parts = 0;   // of the token's rows; rows in no sequence have none
   for (int s = lane; s < A.n_seqs; s += 32) {
     const int q0 = start_of(A.q_starts, s, A.total_q), q1 = start_of(A.q_starts, s + 1, A.total_q);
     if (token >= q0 && token < q1)
-      splits = shares_of(A, q1 - q0, max(start_of(A.k_starts, s + 1, A.total_k) - start_of(A.k_starts, s, A.total_k), 0));
+      parts = shares_of(A, q1 - q0, max(start_of(A.k_starts, s + 1, A.total_k) - start_of(A.k_starts, s, A.total_k), 0));
   }
-  splits = __reduce_max_sync(0xffffffffu, splits);
-  if (splits < 2) return;   // (written as a whole)
+  parts = __reduce_max_sync(0xffffffffu, parts);
+  if (parts < 2) return;   // (in no sequence, or written as a whole)
+  const float2* const ml = A.part_ml + row;
+  const float* const po = A.part_o + row * 128 + 4 * lane;
   float m = -INFINITY, l = 0.f;
-  for (int s = 0; s < splits; ++s) m = fmaxf(m, A.part_ml[s * rows + row].x);
+  for (int s = lane; s < parts; s += 32) m = fmaxf(m, ml[s * rows].x);
+#pragma unroll
+  for (int k = 1; k < 32; k <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, k));
   const float ref = m == -INFINITY ? 0.f : m;
   float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int s = 0; s < splits; ++s) {
-    const float2 part = A.part_ml[s * rows + row];
-    if (part.y == 0.f) continue;   // it had no keys that this row sees
+#pragma unroll 4
+  for (int s = 0; s < parts; ++s) {
+    const float2 part = ml[s * rows];
+    const float4 v = *reinterpret_cast<const float4*>(po + s * rows * 128);
     const float f = exp2_approx(part.x - ref);
-    const float4 v = *reinterpret_cast<const float4*>(A.part_o + (s * rows + row) * 128 + 4 * lane);
-    l += f * part.y;
-    o.x += f * v.x, o.y += f * v.y, o.z += f * v.z, o.w += f * v.w;
+    if (part.y != 0.f) l += f * part.y, o.x += f * v.x, o.y += f * v.y, o.z += f * v.z, o.w += f * v.w;   // (else it has no output)
   }
   const float inv = l == 0.f ? 0.f : 1.f / l;
   *reinterpret_cast<uint2*>(static_cast<T*>(A.out) + row * 128 + 4 * lane) =
@@ -614,7 +712,7 @@ struct ImportanceShape {
 };
 __host__ __device__ constexpr int imp_stage_bytes(const ImportanceShape& g) { return (g.keys + g.columns) * 256; }
 static size_t imp_smem(const ImportanceShape& g) {   // (a product reads 128 rows of K, the last of them beyond a short tile)
-  return 1024 + g.stages * static_cast<size_t>(imp_stage_bytes(g)) + (TILE - g.keys) * 128 + sizeof(ImportanceShared);
+  return g.stages * static_cast<size_t>(imp_stage_bytes(g)) + (TILE - g.keys) * 128 + sizeof(ImportanceShared);
 }
 struct KeyCount {
   int keys;
@@ -625,12 +723,12 @@ struct KeyCount {
 template <bool BF16, int HB>
 __global__ void __launch_bounds__(IMP_THREADS, 1) importance_kernel(const __grid_constant__ PromptArgs A, const __grid_constant__ PromptMaps M,
                                                                     const ImportanceShape G, const float* lse, __half* out) {
-  extern __shared__ unsigned char raw[];
-  unsigned char* const tiles = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  extern __shared__ __align__(1024) unsigned char tiles[];
   const int stage_bytes = imp_stage_bytes(G), k_half = G.keys * 128;
   ImportanceShared& sh = *reinterpret_cast<ImportanceShared*>(tiles + G.stages * stage_bytes + (TILE - G.keys) * 128);
   const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
   const int per_kv = A.nh_q / A.nh_kv / HB, items = A.nh_kv * per_kv;   // products per tile
+  asm volatile("griddepcontrol.launch_dependents;");   // (as in the attention kernel)
   volatile int* const stop = &sh.stop;
   if (warp == 8) tmem_alloc(smem_u32(&sh.tmem), IMP_SLOTS * IMP_COLUMNS);
   if (threadIdx.x == 0) {
@@ -646,13 +744,15 @@ __global__ void __launch_bounds__(IMP_THREADS, 1) importance_kernel(const __grid
     }
     bar_init_fence();
   }
-  Walk<KeyCount> walk(A, KeyCount{G.keys});
-  Place w;
-  auto next = [&](int tile) { return tile < G.tiles && walk.find(tile, w); };   // (never more than the starts allow when in order)
+  if (warp == 9 && lane < 2) prefetch_map(lane ? &M.q : &M.k);
   fence_before();
   __syncthreads();
   fence_after();
   const uint32_t tmem = uniform(sh.tmem);
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  Walk<KeyCount> walk(A, KeyCount{G.keys});
+  Place w;
+  auto next = [&](int tile) { return tile < G.tiles && walk.find(tile, w); };   // (never more than the starts allow when in order)
   int slot = 0;
   unsigned slot_phase = 0;
   auto next_slot = [&] {
@@ -811,10 +911,11 @@ __global__ void __launch_bounds__(IMP_THREADS, 1) importance_kernel(const __grid
 // host side
 // ------------------------------------------------------------------------------------------------
 // Query heads that share a row tile: those of one kv head, as many of them as a power of two takes (at most 32: four tokens).
-static int head_group(int nh_q, int nh_kv) {
-  int g = 1;
-  while (g < 32 && nh_q / nh_kv % (2 * g) == 0) g *= 2;
-  return g;
+static void set_groups(PromptArgs& A) {
+  A.group = 1, A.block_shift = 8;
+  while (A.group < 32 && A.nh_q / A.nh_kv % (2 * A.group) == 0) A.group *= 2, --A.block_shift;
+  A.groups = A.nh_q / A.group;
+  A.groups_per_kv = A.groups / A.nh_kv;
 }
 
 static int prompt_args(const hqkv_prompt_t* p, bool values, PromptArgs& A) {
@@ -856,31 +957,57 @@ static int prompt_args(const hqkv_prompt_t* p, bool values, PromptArgs& A) {
   A.nh_q = p->nh_q, A.nh_kv = p->nh_kv;
   A.causal = p->causal != 0;
   A.bf16 = p->dtype == HQKV_BF16;
-  A.group = head_group(p->nh_q, p->nh_kv);
+  set_groups(A);
   A.scale_log2 = p->scale * 1.4426950408889634f;
   return HQKV_OK;
 }
 
 // Blocks of queries that all sequences together have at most (their lengths are on the device).
 static int64_t most_blocks(const PromptArgs& A) {
-  const int64_t tokens = 2 * TILE / A.group, n = max(1, min(A.n_seqs, A.total_q));
-  return (A.total_q + n * (tokens - 1)) / tokens;
+  const int64_t tokens = int64_t{1} << A.block_shift, n = max(1, min(A.n_seqs, A.total_q));
+  return (A.total_q + n * (tokens - 1)) >> A.block_shift;
 }
 
 // Tiles of keys per share, and the shares that a block has at most.  Where the blocks do not fill the GPU, their keys are shared out:
-// for one sequence so that there is an item for every CTA, for several - of unknown lengths - into shares of which a CTA gets about three.
+// for one sequence so that it takes the least time in all - a microsecond a tile, and every share's parts are written and read - with at most
+// an item for every CTA; for several, of unknown lengths, into shares of which a CTA gets about three.
 static int prompt_shares(PromptArgs& A) {
-  const int64_t blocks = most_blocks(A) * (A.nh_q / A.group), n = max(1, A.n_seqs);
+  const int64_t blocks = most_blocks(A) * A.groups, n = max(1, A.n_seqs);
   const int64_t most = ceil_div(A.prefix_len, TILE) + ceil_div(A.total_k, TILE);
   int64_t per = max(int64_t{1}, most);
   if (blocks < PROMPT_CTAS && most > 1) {
     const int64_t average = ceil_div(A.prefix_len, TILE) + ceil_div(A.total_k, TILE * n);
-    if (n == 1) per = ceil_div(most, PROMPT_CTAS / blocks);
+    if (n == 1) {
+      const double part = 1.6e-4 * A.total_q * A.nh_q;   // us: 1 KB a row, at HBM's rate
+      double best = 0.;
+      for (int64_t shares = 1; shares <= min(most, PROMPT_CTAS / blocks); ++shares) {
+        const double us = static_cast<double>(ceil_div(most, shares)) + (shares > 1 ? part * shares : 0.);
+        if (shares == 1 || us < best) best = us, per = ceil_div(most, shares);
+      }
+    }
     else per = max(int64_t{4}, ceil_div(blocks * average, 3 * PROMPT_CTAS));
     per = max(per, ceil_div(most, max(int64_t{1}, 8 * PROMPT_CTAS / blocks)));   // (the parts take memory)
   }
   A.per_share = static_cast<int>(per);
-  return static_cast<int>(max(int64_t{1}, ceil_div(most, per)));
+  A.shares = static_cast<int>(max(int64_t{1}, ceil_div(most, per)));
+  return A.shares;
+}
+
+// Launched so that it may take its place while the kernel before it ends (see the waits in the kernels).
+template <typename... Params, typename... Args>
+static int launch_behind(void (*kernel)(Params...), int64_t grid, int block, size_t smem, cudaStream_t st, const Args&... args) {
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(grid));
+  cfg.blockDim = dim3(block);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  HQKV_CUDA(cudaLaunchKernelEx(&cfg, kernel, args...));
+  return HQKV_OK;
 }
 
 static int tensor_map(CUtensorMap* map, const void* base, bool bf16, int64_t tokens, int heads, int64_t token_stride, int64_t head_stride,
@@ -923,12 +1050,10 @@ static int launch_prompt(PromptArgs& A, int shares, cudaStream_t st) {
     HQKV_CUDA(cudaFuncSetAttribute(prompt_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(PROMPT_SMEM)));
     if (dev >= 0 && dev < 64) opted_in[dev] = true;
   }
-  const int64_t items = most_blocks(A) * (A.nh_q / A.group) * shares;
+  const int64_t items = most_blocks(A) * A.groups * shares;
   HQKV_REQUIRE(items < (1ll << 30), "prompt: too many rows");
   A.items = static_cast<int>(items);
-  (A.bf16 ? prompt_kernel<true> : prompt_kernel<false>)<<<static_cast<unsigned>(min(items, int64_t{PROMPT_CTAS})), PROMPT_THREADS, PROMPT_SMEM, st>>>(A, M);
-  HQKV_LAUNCH_CHECK("prompt");
-  return HQKV_OK;
+  return launch_behind(A.bf16 ? prompt_kernel<true> : prompt_kernel<false>, min(items, int64_t{PROMPT_CTAS}), PROMPT_THREADS, PROMPT_SMEM, st, A, M);
 }
 
 template <bool BF16, int HB>
@@ -940,9 +1065,7 @@ static int launch_importance(const PromptArgs& A, const PromptMaps& M, const Imp
     HQKV_CUDA(cudaFuncSetAttribute(importance_kernel<BF16, HB>, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024));
     if (dev >= 0 && dev < 64) opted_in[dev] = true;
   }
-  importance_kernel<BF16, HB><<<min(G.tiles, PROMPT_CTAS), IMP_THREADS, imp_smem(G), st>>>(A, M, G, lse, out);
-  HQKV_LAUNCH_CHECK("importance");
-  return HQKV_OK;
+  return launch_behind(importance_kernel<BF16, HB>, min(G.tiles, PROMPT_CTAS), IMP_THREADS, imp_smem(G), st, A, M, G, lse, out);
 }
 
 static int launch_importance(const PromptArgs& A, const float* lse, int rows, __half* out, cudaStream_t st) {
@@ -971,10 +1094,11 @@ static int launch_importance(const PromptArgs& A, const float* lse, int rows, __
   }
 }
 
-int prefix_shares(const hqkv_prompt_t* p) {
+int prefix_parts(const hqkv_prompt_t* p) {
   PromptArgs A;
   A.total_q = static_cast<int>(p->total_q), A.total_k = 0, A.n_seqs = 0, A.prefix_len = static_cast<int>(p->prefix_len);
-  A.nh_q = p->nh_q, A.nh_kv = p->nh_kv, A.group = head_group(p->nh_q, p->nh_kv);
+  A.nh_q = p->nh_q, A.nh_kv = p->nh_kv;
+  set_groups(A);
   return prompt_shares(A);
 }
 
@@ -1021,10 +1145,7 @@ extern "C" int hqkv_prompt_attention(const hqkv_prompt_t* prompt_host, void* out
   A.part_o = static_cast<float*>(workspace);
   A.part_ml = reinterpret_cast<float2*>(static_cast<unsigned char*>(workspace) + ml);
   if (int rc = launch_prompt(A, shares, st)) return rc;
-  const unsigned grid = static_cast<unsigned>(ceil_div(static_cast<int64_t>(A.total_q) * A.nh_q, 8));
-  (A.bf16 ? prompt_join_kernel<true> : prompt_join_kernel<false>)<<<grid, 256, 0, st>>>(A);
-  HQKV_LAUNCH_CHECK("prompt_join");
-  return HQKV_OK;
+  return launch_behind(A.bf16 ? prompt_join_kernel<true> : prompt_join_kernel<false>, ceil_div(static_cast<int64_t>(A.total_q) * A.nh_q, 8), 256, 0, st, A);
 }
 
 extern "C" int hqkv_prompt_waits_expired(int reset, unsigned* count_host) {

@@ -14,9 +14,10 @@ struct PromptArgs {
   int64_t q_token, q_head, k_token, k_head, v_token, v_head, pk_token, pk_head, pv_token, pv_head;
   const int *q_starts, *k_starts;                   // [n_seqs + 1]
   int n_seqs, total_q, total_k, prefix_len, nh_q, nh_kv;
-  int group;                                        // query heads of a kv head that share a row tile
+  int group, groups, groups_per_kv;                 // query heads of a kv head that share a row tile; such groups
+  int block_shift;                                  // log2 of the tokens of a block (two row tiles)
   int items;                                        // most blocks x head groups x shares
-  int per_share;                                    // tiles of keys per share of a block's
+  int per_share, shares;                            // tiles of keys per share of a block's; most shares
   bool causal, bf16, partial;                       // partial: part_o and part_ml are the result
   float scale_log2;                                 // scale * log2(e)
   void* out;                                        // [total_q][nh_q][128]
@@ -29,8 +30,8 @@ struct PromptMaps {   // the tensors as (channel, head, token), for copies by ti
   CUtensorMap q, k, v, pk, pv;
 };
 
-// Attention of p's queries (a token each, no sequences) to its prefix alone: `shares` parts per row, to be joined.
-int prefix_shares(const hqkv_prompt_t* p);
+// Attention of p's queries (a token each, no sequences) to its prefix alone, in parts to be joined; how many.
+int prefix_parts(const hqkv_prompt_t* p);
 int prefix_partial(const hqkv_prompt_t* p, float* part_o, float2* part_ml, cudaStream_t st);
 
 }  // namespace hqkv

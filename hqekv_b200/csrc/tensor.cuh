@@ -60,6 +60,7 @@ __device__ __forceinline__ void copy_box(uint32_t dst, const CUtensorMap* map, i
       "l"(map), "r"(channel), "r"(head), "r"(token), "r"(bar)
       : "memory");
 }
+__device__ __forceinline__ void prefetch_map(const CUtensorMap* map) { asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory"); }
 __device__ __forceinline__ void fence_generic_to_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
 // ---- tcgen05
