@@ -28,28 +28,54 @@ __device__ __forceinline__ int start_of(const int* starts, int s, int total) { r
 // ------------------------------------------------------------------------------------------------
 // A CTA takes blocks of 256 rows of queries - two tiles of 128 rows, a row being a (token, head of the group) - and walks the tiles of 128
 // keys that any of them sees: first the prefix, then the sequence's own.  One pass, with the running maximum and sum of the softmax.
-//   warps 0-3, 4-7   softmax and output of the first and second row tile, a row per thread
+//   warps 0-3, 4-7   softmax of the first and second row tile, a row per thread
 //   warps 8, 11      issue the matrix products of the first and second row tile
-//   warp 9           requests the tiles of Q, K and V (one thread)
+//   warp 9           looks up the items and requests their tiles of Q, K and V (one thread)
 //   warp 10          looks after V tiles that not every row sees (below)
+//   warps 12-15      write the output of an item, while the softmax of the next one has begun
 // Tensor memory: S of both row tiles (128 columns each, overwritten by P in the type of V) and O of both.
-// There is one CTA per SM.  It takes an item - a block of queries, a head group and a share of the keys - after the other, and every
-// warp goes through the same items by itself: the first S of an item is there when the output of the one before is written.
+// An item is a block of queries, a head group and a share of the keys.  The grid has a CTA per item, but one CTA per SM does the work: when
+// warp 9 begins an item it asks for one that has not been launched yet, looks it up while the others are at work and leaves it in shared
+// memory for them.  (Items in a fixed order per CTA: with four prompts of 4 k, some CTAs had 11 % more than their share.)
 constexpr int TILE = 128;                                // keys per tile, rows per row tile
 constexpr int TILE_BYTES = TILE * 128 * 2;               // 64 channels of all its tokens, then the other 64
 constexpr int KV_STAGES = 5;
-constexpr int PROMPT_THREADS = 384;
+constexpr int PROMPT_THREADS = 512;
 constexpr int PROMPT_CTAS = 148;                         // one per SM
 constexpr unsigned TMEM_COLUMNS = 512;
 constexpr float RESCALE_AT = 8.f;                        // powers of two that P may exceed 1 by
 constexpr int BY_POLYNOMIAL = 0;                         // of 16 pairs of exponentials
 
+struct Place {   // a block of a sequence, and where the sequence's queries and keys are
+  int q0, lq, k0, lk, block, rest;   // rest: head group and share
+};
+// an item of the attention kernel
+struct Item {
+  Place at;
+  bool over;                               // there are no more
+  int head0, kv, share, i0;                // i0: the block's first query in its sequence
+  bool part, paired;                       // the result is a part of the rows'; one row tile of queries, on which both halves of the CTA work
+  int before, seen_first, seen_last;       // tiles of the prefix; own keys that the block's first and last query see
+  int lo, hi, hi0, hi1;                    // tiles of keys: [lo, hi), of which the row tiles see those below hi0 and hi1
+  // The tiles that row tile a works on: all that it sees, or of a paired item every other one.
+  __device__ __forceinline__ int first(int a) const { return lo + (paired ? a : 0); }
+  __device__ __forceinline__ int end(int a) const { return a && !paired ? hi1 : hi0; }
+  __device__ __forceinline__ int step() const { return paired ? 2 : 1; }
+  // Own V tiles that hold keys which some rows of the block do not see.  0 x NaN is NaN in a matrix product, so what lies behind
+  // the last key that any row sees is set to 0; an infinity or NaN that only some rows see is set to 0 as well, and those rows
+  // add it at the end.
+  __device__ __forceinline__ bool partly_seen(int tile) const { return tile >= before && (tile - before + 1) * TILE > seen_first; }
+};
+constexpr int ITEMS = 4;   // looked up at a time
+
 struct PromptShared {
-  unsigned long long q_full, q_empty, kv_full[KV_STAGES], kv_empty[KV_STAGES], v_raw[KV_STAGES];
-  unsigned long long s_full[2], p_first[2], p_rest[2], o_full[2], o_empty[2], turn[2], drained[2], pair_full[4], pair_done[4];
+  unsigned long long item_full[ITEMS], item_empty[ITEMS], next_full, q_full, q_empty, kv_full[KV_STAGES], kv_empty[KV_STAGES], v_raw[KV_STAGES];
+  unsigned long long s_full[2], p_first[2], p_rest[2], o_full[2], o_empty[2], turn[2], drained[2], ml_full, ml_empty;
   uint32_t tmem;
-  float2 pair_ml[2][TILE];   // (maximum, sum) of the rows of a paired item's halves
-  int stop, odd[4];   // odd: the last item (by its number, of those with the same two low bits) in which warp 10 found infinities or NaN
+  alignas(16) uint4 next;   // answer to the request for an item
+  Item items[ITEMS];
+  float2 ml[2][TILE];       // (maximum, sum) of the rows
+  int stop, odd[ITEMS];     // odd: the last item (by its number) with this place in which warp 10 found infinities or NaN
 };
 constexpr size_t PROMPT_SMEM = (2 + KV_STAGES) * static_cast<size_t>(TILE_BYTES) + sizeof(PromptShared);
 static_assert(PROMPT_SMEM <= 227 * 1024, "one CTA per SM");
@@ -66,10 +92,7 @@ __device__ __forceinline__ int shares_of(const PromptArgs& A, int lq, int lk) {
   return A.shares == 1 ? 1 : max(1, (tiles_of(A.prefix_len) + tiles_of(keys_seen(A, lq - 1, lq, lk)) + A.per_share - 1) / A.per_share);
 }
 
-// Walks the sequences in order, 32 at a time (a lane each), to the one that holds an item; items are asked for in rising order.
-struct Place {   // a block of a sequence, and where the sequence's queries and keys are
-  int q0, lq, k0, lk, block, rest;   // rest: head group and share
-};
+// Walks the sequences in order, 32 at a time (a lane each), to the one that holds an item.  Items are asked for in rising order, mostly.
 template <typename Count>
 struct Walk {
   const PromptArgs& A;
@@ -95,11 +118,15 @@ struct Walk {
   // The last block of a sequence, which sees the most keys, comes first.  False: there are not as many items.
   __device__ __forceinline__ bool find(int item, Place& p) {
     unsigned past;
+    if (item < before) {
+      at = 0, before = 0;
+      look();
+    }
     while (!(past = __ballot_sync(0xffffffffu, item < before + sum))) {
       before += __shfl_sync(0xffffffffu, sum, 31);
       at += 32;
       if (at >= A.n_seqs) {
-        sum = 0;   // (whoever asks again gets the same answer)
+        sum = 0;   // (all that follow get the same answer)
         return false;
       }
       look();
@@ -141,39 +168,22 @@ __device__ __forceinline__ void exp2_polynomial(uint64_t x2, float& a, float& b)
   b = __int_as_float(__float_as_int(b) + (__float_as_int(m) << 23));
 }
 
-// an item of the attention kernel
-struct Item {
-  Place at;
-  int head0, kv, share, shares, i0;        // i0: the block's first query in its sequence
-  bool part, paired;                       // the result is a part of the rows'; one row tile of queries, on which both halves of the CTA work
-  int before, seen_first, seen_last;       // tiles of the prefix; own keys that the block's first and last query see
-  int lo, hi, hi0, hi1;                    // tiles of keys: [lo, hi), of which the row tiles see those below hi0 and hi1
-  // The tiles that row tile a works on: all that it sees, or of a paired item every other one.
-  __device__ __forceinline__ int first(int a) const { return lo + (paired ? a : 0); }
-  __device__ __forceinline__ int end(int a) const { return a && !paired ? hi1 : hi0; }
-  __device__ __forceinline__ int step() const { return paired ? 2 : 1; }
-  // Own V tiles that hold keys which some rows of the block do not see.  0 x NaN is NaN in a matrix product, so what lies behind
-  // the last key that any row sees is set to 0; an infinity or NaN that only some rows see is set to 0 as well, and those rows
-  // add it at the end.
-  __device__ __forceinline__ bool partly_seen(int tile) const { return tile >= before && (tile - before + 1) * TILE > seen_first; }
-};
 struct ItemCount {
   const PromptArgs& A;
   __device__ __forceinline__ int blocks(int lq, int) const { return (lq + (1 << A.block_shift) - 1) >> A.block_shift; }
   __device__ __forceinline__ int each(int lq, int lk) const { return A.groups * shares_of(A, lq, lk); }
 };
-__device__ __forceinline__ bool next_item(const PromptArgs& A, Walk<ItemCount>& walk, int round, Item& w) {
-  // (every other round backwards: the first items of a causal prompt are the longest)
-  const int item = round * static_cast<int>(gridDim.x) + (round & 1 ? static_cast<int>(gridDim.x - 1 - blockIdx.x) : static_cast<int>(blockIdx.x));
-  if (item >= A.items || !walk.find(item, w.at)) return false;   // (more than there can be: the starts are not in order)
+// false: there are fewer items
+__device__ __forceinline__ bool look_up(const PromptArgs& A, Walk<ItemCount>& walk, int item, Item& w) {
+  w.over = false;
+  if (!walk.find(item, w.at)) return false;
   const int lq = w.at.lq, lk = w.at.lk, half = 1 << (A.block_shift - 1);
-  w.shares = shares_of(A, lq, lk);
   w.share = A.shares == 1 ? 0 : w.at.rest / A.groups;
   const int group = w.at.rest - w.share * A.groups;
   w.head0 = group * A.group;
   w.kv = group / A.groups_per_kv;
   w.i0 = w.at.block << A.block_shift;
-  w.part = A.partial || w.shares > 1;
+  w.part = A.partial || shares_of(A, lq, lk) > 1;
   w.paired = w.i0 + half >= lq;
   w.before = tiles_of(A.prefix_len);
   w.seen_first = keys_seen(A, w.i0, lq, lk);
@@ -216,10 +226,13 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1) prompt_kernel(const __grid_
       bar_init(smem_u32(&sh.turn[a]), 1);
       bar_init(smem_u32(&sh.drained[a]), 1);
     }
-    for (int i = 0; i < 4; ++i) {
-      bar_init(smem_u32(&sh.pair_full[i]), 2);
-      bar_init(smem_u32(&sh.pair_done[i]), 2);
+    for (int i = 0; i < ITEMS; ++i) {
+      bar_init(smem_u32(&sh.item_full[i]), 1);
+      bar_init(smem_u32(&sh.item_empty[i]), PROMPT_THREADS / 32 - 1);
     }
+    bar_init(smem_u32(&sh.next_full), 1);
+    bar_init(smem_u32(&sh.ml_full), 8);
+    bar_init(smem_u32(&sh.ml_empty), 4);
     bar_init_fence();
   }
   if (warp == 9 && lane < 5) prefetch_map(lane == 0 ? &M.q : lane == 1 ? &M.k : lane == 2 ? &M.v : lane == 3 ? &M.pk : &M.pv);
@@ -229,11 +242,20 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1) prompt_kernel(const __grid_
   const uint32_t tmem = uniform(sh.tmem);
   // (nothing before this reads or writes what an earlier kernel may still be working on)
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  Walk<ItemCount> walk(A, ItemCount{A});
-  Item w;
+  // item number `round`, for the warps that work on it; null: there are no more, or a wait has run out
+  auto item = [&](int round) -> const Item* {
+    const int at = round % ITEMS;
+    if (!__all_sync(0xffffffffu, bar_wait(smem_u32(&sh.item_full[at]), round / ITEMS & 1, stop))) return nullptr;
+    return sh.items[at].over ? nullptr : &sh.items[at];
+  };
+  auto done = [&](int round) {
+    __syncwarp();
+    if (lane == 0) bar_arrive(smem_u32(&sh.item_empty[round % ITEMS]));
+  };
 
-  // 384 threads are launched with 168 registers each: 2 x 128 x 208 + 128 x 88 = 384 x 168
-  if (warp < 8) more_registers<208>();
+  // 512 threads are launched with 128 registers each: 2 x 128 x 184 + 128 x 56 + 128 x 88 = 512 x 128
+  if (warp < 8) more_registers<184>();
+  else if (warp < 12) fewer_registers<56>();
   else fewer_registers<88>();
   if (warp < 8) {
     // ---- softmax
@@ -241,13 +263,15 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1) prompt_kernel(const __grid_
     const uint32_t lanes = tmem + (static_cast<uint32_t>(warp & 3) << 21);   // (32 lanes a warp, in bits 16 and up)
     const uint32_t s_at = lanes + a * TILE, o_at = lanes + 2 * TILE + a * 128;
     const float scale = A.scale_log2;
-    unsigned s_phase = 0, o_phase = 0, pair_phase = 0;
+    unsigned s_phase = 0, ml_phase = 1;
     bool ok = true;
 #pragma unroll 1
-    for (int round = 0; ok && next_item(A, walk, round, w); ++round) {
-      const int i = w.i0 + token + (w.paired ? 0 : a * half), head = w.head0 + row % A.group, first = w.first(a), end = w.end(a), step = w.step();
-      const bool live = i < w.at.lq;
-      const int seen = live ? keys_seen(A, i, w.at.lq, w.at.lk) : w.at.lk;
+    for (int round = 0; ok; ++round) {
+      const Item* const item_at = item(round);
+      if (!item_at) break;
+      const Item& w = *item_at;
+      const int i = w.i0 + token + (w.paired ? 0 : a * half), first = w.first(a), end = w.end(a), step = w.step(), before = w.before;
+      const int seen = i < w.at.lq ? keys_seen(A, i, w.at.lq, w.at.lk) : w.at.lk;
       float ref = -INFINITY, sum = 0.f;
 #pragma unroll 1
       for (int tile = first; tile < end; tile += step) {
@@ -258,7 +282,7 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1) prompt_kernel(const __grid_
 #pragma unroll
         for (int c = 0; c < TILE; c += 32) tmem_load32(s_at + c, s + c);
         wait_loads(s);
-        const int limit = tile < w.before ? A.prefix_len - tile * TILE : seen - (tile - w.before) * TILE;
+        const int limit = tile < before ? A.prefix_len - tile * TILE : seen - (tile - before) * TILE;
         if (__any_sync(0xffffffffu, limit < TILE)) {
 #pragma unroll
           for (int c = 0; c < TILE; ++c)
@@ -328,100 +352,105 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1) prompt_kernel(const __grid_
         sum += x + y;
       }
       if (!ok) break;
-      // ---- output
-      const bool any = end > first;
-      if (any) {
-        if (!(ok = __all_sync(0xffffffffu, bar_wait(smem_u32(&sh.o_full[a]), o_phase, stop)))) break;
-        o_phase ^= 1;
-        fence_after();
+      if (!(ok = __all_sync(0xffffffffu, bar_wait(smem_u32(&sh.ml_empty), ml_phase, stop)))) break;
+      ml_phase ^= 1;
+      sh.ml[a][row] = make_float2(ref, sum);
+      __syncwarp();
+      if (lane == 0) bar_arrive(smem_u32(&sh.ml_full));
+      done(round);
+    }
+  } else if (warp >= 12) {
+    // ---- output: a row of each row tile per thread, or of a paired item the one row that both halves have worked on
+    const int row = threadIdx.x & 127, token = row / A.group;
+    const uint32_t o_at = tmem + (static_cast<uint32_t>(warp & 3) << 21) + 2 * TILE;
+    const int64_t rows = static_cast<int64_t>(A.total_q) * A.nh_q;
+    unsigned ml_phase = 0, o_phase[2] = {0, 0};
+    bool ok = true;
+#pragma unroll 1
+    for (int round = 0; ok; ++round) {
+      const Item* const item_at = item(round);
+      if (!item_at) break;
+      const Item& w = *item_at;
+      if (!(ok = __all_sync(0xffffffffu, bar_wait(smem_u32(&sh.ml_full), ml_phase, stop)))) break;
+      ml_phase ^= 1;
+      float2 ml[2] = {sh.ml[0][row], sh.ml[1][row]};
+      __syncwarp();
+      if (lane == 0) bar_arrive(smem_u32(&sh.ml_empty));
+      float f[2] = {1.f, 1.f};
+      if (w.paired) {
+        const float top = fmaxf(ml[0].x, ml[1].x), base = top == -INFINITY ? 0.f : top;
+        f[0] = exp2_approx(ml[0].x - base), f[1] = exp2_approx(ml[1].x - base);
+        ml[0] = make_float2(top, f[0] * ml[0].y + f[1] * ml[1].y);
       }
-      const int64_t at = static_cast<int64_t>(w.at.q0 + i) * A.nh_q + head, rows = static_cast<int64_t>(A.total_q) * A.nh_q;
-      bool odd = *const_cast<volatile int*>(&sh.odd[round & 3]) == round;
-      // 32 channels of the row, not yet normalised, from `o`
-      auto store = [&](uint32_t (&o)[32], int c, float by) {
-        if (!live) return;
-        if (odd) {
-          const int to = min(seen, (w.hi - w.before) * TILE);
-          for (int j = max(w.seen_first, (w.lo - w.before) * TILE); j < to; ++j) {
-            const T* v = static_cast<const T*>(A.v) + (w.at.k0 + j) * A.v_token + w.kv * A.v_head + c;
 #pragma unroll
-            for (int k = 0; k < 32; ++k) {
-              const float x = to_float(v[k]);
-              if (!isfinite(x)) o[k] = __float_as_uint(__uint_as_float(o[k]) + x);
-            }
-          }
+      for (int a = 0; a < 2; ++a) {
+        const bool any = w.end(a) > w.first(a);
+        if (any) {
+          if (!(ok = __all_sync(0xffffffffu, bar_wait(smem_u32(&sh.o_full[a]), o_phase[a], stop)))) break;
+          o_phase[a] ^= 1;
+          fence_after();
         }
-        if (w.part) {
-          uint4* to = reinterpret_cast<uint4*>(A.part_o + (w.share * rows + at) * 128 + c);
-#pragma unroll
-          for (int k = 0; k < 8; ++k) to[k] = make_uint4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]);
-        } else {
-          uint32_t h[16];
-#pragma unroll
-          for (int k = 0; k < 16; ++k) h[k] = narrow2<BF16>(__uint_as_float(o[2 * k]) * by, __uint_as_float(o[2 * k + 1]) * by);
-          uint4* to = reinterpret_cast<uint4*>(static_cast<T*>(A.out) + at * 128 + c);
-#pragma unroll
-          for (int k = 0; k < 4; ++k) to[k] = make_uint4(h[4 * k], h[4 * k + 1], h[4 * k + 2], h[4 * k + 3]);
-        }
-      };
-      auto statistics = [&](float ref, float sum) {
-        if (!live) return;
-        if (w.part) A.part_ml[w.share * rows + at] = make_float2(ref, sum);
-        else A.lse[static_cast<int64_t>(head) * A.total_q + w.at.q0 + i] = sum == 0.f ? -INFINITY : (ref + log2f(sum)) * 0.6931471805599453f;
-      };
-      if (!w.paired) {
-        statistics(ref, sum);
-        if (!any && w.part) continue;   // (nobody reads a part whose sum is 0)
-        const float by = sum == 0.f ? 0.f : 1.f / sum;
+        if (w.paired && a == 0) continue;   // (its output comes with the other half's)
+        const int half_a = w.paired ? 0 : a, i = w.i0 + token + half_a * half, head = w.head0 + row % A.group;
+        const bool live = i < w.at.lq, first = w.paired ? w.end(0) > w.first(0) : any, second = w.paired && any;
+        const float ref = ml[half_a].x, sum = ml[half_a].y;
+        const int64_t at = static_cast<int64_t>(w.at.q0 + i) * A.nh_q + head;
+        if (live && w.part) A.part_ml[w.share * rows + at] = make_float2(ref, sum);
+        else if (live) A.lse[static_cast<int64_t>(head) * A.total_q + w.at.q0 + i] = sum == 0.f ? -INFINITY : (ref + log2f(sum)) * 0.6931471805599453f;
+        if (w.part && !first && !second) continue;   // (nobody reads a part whose sum is 0)
+        const float by = w.part ? 1.f : sum == 0.f ? 0.f : 1.f / sum, f0 = f[0] * by, f1 = f[1] * by;
+        const bool odd = *const_cast<volatile int*>(&sh.odd[round % ITEMS]) == round;
 #pragma unroll 1
         for (int c = 0; c < 128; c += 32) {
           uint32_t o[32] = {};
-          if (any) {
-            tmem_load32(o_at + c, o);
+          if (first) {
+            tmem_load32(o_at + half_a * 128 + c, o);
             wait_loads(o);
-            if (c == 96) {
-              fence_before();
-              __syncwarp();
-              if (lane == 0) bar_arrive(smem_u32(&sh.o_empty[a]));
+#pragma unroll
+            for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * f0);
+          }
+          if (second) {
+            uint32_t x[32];
+            tmem_load32(o_at + 128 + c, x);
+            wait_loads(x);
+#pragma unroll
+            for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(fmaf(__uint_as_float(x[k]), f1, __uint_as_float(o[k])));
+          }
+          if (c == 96) {   // the last of it has been read
+            fence_before();
+            __syncwarp();
+            if (lane == 0 && first) bar_arrive(smem_u32(&sh.o_empty[half_a]));
+            if (lane == 0 && second) bar_arrive(smem_u32(&sh.o_empty[1]));
+          }
+          if (!live) continue;
+          if (odd) {
+            const int to = min(keys_seen(A, i, w.at.lq, w.at.lk), (w.hi - w.before) * TILE);
+            for (int j = max(w.seen_first, (w.lo - w.before) * TILE); j < to; ++j) {
+              const T* v = static_cast<const T*>(A.v) + (w.at.k0 + j) * A.v_token + w.kv * A.v_head + c;
+#pragma unroll
+              for (int k = 0; k < 32; ++k) {
+                const float x = to_float(v[k]);
+                if (!isfinite(x)) o[k] = __float_as_uint(__uint_as_float(o[k]) + x);
+              }
             }
           }
-          store(o, c, by);
-        }
-      } else {
-        // The halves of the CTA have every other tile of the same rows: a warp of each (which can read the same part of tensor memory)
-        // joins 64 channels of both.
-        const bool others = w.end(a ^ 1) > w.first(a ^ 1);
-        sh.pair_ml[a][row] = make_float2(ref, sum);
-        fence_before();
-        __syncwarp();
-        if (lane == 0) bar_arrive(smem_u32(&sh.pair_full[warp & 3]));
-        if (!(ok = __all_sync(0xffffffffu, bar_wait(smem_u32(&sh.pair_full[warp & 3]), pair_phase, stop)))) break;
-        fence_after();
-        odd = *const_cast<volatile int*>(&sh.odd[round & 3]) == round;   // (found in the other half's tiles, maybe)
-        const float2 other = sh.pair_ml[a ^ 1][row];
-        const float top = fmaxf(ref, other.x), base = top == -INFINITY ? 0.f : top;
-        // (a half without tiles has nothing in tensor memory)
-        const float f = any ? exp2_approx(ref - base) : 0.f, g = others ? exp2_approx(other.x - base) : 0.f, all = f * sum + g * other.y;
-        if (a == 0) statistics(top, all);
-        const float by = all == 0.f ? 0.f : 1.f / all;
-#pragma unroll 1
-        for (int c = 64 * a; c < 64 * a + 64; c += 32) {
-          uint32_t o[32] = {}, x[32] = {};
-          if (any) tmem_load32(o_at + c, o);
-          if (others) tmem_load32(lanes + 2 * TILE + (a ^ 1) * 128 + c, x);
-          wait_loads(o);
-          wait_loads(x);
+          if (w.part) {
+            uint4* to = reinterpret_cast<uint4*>(A.part_o + (w.share * rows + at) * 128 + c);
 #pragma unroll
-          for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(f * __uint_as_float(o[k]) + g * __uint_as_float(x[k]));
-          store(o, c, by);
+            for (int k = 0; k < 8; ++k) to[k] = make_uint4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]);
+          } else {
+            uint4* to = reinterpret_cast<uint4*>(static_cast<T*>(A.out) + at * 128 + c);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              uint32_t h[4];
+#pragma unroll
+              for (int m = 0; m < 4; ++m) h[m] = narrow2<BF16>(__uint_as_float(o[8 * k + 2 * m]), __uint_as_float(o[8 * k + 2 * m + 1]));
+              to[k] = make_uint4(h[0], h[1], h[2], h[3]);
+            }
+          }
         }
-        fence_before();
-        __syncwarp();
-        if (lane == 0) bar_arrive(smem_u32(&sh.pair_done[warp & 3]));
-        if (!(ok = __all_sync(0xffffffffu, bar_wait(smem_u32(&sh.pair_done[warp & 3]), pair_phase, stop)))) break;
-        pair_phase ^= 1;
-        if (any && lane == 0) bar_arrive(smem_u32(&sh.o_empty[a]));
       }
+      done(round);
     }
   } else if (warp == 8 || warp == 11) {
     // ---- matrix products of a row tile.  One warp for both was busy all the time with waiting (some 150 cycles for a barrier that is
@@ -481,12 +510,17 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1) prompt_kernel(const __grid_
       }
     };
 #pragma unroll 1
-    for (int round = 0; ok && next_item(A, walk, round, w); ++round) {
+    for (int round = 0; ok; ++round) {
+      const Item* const item_at = item(round);
+      if (!item_at) break;
+      const Item& w = *item_at;
       const int lo = uniform(w.lo), hi = uniform(w.hi), end = uniform(w.end(a)), both = uniform(min(w.hi0, w.hi1));
+      const bool paired = uniform(w.paired);
+      done(round);
       if (hi <= lo) continue;
       if (!wait(smem_u32(&sh.q_full), q_phase)) break;
       q_phase ^= 1;
-      if (w.paired) {
+      if (paired) {
         // tile by tile, and those of the other half of the CTA are let go.  (No turns: copies take longer than products here.)
         q_operand = operand(q_at, 16);
         const int first = lo + a;
@@ -551,14 +585,30 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1) prompt_kernel(const __grid_
       }
     }
   } else if (warp == 9) {
-    // ---- copies: of every item Q, then K and V of one tile after the other
-    int stage = 0;
+    // ---- items, and their copies: Q, then K and V of one tile after the other
+    Walk<ItemCount> walk(A, ItemCount{A});
+    Item w;
+    int stage = 0, round = 0, asked = 0;
     unsigned kv_phase = 1, q_phase = 1, to_raw = 0, raw_parity = 0, full_parity = 0, used = 0;   // a bit per stage: of the last copy into it
     bool ok = true;
-#pragma unroll 1
-    for (int round = 0; next_item(A, walk, round, w); ++round) {
-      if (w.hi <= w.lo) continue;
+    auto publish = [&] {
+      const int at = round % ITEMS;
+      if (!(ok = __all_sync(0xffffffffu, bar_wait(smem_u32(&sh.item_empty[at]), (round / ITEMS & 1) ^ 1, stop)))) return;
       if (lane == 0) {
+        sh.items[at] = w;
+        bar_arrive(smem_u32(&sh.item_full[at]));
+      }
+      ++round;
+    };
+#pragma unroll 1
+    for (int next = blockIdx.x; next >= 0;) {
+      if (lane == 0) {
+        bar_expect(smem_u32(&sh.next_full), 16);
+        request_cta(smem_u32(&sh.next), smem_u32(&sh.next_full));
+      }
+      if (look_up(A, walk, next, w)) publish();
+      else w.lo = w.hi = 0;
+      if (ok && w.hi > w.lo && lane == 0) {
         if ((ok = bar_wait(smem_u32(&sh.q_empty), q_phase, stop))) {
           q_phase ^= 1;
           bar_expect(smem_u32(&sh.q_full), w.paired ? TILE_BYTES : 2 * TILE_BYTES);
@@ -586,8 +636,21 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1) prompt_kernel(const __grid_
           }
         }
       }
-      if (__any_sync(0xffffffffu, !ok)) break;
+      ok = __all_sync(0xffffffffu, ok);
+      // (an answer that does not come is waited for even where something else has gone wrong: it lands in this CTA's memory)
+      if (!__all_sync(0xffffffffu, bar_wait(smem_u32(&sh.next_full), asked & 1, stop)) || !ok) {
+        for (int k = 0; k < WAIT_TRIES && !bar_try(smem_u32(&sh.next_full), asked & 1); ++k) {
+        }
+        ok = false;
+        break;
+      }
+      ++asked;
+      next = requested_cta(smem_u32(&sh.next));
+      fence_generic_to_async();   // (read before the next answer is written)
+      __syncwarp();
     }
+    w.over = true;
+    if (ok) publish();
     if (lane == 0 && !ok) {   // copies in flight land before the CTA ends
       auto landed = [&](const unsigned long long& bar, unsigned parity) {
         for (int k = 0; k < WAIT_TRIES && !bar_try(smem_u32(&bar), parity); ++k) {
@@ -605,7 +668,10 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1) prompt_kernel(const __grid_
     unsigned parity = 0, fills = 0;   // a bit per stage; copies into stages before this item's
     bool ok = true;
 #pragma unroll 1
-    for (int round = 0; ok && next_item(A, walk, round, w); ++round) {
+    for (int round = 0; ok; ++round) {
+      const Item* const item_at = item(round);
+      if (!item_at) break;
+      const Item& w = *item_at;
 #pragma unroll 1
       for (int i = max(w.lo, w.before + w.seen_first / TILE); i < w.hi; ++i) {
         const int stage = (fills + 2 * (i - w.lo) + 1) % KV_STAGES, first = (i - w.before) * TILE;
@@ -635,13 +701,14 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1) prompt_kernel(const __grid_
             *at = x;
           }
         }
-        if (odd) *const_cast<volatile int*>(&sh.odd[round & 3]) = round;
+        if (odd) *const_cast<volatile int*>(&sh.odd[round % ITEMS]) = round;
         fence_generic_to_async();
         __syncwarp();
         if (lane == 0) bar_arrive(smem_u32(&sh.kv_full[stage]));
       }
       fills += 2 * max(w.hi - w.lo, 0);
       fills %= KV_STAGES;
+      done(round);
     }
   }
   __syncwarp();
@@ -1052,8 +1119,7 @@ static int launch_prompt(PromptArgs& A, int shares, cudaStream_t st) {
   }
   const int64_t items = most_blocks(A) * A.groups * shares;
   HQKV_REQUIRE(items < (1ll << 30), "prompt: too many rows");
-  A.items = static_cast<int>(items);
-  return launch_behind(A.bf16 ? prompt_kernel<true> : prompt_kernel<false>, min(items, int64_t{PROMPT_CTAS}), PROMPT_THREADS, PROMPT_SMEM, st, A, M);
+  return launch_behind(A.bf16 ? prompt_kernel<true> : prompt_kernel<false>, items, PROMPT_THREADS, PROMPT_SMEM, st, A, M);
 }
 
 template <bool BF16, int HB>

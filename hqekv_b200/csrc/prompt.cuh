@@ -16,7 +16,6 @@ struct PromptArgs {
   int n_seqs, total_q, total_k, prefix_len, nh_q, nh_kv;
   int group, groups, groups_per_kv;                 // query heads of a kv head that share a row tile; such groups
   int block_shift;                                  // log2 of the tokens of a block (two row tiles)
-  int items;                                        // most blocks x head groups x shares
   int per_share, shares;                            // tiles of keys per share of a block's; most shares
   bool causal, bf16, partial;                       // partial: part_o and part_ml are the result
   float scale_log2;                                 // scale * log2(e)

@@ -63,6 +63,22 @@ __device__ __forceinline__ void copy_box(uint32_t dst, const CUtensorMap* map, i
 __device__ __forceinline__ void prefetch_map(const CUtensorMap* map) { asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory"); }
 __device__ __forceinline__ void fence_generic_to_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
+// ---- work of CTAs that have not been launched yet: a request for the next one, and its index out of the answer (-1: there is none)
+__device__ __forceinline__ void request_cta(uint32_t answer, uint32_t bar) {
+  asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(answer), "r"(bar) : "memory");
+}
+__device__ __forceinline__ int requested_cta(uint32_t answer) {
+  int x;
+  asm volatile(
+      "{\n.reg .pred p;\n.reg .b128 a;\n.reg .b32 y, z;\nld.shared.b128 a, [%1];\n"
+      "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, a;\nmov.b32 %0, -1;\n"
+      "@p clusterlaunchcontrol.query_cancel.get_first_ctaid.v4.b32.b128 {%0, y, z, _}, a;\n}"
+      : "=r"(x)
+      : "r"(answer)
+      : "memory");
+  return x;
+}
+
 // ---- tcgen05
 __device__ __forceinline__ void tmem_alloc(uint32_t slot, unsigned columns) {
   asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(slot), "r"(columns) : "memory");
