@@ -61,9 +61,8 @@ struct Item {
   __device__ __forceinline__ int first(int a) const { return lo + (paired ? a : 0); }
   __device__ __forceinline__ int end(int a) const { return a && !paired ? hi1 : hi0; }
   __device__ __forceinline__ int step() const { return paired ? 2 : 1; }
-  // Own V tiles that hold keys which some rows of the block do not see.  0 x NaN is NaN in a matrix product, so what lies behind
-  // the last key that any row sees is set to 0; an infinity or NaN that only some rows see is set to 0 as well, and those rows
-  // add it at the end.
+  // Own V tiles that hold keys which some rows of the block do not see.  0 x NaN is NaN in a matrix product, so infinities and NaN
+  // of such keys are set to 0, and the rows that do see them add them at the end.
   __device__ __forceinline__ bool partly_seen(int tile) const { return tile >= before && (tile - before + 1) * TILE > seen_first; }
 };
 constexpr int ITEMS = 4;   // looked up at a time
@@ -147,6 +146,14 @@ __device__ __forceinline__ bool odd_pair(uint32_t v) {   // an infinity or NaN i
   return (v & e) == e || (v >> 16 & e) == e;
 }
 
+template <bool BF16>
+__device__ __forceinline__ uint32_t add_zeros(uint32_t sum, uint32_t v) {   // sum + v * 0, both halves
+  uint32_t r;
+  if constexpr (BF16) asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(v), "r"(0u), "r"(sum));
+  else asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(v), "r"(0u), "r"(sum));
+  return r;
+}
+
 // 2^x of two numbers without the special function unit, which would otherwise take as long as the matrix products: x = n + f with
 // |f| <= 1/2, a polynomial of degree 5 in f with the least largest relative error (7.5e-8; coefficients by Remez's exchange), n added
 // to the exponent.  x is at most 8 here; below -126 the result is 2^-126.
@@ -194,6 +201,25 @@ __device__ __forceinline__ bool look_up(const PromptArgs& A, Walk<ItemCount>& wa
   w.hi = min(w.lo + A.per_share, max(n0, n1));
   w.hi0 = min(w.hi, n0), w.hi1 = min(w.hi, n1);
   return true;
+}
+
+// Adds the infinities and NaN of keys that only some rows of the block see to query i's output.
+template <bool BF16>
+__device__ __noinline__ void add_odd_values(const PromptArgs& A, const Item& w, int i, float* part_to, std::conditional_t<BF16, __nv_bfloat16, __half>* to) {
+  using T = std::conditional_t<BF16, __nv_bfloat16, __half>;
+  const int from = max(w.seen_first, (w.lo - w.before) * TILE), last = min(keys_seen(A, i, w.at.lq, w.at.lk), (w.hi - w.before) * TILE);
+#pragma unroll 1
+  for (int c = 0; c < 128; ++c) {
+    float sum = 0.f;
+#pragma unroll 1
+    for (int j = from; j < last; ++j) {
+      const float x = to_float(static_cast<const T*>(A.v)[(w.at.k0 + j) * A.v_token + w.kv * A.v_head + c]);
+      if (!isfinite(x)) sum += x;
+    }
+    if (sum == 0.f) continue;
+    if (w.part) part_to[c] += sum;
+    else to[c] = static_cast<T>(to_float(to[c]) + sum);
+  }
 }
 
 template <bool BF16>
@@ -259,7 +285,7 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1) prompt_kernel(const __grid_
   else fewer_registers<88>();
   if (warp < 8) {
     // ---- softmax
-    const int a = warp >> 2, row = threadIdx.x & 127, token = row / A.group;
+    const int a = warp >> 2, row = threadIdx.x & 127, token = row >> (8 - A.block_shift);
     const uint32_t lanes = tmem + (static_cast<uint32_t>(warp & 3) << 21);   // (32 lanes a warp, in bits 16 and up)
     const uint32_t s_at = lanes + a * TILE, o_at = lanes + 2 * TILE + a * 128;
     const float scale = A.scale_log2;
@@ -361,7 +387,7 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1) prompt_kernel(const __grid_
     }
   } else if (warp >= 12) {
     // ---- output: a row of each row tile per thread, or of a paired item the one row that both halves have worked on
-    const int row = threadIdx.x & 127, token = row / A.group;
+    const int row = threadIdx.x & 127, token = row >> (8 - A.block_shift);
     const uint32_t o_at = tmem + (static_cast<uint32_t>(warp & 3) << 21) + 2 * TILE;
     const int64_t rows = static_cast<int64_t>(A.total_q) * A.nh_q;
     unsigned ml_phase = 0, o_phase[2] = {0, 0};
@@ -391,7 +417,7 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1) prompt_kernel(const __grid_
           fence_after();
         }
         if (w.paired && a == 0) continue;   // (its output comes with the other half's)
-        const int half_a = w.paired ? 0 : a, i = w.i0 + token + half_a * half, head = w.head0 + row % A.group;
+        const int half_a = w.paired ? 0 : a, i = w.i0 + token + half_a * half, head = w.head0 + (row & (A.group - 1));
         const bool live = i < w.at.lq, first = w.paired ? w.end(0) > w.first(0) : any, second = w.paired && any;
         const float ref = ml[half_a].x, sum = ml[half_a].y;
         const int64_t at = static_cast<int64_t>(w.at.q0 + i) * A.nh_q + head;
@@ -399,56 +425,35 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1) prompt_kernel(const __grid_
         else if (live) A.lse[static_cast<int64_t>(head) * A.total_q + w.at.q0 + i] = sum == 0.f ? -INFINITY : (ref + log2f(sum)) * 0.6931471805599453f;
         if (w.part && !first && !second) continue;   // (nobody reads a part whose sum is 0)
         const float by = w.part ? 1.f : sum == 0.f ? 0.f : 1.f / sum, f0 = f[0] * by, f1 = f[1] * by;
-        const bool odd = *const_cast<volatile int*>(&sh.odd[round % ITEMS]) == round;
+        float* const part_to = A.part_o + (w.share * rows + at) * 128;
+        T* const to = static_cast<T*>(A.out) + at * 128;
+        const bool part = w.part;
+        // (Few instructions, gone through eight times: written out at length this took twice as long, most of it to fetch them.)
 #pragma unroll 1
-        for (int c = 0; c < 128; c += 32) {
-          uint32_t o[32] = {};
-          if (first) {
-            tmem_load32(o_at + half_a * 128 + c, o);
-            wait_loads(o);
+        for (int c = 0; c < 128; c += 16) {
+          uint32_t o[16] = {}, x[16] = {};
+          if (first) tmem_load16(o_at + half_a * 128 + c, o);
+          if (second) tmem_load16(o_at + 128 + c, x);
+          wait_loads(o);
+          wait_loads(x);
 #pragma unroll
-            for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * f0);
-          }
-          if (second) {
-            uint32_t x[32];
-            tmem_load32(o_at + 128 + c, x);
-            wait_loads(x);
-#pragma unroll
-            for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(fmaf(__uint_as_float(x[k]), f1, __uint_as_float(o[k])));
-          }
-          if (c == 96) {   // the last of it has been read
-            fence_before();
-            __syncwarp();
-            if (lane == 0 && first) bar_arrive(smem_u32(&sh.o_empty[half_a]));
-            if (lane == 0 && second) bar_arrive(smem_u32(&sh.o_empty[1]));
-          }
+          for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(fmaf(__uint_as_float(x[k]), f1, __uint_as_float(o[k]) * f0));
           if (!live) continue;
-          if (odd) {
-            const int to = min(keys_seen(A, i, w.at.lq, w.at.lk), (w.hi - w.before) * TILE);
-            for (int j = max(w.seen_first, (w.lo - w.before) * TILE); j < to; ++j) {
-              const T* v = static_cast<const T*>(A.v) + (w.at.k0 + j) * A.v_token + w.kv * A.v_head + c;
-#pragma unroll
-              for (int k = 0; k < 32; ++k) {
-                const float x = to_float(v[k]);
-                if (!isfinite(x)) o[k] = __float_as_uint(__uint_as_float(o[k]) + x);
-              }
-            }
-          }
-          if (w.part) {
-            uint4* to = reinterpret_cast<uint4*>(A.part_o + (w.share * rows + at) * 128 + c);
-#pragma unroll
-            for (int k = 0; k < 8; ++k) to[k] = make_uint4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]);
+          if (part) {
+            store_sector(part_to + c, o);
+            store_sector(part_to + c + 8, o + 8);
           } else {
-            uint4* to = reinterpret_cast<uint4*>(static_cast<T*>(A.out) + at * 128 + c);
+            uint32_t h[8];
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              uint32_t h[4];
-#pragma unroll
-              for (int m = 0; m < 4; ++m) h[m] = narrow2<BF16>(__uint_as_float(o[8 * k + 2 * m]), __uint_as_float(o[8 * k + 2 * m + 1]));
-              to[k] = make_uint4(h[0], h[1], h[2], h[3]);
-            }
+            for (int m = 0; m < 8; ++m) h[m] = narrow2<BF16>(__uint_as_float(o[2 * m]), __uint_as_float(o[2 * m + 1]));
+            store_sector(to + c, h);
           }
         }
+        fence_before();   // O has been read
+        __syncwarp();
+        if (lane == 0 && first) bar_arrive(smem_u32(&sh.o_empty[half_a]));
+        if (lane == 0 && second) bar_arrive(smem_u32(&sh.o_empty[1]));
+        if (live && *const_cast<volatile int*>(&sh.odd[round % ITEMS]) == round) add_odd_values<BF16>(A, w, i, part_to, to);
       }
       done(round);
     }
@@ -678,30 +683,30 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1) prompt_kernel(const __grid_
         if (!w.partly_seen(i)) continue;
         if (!(ok = __all_sync(0xffffffffu, bar_wait(smem_u32(&sh.v_raw[stage]), parity >> stage & 1, stop)))) break;
         parity ^= 1u << stage;
-        unsigned char* const v = tiles + (2 + stage) * TILE_BYTES;
-        bool odd = false;
-        // (which of a row's pieces of 16 bytes comes where does not matter here)
-        for (int k = lane; k < TILE_BYTES / 16; k += 32) {
-          const int j = first + (k >> 3 & (TILE - 1));
-          if (j < w.seen_first) continue;
-          uint4* const at = reinterpret_cast<uint4*>(v + k * 16);
-          if (j >= w.seen_last) {
-            *at = make_uint4(0u, 0u, 0u, 0u);
-            continue;
+        // x * 0 added up is 0 as long as x is finite.  (Looked at one by one, the values of a tile took 7000 cycles.)
+        uint4* const v = reinterpret_cast<uint4*>(tiles + (2 + stage) * TILE_BYTES);   // (which piece of a row comes where does not matter)
+        const int from = max(w.seen_first - first, 0) * 8 + lane;                       // eight pieces of 16 bytes per row of 64 channels
+        uint32_t zero = 0;
+#pragma unroll 1
+        for (int half_at = 0; half_at < TILE_BYTES / 16; half_at += TILE_BYTES / 32)
+#pragma unroll 8
+          for (int k = from; k < TILE_BYTES / 32; k += 32) {
+            const uint4 x = v[half_at + k];
+            zero = add_zeros<BF16>(zero, x.x), zero = add_zeros<BF16>(zero, x.y), zero = add_zeros<BF16>(zero, x.z), zero = add_zeros<BF16>(zero, x.w);
           }
-          uint4 x = *at;
-          if (odd_pair<BF16>(x.x) || odd_pair<BF16>(x.y) || odd_pair<BF16>(x.z) || odd_pair<BF16>(x.w)) {
-            odd = true;
-            uint32_t* word = &x.x;
-            constexpr uint32_t e = BF16 ? 0x7F80u : 0x7C00u;
-            for (int m = 0; m < 4; ++m) {
-              if ((word[m] & e) == e) word[m] &= 0xFFFF0000u;
-              if ((word[m] >> 16 & e) == e) word[m] &= 0x0000FFFFu;
-            }
-            *at = x;
+        if (__any_sync(0xffffffffu, odd_pair<BF16>(zero))) {
+          constexpr uint32_t e = BF16 ? 0x7F80u : 0x7C00u;
+          uint32_t* const word = reinterpret_cast<uint32_t*>(v);
+          bool odd = false;
+          for (int k = lane; k < TILE_BYTES / 4; k += 32) {
+            const int j = first + (k >> 5 & (TILE - 1));
+            if (j < w.seen_first || !odd_pair<BF16>(word[k])) continue;
+            odd |= j < w.seen_last;
+            if ((word[k] & e) == e) word[k] &= 0xFFFF0000u;
+            if ((word[k] >> 16 & e) == e) word[k] &= 0x0000FFFFu;
           }
+          if (odd) *const_cast<volatile int*>(&sh.odd[round % ITEMS]) = round;
         }
-        if (odd) *const_cast<volatile int*>(&sh.odd[round % ITEMS]) = round;
         fence_generic_to_async();
         __syncwarp();
         if (lane == 0) bar_arrive(smem_u32(&sh.kv_full[stage]));
@@ -1199,7 +1204,7 @@ extern "C" int hqkv_prompt_attention(const hqkv_prompt_t* prompt_host, void* out
   PromptArgs A;
   if (int rc = prompt_args(prompt_host, true, A)) return rc;
   if (A.total_q == 0 || A.n_seqs == 0) return HQKV_OK;
-  HQKV_REQUIRE(out && lse && aligned(out, 16) && aligned(lse, 4), "prompt: the outputs are null or misaligned");
+  HQKV_REQUIRE(out && lse && aligned(out, 32) && aligned(lse, 4), "prompt: the outputs are null or misaligned");
   A.out = out, A.lse = lse;
   const int shares = prompt_shares(A);
   size_t ml;

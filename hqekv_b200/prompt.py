@@ -98,7 +98,7 @@ def prompt_attention(q, k, v, seq_starts, kv_starts=None, *, prefix=None, causal
     (query heads of one kv head are neighbours).  ``kv_starts``: where the keys of each sequence begin, if they are not those of
     the queries; a causal query sees its own keys up to its distance from the end (query i of Lq sees keys j <= i + Lk - Lq), so a
     chunk of a prompt attends to all that is cached before it.  ``prefix`` = (k, v) [P, nh_kv, 128]: tokens that every query of every
-    sequence sees before its own keys.  ``scale``: 1 / sqrt(128) if not given.  ``out``: a contiguous tensor to write to.
+    sequence sees before its own keys.  ``scale``: 1 / sqrt(128) if not given.  ``out``: a contiguous, 32-byte aligned tensor to write to.
 
     ``lse`` is the natural logarithm of each row's softmax denominator.  A query that sees no key has output 0 and lse -inf.
     Rows of queries in no sequence (behind the last start, or before the first) are not written: in ``out`` they stay as they were,
@@ -114,8 +114,8 @@ def prompt_attention(q, k, v, seq_starts, kv_starts=None, *, prefix=None, causal
     q = keep[0]
     if out is None:
         out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    elif out.shape != q.shape or out.dtype != q.dtype or out.device != q.device or not out.is_contiguous() or out.data_ptr() % 16:
-        raise ValueError("out must be a contiguous, 16-byte aligned tensor of q's shape, type and device")
+    elif out.shape != q.shape or out.dtype != q.dtype or out.device != q.device or not out.is_contiguous() or out.data_ptr() % 32:
+        raise ValueError("out must be a contiguous, 32-byte aligned tensor of q's shape, type and device")
     lse = torch.empty(q.shape[1], q.shape[0], dtype=torch.float32, device=q.device)
     with torch.cuda.device(q.device):
         need = lib.hqkv_prompt_workspace_bytes(C.byref(p))

@@ -522,7 +522,7 @@ typedef struct {
 
 /*
  * softmax(scale q K^T) V: what the flash-attention branch of the prefill computes (model/llama_hqe.py:141-166), for sequences of any
- * lengths in one call.  out [total_q, nh_q, D] and lse fp32 [nh_q, total_q] (the log of the softmax's denominator), both dense.
+ * lengths in one call.  out [total_q, nh_q, D] (32-byte aligned) and lse fp32 [nh_q, total_q] (the log of the softmax's denominator), both dense.
  * A query that sees no key has output 0 and lse -inf; rows of queries in no sequence are not written.  Scratch (for calls with few rows, whose
  * keys are shared out) as hqkv_prompt_workspace_bytes says, 256-byte aligned, of any contents; the size depends on sizes alone,
  * not on the starts.

@@ -124,7 +124,7 @@ def test_c_abi_refuses_outputs_and_rows():
     p = good_prompt()
     assert _lib.lib.hqkv_prompt_attention(None, 1 << 20, 1 << 20, None, 0, None) == -1
     assert _lib.lib.hqkv_prompt_attention(C.byref(p), None, 1 << 20, None, 0, None) == -1
-    assert _lib.lib.hqkv_prompt_attention(C.byref(p), 8 + (1 << 20), 1 << 20, None, 0, None) == -1
+    assert _lib.lib.hqkv_prompt_attention(C.byref(p), 16 + (1 << 20), 1 << 20, None, 0, None) == -1
     assert _lib.lib.hqkv_prompt_attention(C.byref(p), 1 << 20, None, None, 0, None) == -1
     for rows in (0, 65):
         assert _lib.lib.hqkv_prompt_importance(C.byref(p), 1 << 20, rows, 1 << 20, None) == -1
