@@ -6,11 +6,15 @@ Restates, with plain torch modules and no dependency on a transformers release, 
 do around the path this package implements:
 
 * prefill: dense causal attention; the probabilities of the last 20 queries seed the importance ring;
-  the cache tuple starts as 39 empty slots + (K, V, length);
+  the cache tuple starts as 39 empty slots + (K, V, length).  ``fused_prompt=True`` takes both from this package's
+  own kernels (``prompt_attention``, ``prompt_importance``) instead of the library's;
 * decode: the new K / V row is appended to the fp16 residual window and ``qkv_matmul_hqe_2`` attends
   over all tiers; the head-summed probability row goes into the ring;
 * whenever 32 or more tokens are unquantised: rank blocks by importance, derive the six tier counts
   from the configured shares (:class:`TierSchedule`), and flush with ``KV_cache_hqe_2``.
+
+A batch may share a prefix (``set_prefix``): every sequence attends to its dense K / V before its own tokens, in the prefill
+and in every decode step, and it is neither copied per sequence nor quantised.  No counterpart in the reference.
 
 Signature and results of ``forward`` are the reference's: ``(attn_output, attn_weights | None,
 past_key_value, auxiliary_parameters)`` where ``auxiliary_parameters = (compress_ratio, K_bit_num,
@@ -21,8 +25,9 @@ from typing import Optional, Tuple
 import torch
 from torch import nn
 
+from ..prompt import prompt_attention, prompt_importance
 from ..quant.hqe_2 import KV_cache_hqe_2
-from ..quant.hqe_matmul import qkv_matmul_hqe_2
+from ..quant.hqe_matmul import qkv_matmul_hqe_2, qkv_matmul_hqe_prefix
 from .public_func import get_block_token_idx, last_attn_weights, make_sum_equal
 
 BLOCK = 32          # tokens per ranking block = K group = V group on this path (model/llama_hqe.py:208,230)
@@ -132,14 +137,16 @@ class HqeAttention(nn.Module):
     """One attention layer with the tiered KV cache.
 
     ``quant_strategy``: 'uniform_group' or 'high_uniform_group_low_normal_group'; ``times_range``: rank V
-    blocks by importance x value range.  ``qk_norm=True`` gives the Qwen3 flavour.  Per-sequence state
+    blocks by importance x value range.  ``qk_norm=True`` gives the Qwen3 flavour.  ``fused_prompt``: the prefill runs this
+    package's kernels (inference only, no attention mask; ``forward`` then has no probabilities of a prefill to return), as
+    it does behind a prefix in any case.  Per-sequence state
     (ring, lengths, shares) lives on the module as in the reference; call :meth:`reset` between sequences
     and :meth:`set_max_length` before the prefill."""
 
     def __init__(self, hidden_size: int, num_heads: int, num_kv_heads: int, head_dim: int = 128,
                  quant_strategy: str = "high_uniform_group_low_normal_group", times_range: bool = True,
                  bit_0: float = 0.25, bit_4: float = 0.25, bit_2: float = 0.25, bit_1: float = 0.25,
-                 qk_norm: bool = False, rms_eps: float = 1e-6, bias: bool = False):
+                 qk_norm: bool = False, rms_eps: float = 1e-6, bias: bool = False, fused_prompt: bool = False):
         super().__init__()
         self.hidden_size, self.num_heads, self.num_kv_heads, self.head_dim = hidden_size, num_heads, num_kv_heads, head_dim
         self.num_key_value_groups = num_heads // num_kv_heads
@@ -153,6 +160,8 @@ class HqeAttention(nn.Module):
         self.k_norm = HeadRMSNorm(head_dim, rms_eps) if qk_norm else None
         self.schedule = TierSchedule(bit_0, bit_4, bit_2, bit_1)
         self.last_weights = last_attn_weights(last_length=SEED_QUERIES)
+        self.fused_prompt = fused_prompt
+        self.prefix = None
 
     # -- per-sequence state ---------------------------------------------------------------------
     def reset(self):
@@ -161,6 +170,16 @@ class HqeAttention(nn.Module):
 
     def set_max_length(self, max_length: int):
         self.last_weights.set_max_length(max_length)
+
+    def set_prefix(self, k: Optional[torch.Tensor] = None, v: Optional[torch.Tensor] = None):
+        """K and V [P, num_kv_heads, head_dim] of tokens that all sequences have before their own, rotated for positions
+        0 ... P - 1 (a sequence's own begin at P); without arguments: none."""
+        if (k is None) != (v is None):
+            raise ValueError("a prefix needs both K and V")
+        for x in (k, v):
+            if x is not None and (x.dim() != 3 or x.shape[0] == 0 or x.shape != k.shape or tuple(x.shape[1:]) != (self.num_kv_heads, self.head_dim)):
+                raise ValueError(f"a prefix must be [P, {self.num_kv_heads}, {self.head_dim}] with at least one token")
+        self.prefix = None if k is None else (k, v)
 
     @property
     def current_length(self):
@@ -202,6 +221,19 @@ class HqeAttention(nn.Module):
         weights = nn.functional.softmax(scores, dim=-1, dtype=torch.float32).to(q.dtype)
         return weights, out
 
+    def _prefill_fused(self, q, k, v, attention_mask):
+        """The same from packed tokens (a batch is stored token by token, so nothing is copied): the output, and the ring rows
+        in the place of the probabilities (of causal attention, as the reference's mask makes it).  The rows of a batch are added
+        up as its probabilities would be."""
+        if attention_mask is not None:
+            raise ValueError("the fused prefill takes no attention mask")
+        B, nh, S, Dh = q.shape
+        q, k, v = (x.transpose(1, 2).reshape(B * S, -1, Dh) for x in (q, k, v))
+        starts = torch.arange(0, B * S + 1, S, dtype=torch.int32, device=q.device)
+        out, lse = prompt_attention(q, k, v, starts, prefix=self.prefix, scale=self.scaling)
+        rows = prompt_importance(q, k, lse, starts, rows=min(S, SEED_QUERIES), scale=self.scaling).view(-1, B, S)
+        return rows[:, 0] if B == 1 else rows.sum(1), out.view(B, S, nh, Dh).transpose(1, 2)
+
     def _flush(self, past_key_value, auxiliary_parameters):
         sch = self.schedule
         compress, total, block_num = sch.lengths()
@@ -233,8 +265,16 @@ class HqeAttention(nn.Module):
             new_k = k if past_key_value[-3] is None else torch.cat((past_key_value[-3], k), dim=2)
             new_v = v if past_key_value[-2] is None else torch.cat((past_key_value[-2], v), dim=2)
             past_key_value = tuple(past_key_value[:-3]) + (new_k, new_v, kv_seq_len)
-            attn_weights, attn_output = qkv_matmul_hqe_2(q, past_key_value, attention_mask, self.head_dim,
-                                                         self.quant_strategy, BLOCK, BLOCK)
+            if self.prefix is not None:
+                attn_weights, attn_output = qkv_matmul_hqe_prefix(q, past_key_value, self.prefix, self.head_dim,
+                                                                  self.quant_strategy, BLOCK, BLOCK)
+            else:
+                attn_weights, attn_output = qkv_matmul_hqe_2(q, past_key_value, attention_mask, self.head_dim,
+                                                             self.quant_strategy, BLOCK, BLOCK)
+        elif self.fused_prompt or self.prefix is not None:
+            rows, attn_output = self._prefill_fused(q, k, v, attention_mask)
+            attn_weights = None
+            past_key_value = (None,) * 39 + (k, v, kv_seq_len)
         else:
             attn_weights, attn_output = self._prefill(q, k, v, attention_mask)
             past_key_value = (None,) * 39 + (k, v, kv_seq_len)
@@ -244,7 +284,10 @@ class HqeAttention(nn.Module):
         # call can write the row itself (qkv_matmul_hqe_2(head_sum_out=...)), one launch less, but measured slower
         # at batch 1: the last CTA to finish a chunk then gathers that chunk's 16 k probabilities alone, while this
         # launch spreads the same gathers over the whole GPU (37.5 against 26.4 us per layer at 32 k context).
-        self.last_weights.update(attn_weights)
+        if attn_weights is None:
+            self.last_weights.seed(rows)
+        else:
+            self.last_weights.update(attn_weights)
         if self.schedule.due():
             past_key_value, auxiliary_parameters = self._flush(past_key_value, auxiliary_parameters)
         else:

@@ -60,6 +60,8 @@ def main(argv=None):
     ap.add_argument("--steps", type=int, default=64)
     ap.add_argument("--warmup", type=int, default=3)
     ap.add_argument("--strategy", default="high_uniform_group_low_normal_group")
+    ap.add_argument("--fused-prompt", action="store_true", help="prefill with this package's prompt kernels")
+    ap.add_argument("--shared-prefix", type=int, default=0, help="tokens that all sequences of the batch share before their own")
     ap.add_argument("--no-graphs", action="store_true", help="issue the dense parts of a decode step eagerly")
     ap.add_argument("--tiers", choices=["model"] + sorted(TIER_MIXES), default="model",
                     help="model: the shares the reference's model files derive (64 fp16 tokens, 4/2/1-bit, eviction); "
@@ -73,7 +75,7 @@ def main(argv=None):
     dev = torch.device("cuda", torch.cuda.current_device())
     base = MODELS[args.model]
     cfg = DecoderConfig(**{**base.__dict__, "quant_strategy": args.strategy,
-                           "num_layers": args.layers or base.num_layers})
+                           "num_layers": args.layers or base.num_layers, "fused_prompt": args.fused_prompt})
     torch.set_default_dtype(torch.float16)
     try:
         with torch.device(dev):
@@ -87,6 +89,8 @@ def main(argv=None):
     total_steps = args.warmup + args.steps
     model.start_sequence(args.ctx + total_steps + 1)
     with torch.no_grad():
+        if args.shared_prefix:
+            model.share_prefix(torch.randn(1, args.shared_prefix, cfg.hidden_size, generator=gen, device=dev, dtype=torch.float16))
         torch.cuda.synchronize()
         t0 = time.perf_counter()
         sched = model.layers[0].self_attn.schedule
@@ -135,7 +139,7 @@ def main(argv=None):
         "flush_steps": int(sum(timed_flush)), "steps": len(timed), "warmup": args.warmup,
         "prefill_s": round(prefill_s, 3),
         "config": {"model": args.model, "layers": cfg.num_layers, "batch": args.batch, "context": args.ctx,
-                   "strategy": args.strategy, "tiers": args.tiers,
+                   "strategy": args.strategy, "tiers": args.tiers, "fused_prompt": args.fused_prompt, "shared_prefix": args.shared_prefix,
                    "dense_parts": "eager" if args.no_graphs else "cuda graphs", "shares_evict_4_2_1": [cfg.bit_0, cfg.bit_4, cfg.bit_2, cfg.bit_1]},
         "cached_tokens": cached_tokens, "positions": pos,
         "cache_bytes": cache_nbytes(caches), "fp16_cache_bytes": fp16_bytes,

@@ -13,6 +13,7 @@ from typing import List, Optional
 import torch
 from torch import nn
 
+from ..prompt import prompt_attention
 from .attention_hqe import HeadRMSNorm, HqeAttention, rotary_tables
 
 
@@ -34,6 +35,7 @@ class DecoderConfig:
     bit_4: float = 0.25
     bit_2: float = 0.25
     bit_1: float = 0.25
+    fused_prompt: bool = False     # prefill with this package's prompt kernels
 
 
 LLAMA31_8B = DecoderConfig()
@@ -55,7 +57,8 @@ class HqeDecoderLayer(nn.Module):
     def __init__(self, cfg: DecoderConfig):
         super().__init__()
         self.self_attn = HqeAttention(cfg.hidden_size, cfg.num_heads, cfg.num_kv_heads, cfg.head_dim, cfg.quant_strategy,
-                                      cfg.times_range, cfg.bit_0, cfg.bit_4, cfg.bit_2, cfg.bit_1, cfg.qk_norm, cfg.rms_eps)
+                                      cfg.times_range, cfg.bit_0, cfg.bit_4, cfg.bit_2, cfg.bit_1, cfg.qk_norm, cfg.rms_eps,
+                                      fused_prompt=cfg.fused_prompt)
         self.mlp = SwiGLU(cfg.hidden_size, cfg.intermediate_size)
         self.input_layernorm = HeadRMSNorm(cfg.hidden_size, cfg.rms_eps)
         self.post_attention_layernorm = HeadRMSNorm(cfg.hidden_size, cfg.rms_eps)
@@ -70,7 +73,8 @@ class HqeDecoderLayer(nn.Module):
 
 class HqeDecoder(nn.Module):
     """Stack of decoder layers with per-layer tiered caches.  ``forward(inputs, caches, position)`` takes token
-    ids [B, S] (``vocab_size > 0``) or hidden states [B, S, hidden]; returns (logits or hidden states, caches)."""
+    ids [B, S] (``vocab_size > 0``) or hidden states [B, S, hidden]; returns (logits or hidden states, caches).  ``position``
+    counts a sequence's own tokens, from 0 behind a shared prefix, too."""
 
     def __init__(self, cfg: DecoderConfig):
         super().__init__()
@@ -79,6 +83,32 @@ class HqeDecoder(nn.Module):
         self.layers = nn.ModuleList(HqeDecoderLayer(cfg) for _ in range(cfg.num_layers))
         self.norm = HeadRMSNorm(cfg.hidden_size, cfg.rms_eps)
         self.lm_head = nn.Linear(cfg.hidden_size, cfg.vocab_size, bias=False) if cfg.vocab_size else None
+        self.prefix_length = 0
+
+    @torch.no_grad()
+    def share_prefix(self, inputs: Optional[torch.Tensor] = None):
+        """Run ``inputs`` ([1, P] token ids or [1, P, hidden]) through the layers once and let every sequence of the batches that
+        follow attend to it before its own tokens; without arguments: no prefix any more.  Its K / V stay dense, one copy for
+        all sequences.  Sequences started before are not affected by what they have cached, so start new ones."""
+        for layer in self.layers:
+            layer.self_attn.set_prefix()
+        self.prefix_length = 0
+        if inputs is None:
+            return
+        x = self.embed_tokens(inputs) if self.embed_tokens is not None else inputs
+        if x.shape[0] != 1 or x.shape[1] == 0:
+            raise ValueError("a shared prefix is one sequence of at least one token")
+        P = x.shape[1]
+        rope = rotary_tables(torch.arange(P, device=x.device).unsqueeze(0), self.cfg.head_dim, self.cfg.rope_theta, x.dtype)
+        starts = torch.tensor([0, P], dtype=torch.int32, device=x.device)
+        for layer in self.layers:
+            a = layer.self_attn
+            q, k, v = (t[0].transpose(0, 1) for t in a._project(layer.input_layernorm(x), rope))
+            out, _ = prompt_attention(q, k, v, starts, scale=a.scaling)
+            x = x + a.o_proj(out.view(1, P, -1))
+            x = x + layer.mlp(layer.post_attention_layernorm(x))
+            a.set_prefix(k.contiguous(), v.contiguous())
+        self.prefix_length = P
 
     def start_sequence(self, max_length: int):
         """Forget the previous sequence and size the importance rings (model/llama_hqe.py:557, 691-695)."""
@@ -92,6 +122,7 @@ class HqeDecoder(nn.Module):
         layer derives from its configured shares (the reference's layers accept them the same way)."""
         x = self.embed_tokens(inputs) if self.embed_tokens is not None else inputs
         B, S, _ = x.shape
+        position += self.prefix_length
         pos = torch.arange(position, position + S, device=x.device).unsqueeze(0).expand(B, S)
         rope = rotary_tables(pos, self.cfg.head_dim, self.cfg.rope_theta, x.dtype)
         caches = [None] * len(self.layers) if caches is None else list(caches)
@@ -230,7 +261,7 @@ class GraphedDecodeStep:
     def __call__(self, inputs: torch.Tensor, caches: List[tuple], position: int,
                  auxiliary_parameters: Optional[tuple] = None):
         (self.ids if self.ids is not None else self.x).copy_(inputs)
-        self.pos.fill_(position)
+        self.pos.fill_(position + self.model.prefix_length)
         caches = list(caches)
         aux = auxiliary_parameters
         self.graphs[0].replay()

@@ -133,6 +133,24 @@ class last_attn_weights:
         self.kv_seq_len = L
         self.next_line = (self.next_line + 1) % self.last_length
 
+    def seed(self, rows: torch.Tensor):
+        """What ``update`` does with the probabilities of a prompt, from their sums over the heads: ``rows`` float16
+        [n, L], the n last queries' (``prompt_importance``)."""
+        n, L = rows.shape
+        cap = self.max_length if self.weights is None else self.weights.shape[1]
+        if L > cap or n > self.last_length:
+            raise ValueError(f"rows holds {n} queries and {L} positions but the ring is sized for {self.last_length} and {cap} "
+                             "(call set_max_length with the longest sequence before the first update)")
+        if rows.dtype != torch.float16:
+            raise ValueError("rows must be float16")
+        require_cuda(rows)
+        if self.weights is None:
+            self.weights = torch.zeros(self.last_length, self.max_length, dtype=torch.float16, device=rows.device)
+        first = self.next_line if n == 1 else 0   # (as update: one query is a decode step)
+        self.weights[first:first + n, :L] = rows
+        self.kv_seq_len = L
+        self.next_line = (self.next_line + n) % self.last_length
+
     def update(self, attn_weights: torch.Tensor):
         cap = self.max_length if self.weights is None else self.weights.shape[1]
         if attn_weights.shape[-1] > cap:
