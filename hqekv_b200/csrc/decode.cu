@@ -2458,18 +2458,26 @@ struct JoinParams {
   __half *out, *weights;
   int nk_ctas, r4, L, rows, parts;
 };
-constexpr int JOIN_THREADS = 128, JOIN_TOKENS = 2048, JOIN_PARTS = 148;   // tokens whose weights a CTA writes; most parts
-static_assert(JOIN_THREADS == D, "a thread per channel");
+constexpr int JOIN_THREADS = 128, JOIN_WARPS = JOIN_THREADS / 32, JOIN_TOKENS = 1024;   // tokens whose weights a CTA writes
+constexpr int JOIN_EARLY = 4;   // ... whose logits a thread requests first of all
 
 // CTA: a (sequence, query head) and a share of its own tokens.  With M the largest of all logits (base 2) the parts' outputs are
 // scaled by 2^(m - M), the cache's by its own sum, and the sum of all of them divides.  The weights are formed from the
 // fp32 logits again: scaling the fp16 probabilities that the V pass has written would round them twice.
+// Nothing here is much work; what takes the time is one round trip to L2 after the other, so that a row's parts are read by four
+// warps at once and the logits are requested before the sums are known.
 __global__ void __launch_bounds__(JOIN_THREADS) join_prefix_kernel(const __grid_constant__ JoinParams P) {
-  const int row = blockIdx.x, tid = threadIdx.x, plane = row / P.r4, head = row - plane * P.r4;
-  __shared__ float2 warp_ml[2][JOIN_THREADS / 32];
-  __shared__ float part_f[JOIN_PARTS];
+  const int row = blockIdx.x, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, plane = row / P.r4, head = row - plane * P.r4;
+  __shared__ float2 warp_ml[2][JOIN_WARPS];
+  __shared__ float warp_o[JOIN_WARPS][D];
   const float2* pairs = P.k_part + static_cast<int64_t>(row) * P.nk_ctas;
+  const float* logits = P.logits + static_cast<int64_t>(plane) * P.r4 * P.L;
+  const int begin = blockIdx.y * JOIN_TOKENS + tid, end = min(P.L, (static_cast<int>(blockIdx.y) + 1) * JOIN_TOKENS);
+  asm volatile("griddepcontrol.launch_dependents;");
   asm volatile("griddepcontrol.wait;" ::: "memory");
+  float early[JOIN_EARLY];
+#pragma unroll
+  for (int k = 0; k < JOIN_EARLY; ++k) early[k] = begin + k * JOIN_THREADS < end ? __ldcg(logits + logit_at(begin + k * JOIN_THREADS, head, P.r4, P.L)) : 0.f;
   // (maximum, sum) of the cache and of the prefix, in base 2
   float m = -INFINITY, l = 0.f, pm = -INFINITY, pl = 0.f;
   auto add = [](float& m, float& l, float m2, float l2) {
@@ -2477,44 +2485,54 @@ __global__ void __launch_bounds__(JOIN_THREADS) join_prefix_kernel(const __grid_
     l = l * fast_exp2(m - ref) + l2 * fast_exp2(m2 - ref);
     m = mx;
   };
-  for (int c = tid; c < P.nk_ctas; c += JOIN_THREADS) add(m, l, pairs[c].x * LOG2E, pairs[c].y);
+  for (int c = tid; c < P.nk_ctas; c += JOIN_THREADS) {
+    const float2 pair = __ldcg(pairs + c);
+    add(m, l, pair.x * LOG2E, pair.y);
+  }
   for (int s = tid; s < P.parts; s += JOIN_THREADS) {
-    const float2 part = P.part_ml[static_cast<int64_t>(s) * P.rows + row];
+    const float2 part = __ldcg(P.part_ml + static_cast<int64_t>(s) * P.rows + row);
     add(pm, pl, part.x, part.y);
-    part_f[s] = part.x;
   }
 #pragma unroll
   for (int k = 1; k < 32; k <<= 1) {
     add(m, l, __shfl_xor_sync(0xffffffffu, m, k), __shfl_xor_sync(0xffffffffu, l, k));
     add(pm, pl, __shfl_xor_sync(0xffffffffu, pm, k), __shfl_xor_sync(0xffffffffu, pl, k));
   }
-  if ((tid & 31) == 0) warp_ml[0][tid >> 5] = make_float2(m, l), warp_ml[1][tid >> 5] = make_float2(pm, pl);
+  if (lane == 0) warp_ml[0][warp] = make_float2(m, l), warp_ml[1][warp] = make_float2(pm, pl);
   __syncthreads();
   m = -INFINITY, l = 0.f;
 #pragma unroll
-  for (int w = 0; w < JOIN_THREADS / 32; ++w) add(m, l, warp_ml[0][w].x, warp_ml[0][w].y);
+  for (int w = 0; w < JOIN_WARPS; ++w) add(m, l, warp_ml[0][w].x, warp_ml[0][w].y);
   const float own_m = m, own_l = l;
 #pragma unroll
-  for (int w = 0; w < JOIN_THREADS / 32; ++w) add(m, l, warp_ml[1][w].x, warp_ml[1][w].y);
+  for (int w = 0; w < JOIN_WARPS; ++w) add(m, l, warp_ml[1][w].x, warp_ml[1][w].y);
   const float ref = m == -INFINITY ? 0.f : m, inv = 1.f / l;
   if (blockIdx.y == 0) {
-    const int64_t at = static_cast<int64_t>(row) * D + tid;
-    float o = own_l * fast_exp2(own_m - ref) * P.own[at];
-    const float* from = P.part_o + at;
-#pragma unroll 8
-    for (int s = 0; s < P.parts; ++s) {   // (every part has tokens, and a row that sees them)
-      o += fast_exp2(part_f[s] - ref) * *from;
-      from += static_cast<int64_t>(P.rows) * D;
-    }
-    P.out[at] = __float2half_rn(o * inv);
-  }
-  const float* logits = P.logits + static_cast<int64_t>(plane) * P.r4 * P.L;
-  __half* weights = P.weights + static_cast<int64_t>(row) * P.L;
-  const int end = min(P.L, (static_cast<int>(blockIdx.y) + 1) * JOIN_TOKENS);
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
-  for (int t = blockIdx.y * JOIN_TOKENS + tid; t < end; t += JOIN_THREADS)
-    weights[t] = __float2half_rn(fast_exp2(fmaf(logits[logit_at(t, head, P.r4, P.L)], LOG2E, -ref)) * inv);
+    for (int s = warp; s < P.parts; s += JOIN_WARPS) {   // (every part has tokens, and a row that sees them)
+      const int64_t at = static_cast<int64_t>(s) * P.rows + row;
+      const float f = fast_exp2(__ldcg(P.part_ml + at).x - ref);
+      const float4 v = __ldcg(reinterpret_cast<const float4*>(P.part_o + at * D + 4 * lane));
+      o.x = fmaf(f, v.x, o.x), o.y = fmaf(f, v.y, o.y), o.z = fmaf(f, v.z, o.z), o.w = fmaf(f, v.w, o.w);
+    }
+    *reinterpret_cast<float4*>(&warp_o[warp][4 * lane]) = o;
+    __syncthreads();
+    const int64_t at = static_cast<int64_t>(row) * D + tid;
+    float sum = own_l * fast_exp2(own_m - ref) * __ldcg(P.own + at);
+#pragma unroll
+    for (int w = 0; w < JOIN_WARPS; ++w) sum += warp_o[w][tid];
+    P.out[at] = __float2half_rn(sum * inv);
+  }
+  __half* weights = P.weights + static_cast<int64_t>(row) * P.L;
+#pragma unroll
+  for (int k = 0; k < JOIN_EARLY; ++k)
+    if (begin + k * JOIN_THREADS < end) weights[begin + k * JOIN_THREADS] = __float2half_rn(fast_exp2(fmaf(early[k], LOG2E, -ref)) * inv);
+#pragma unroll 4
+  for (int t = begin + JOIN_EARLY * JOIN_THREADS; t < end; t += JOIN_THREADS)
+    weights[t] = __float2half_rn(fast_exp2(fmaf(__ldcg(logits + logit_at(t, head, P.r4, P.L)), LOG2E, -ref)) * inv);
 }
+static_assert(JOIN_THREADS == D, "a thread per channel");
 
 // the prefix's side of such a call
 static hqkv_prompt_t prefix_of(const hqkv_cache_desc_t* c, int64_t prefix_len) {
@@ -2590,7 +2608,6 @@ extern "C" int hqkv_decode_attention_prefix(const hqkv_cache_desc_t* cache_host,
   cfg.stream = st;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  HQKV_REQUIRE(J.parts <= JOIN_PARTS, "decode_prefix: too many parts");
   HQKV_CUDA(cudaLaunchKernelEx(&cfg, join_prefix_kernel, J));
   return HQKV_OK;
 }

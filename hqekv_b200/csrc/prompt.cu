@@ -21,7 +21,7 @@ __device__ __forceinline__ float to_float(__half x) { return __half2float(x); }
 template <>
 __device__ __forceinline__ float to_float(__nv_bfloat16 x) { return __bfloat162float(x); }
 
-__device__ __forceinline__ int start_of(const int* starts, int s, int total) { return min(max(starts[s], 0), total); }
+__device__ __forceinline__ int start_of(const int* starts, int s, int total) { return min(max(__ldcg(starts + s), 0), total); }
 
 // ------------------------------------------------------------------------------------------------
 // Attention
@@ -732,6 +732,7 @@ __global__ void __launch_bounds__(256) prompt_join_kernel(const PromptArgs A) {
   const int lane = threadIdx.x & 31;
   if (row >= rows) return;
   const int token = static_cast<int>(row / A.nh_q), head = static_cast<int>(row % A.nh_q);
+  asm volatile("griddepcontrol.launch_dependents;");
   asm volatile("griddepcontrol.wait;" ::: "memory");
   int parts = 0;   // of the token's rows; rows in no sequence have none
   for (int s = lane; s < A.n_seqs; s += 32) {
@@ -744,15 +745,15 @@ __global__ void __launch_bounds__(256) prompt_join_kernel(const PromptArgs A) {
   const float2* const ml = A.part_ml + row;
   const float* const po = A.part_o + row * 128 + 4 * lane;
   float m = -INFINITY, l = 0.f;
-  for (int s = lane; s < parts; s += 32) m = fmaxf(m, ml[s * rows].x);
+  for (int s = lane; s < parts; s += 32) m = fmaxf(m, __ldcg(ml + s * rows).x);
 #pragma unroll
   for (int k = 1; k < 32; k <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, k));
   const float ref = m == -INFINITY ? 0.f : m;
   float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
   for (int s = 0; s < parts; ++s) {
-    const float2 part = ml[s * rows];
-    const float4 v = *reinterpret_cast<const float4*>(po + s * rows * 128);
+    const float2 part = __ldcg(ml + s * rows);
+    const float4 v = __ldcg(reinterpret_cast<const float4*>(po + s * rows * 128));
     const float f = exp2_approx(part.x - ref);
     if (part.y != 0.f) l += f * part.y, o.x += f * v.x, o.y += f * v.y, o.z += f * v.z, o.w += f * v.w;   // (else it has no output)
   }
@@ -955,7 +956,7 @@ __global__ void __launch_bounds__(IMP_THREADS, 1) importance_kernel(const __grid
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
           const int column = lane + 32 * k, r = column / HB, head = item * HB + column % HB;
-          v[k] = item < n && r < t ? 1.4426950408889634f * __ldg(from + static_cast<int64_t>(head) * A.total_q + r) : 0.f;
+          v[k] = item < n && r < t ? 1.4426950408889634f * __ldcg(from + static_cast<int64_t>(head) * A.total_q + r) : 0.f;
         }
       };
       load(0);
