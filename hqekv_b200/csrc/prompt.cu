@@ -44,7 +44,6 @@ constexpr int PROMPT_THREADS = 512;
 constexpr int PROMPT_CTAS = 148;                         // one per SM
 constexpr unsigned TMEM_COLUMNS = 512;
 constexpr float RESCALE_AT = 8.f;                        // powers of two that P may exceed 1 by
-constexpr int BY_POLYNOMIAL = 0;                         // of 16 pairs of exponentials
 
 struct Place {   // a block of a sequence, and where the sequence's queries and keys are
   int q0, lq, k0, lk, block, rest;   // rest: head group and share
@@ -152,27 +151,6 @@ __device__ __forceinline__ uint32_t add_zeros(uint32_t sum, uint32_t v) {   // s
   if constexpr (BF16) asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(v), "r"(0u), "r"(sum));
   else asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(v), "r"(0u), "r"(sum));
   return r;
-}
-
-// 2^x of two numbers without the special function unit, which would otherwise take as long as the matrix products: x = n + f with
-// |f| <= 1/2, a polynomial of degree 5 in f with the least largest relative error (7.5e-8; coefficients by Remez's exchange), n added
-// to the exponent.  x is at most 8 here; below -126 the result is 2^-126.
-__device__ __forceinline__ void exp2_polynomial(uint64_t x2, float& a, float& b) {
-  unpair(x2, a, b);
-  x2 = pair(fmaxf(a, -126.f), fmaxf(b, -126.f));
-  const uint64_t whole = pair(12582912.f, 12582912.f), minus = pair(-12582912.f, -12582912.f), sign = pair(-1.f, -1.f);   // 1.5 * 2^23
-  const uint64_t t = pair_add(x2, whole), f = pair_fma(pair_add(t, minus), sign, x2);
-  auto c = [](float v) { return pair(v, v); };
-  uint64_t p = pair_fma(c(0.00132764724f), f, c(0.00967554096f));
-  p = pair_fma(p, f, c(0.0555071309f));
-  p = pair_fma(p, f, c(0.240221202f));
-  p = pair_fma(p, f, c(0.693146944f));
-  p = pair_fma(p, f, c(1.00000012f));
-  float n, m;
-  unpair(t, n, m);
-  unpair(p, a, b);
-  a = __int_as_float(__float_as_int(a) + (__float_as_int(n) << 23));
-  b = __int_as_float(__float_as_int(b) + (__float_as_int(m) << 23));
 }
 
 struct ItemCount {
@@ -350,12 +328,8 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1) prompt_kernel(const __grid_
           for (int k = 0; k < 16; ++k) {
             float x, y;
             const uint64_t e = pair_fma(pair(__uint_as_float(s[c + 2 * k]), __uint_as_float(s[c + 2 * k + 1])), scale2, shift2);
-            if (k * BY_POLYNOMIAL % 16 < BY_POLYNOMIAL) {
-              exp2_polynomial(e, x, y);
-            } else {
-              unpair(e, x, y);
-              x = exp2_approx(x), y = exp2_approx(y);
-            }
+            unpair(e, x, y);
+            x = exp2_approx(x), y = exp2_approx(y);
             sums[k & 1] = pair_add(sums[k & 1], pair(x, y));
             p[k] = narrow2<BF16>(x, y);
             if (c == TILE - 32 && k == 7) {
@@ -586,8 +560,7 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1) prompt_kernel(const __grid_
     }
     if (!ok && lane == 0) {   // products in flight end before the CTA does
       mma_commit(smem_u32(&sh.drained[a]));
-      for (int k = 0; k < WAIT_TRIES && !bar_try(smem_u32(&sh.drained[a]), 0); ++k) {
-      }
+      bar_drain(smem_u32(&sh.drained[a]), 0);
     }
   } else if (warp == 9) {
     // ---- items, and their copies: Q, then K and V of one tile after the other
@@ -644,8 +617,7 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1) prompt_kernel(const __grid_
       ok = __all_sync(0xffffffffu, ok);
       // (an answer that does not come is waited for even where something else has gone wrong: it lands in this CTA's memory)
       if (!__all_sync(0xffffffffu, bar_wait(smem_u32(&sh.next_full), asked & 1, stop)) || !ok) {
-        for (int k = 0; k < WAIT_TRIES && !bar_try(smem_u32(&sh.next_full), asked & 1); ++k) {
-        }
+        bar_drain(smem_u32(&sh.next_full), asked & 1);
         ok = false;
         break;
       }
@@ -657,10 +629,7 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1) prompt_kernel(const __grid_
     w.over = true;
     if (ok) publish();
     if (lane == 0 && !ok) {   // copies in flight land before the CTA ends
-      auto landed = [&](const unsigned long long& bar, unsigned parity) {
-        for (int k = 0; k < WAIT_TRIES && !bar_try(smem_u32(&bar), parity); ++k) {
-        }
-      };
+      auto landed = [&](const unsigned long long& bar, unsigned parity) { bar_drain(smem_u32(&bar), parity); };
       if (used) landed(sh.q_full, q_phase);
       for (int k = 0; k < KV_STAGES; ++k) {
         if (!(used >> k & 1)) continue;
@@ -911,8 +880,7 @@ __global__ void __launch_bounds__(IMP_THREADS, 1) importance_kernel(const __grid
     }
     if (!ok && lane == 0) {   // products in flight end before the CTA does
       mma_commit(smem_u32(&sh.drained));
-      for (int k = 0; k < WAIT_TRIES && !bar_try(smem_u32(&sh.drained), 0); ++k) {
-      }
+      bar_drain(smem_u32(&sh.drained), 0);
     }
   } else if (warp == 9) {
     const uint32_t tiles_at = smem_u32(tiles);
@@ -942,8 +910,7 @@ __global__ void __launch_bounds__(IMP_THREADS, 1) importance_kernel(const __grid
       for (int i = 1; i <= used; ++i) {
         const int at = (stage - i + G.stages) % G.stages;
         const unsigned parity = at < stage ? phase ^ 1 : phase;
-        for (int k = 0; k < WAIT_TRIES && !bar_try(smem_u32(&sh.full[at]), parity); ++k) {
-        }
+        bar_drain(smem_u32(&sh.full[at]), parity);
       }
   } else if (warp == 10) {
     bool ok = true;
@@ -1001,7 +968,7 @@ static int prompt_args(const hqkv_prompt_t* p, bool values, PromptArgs& A) {
   HQKV_REQUIRE(p->n_seqs >= 0 && p->total_q >= 0 && p->total_k >= 0 && p->prefix_len >= 0, "prompt: negative size");
   HQKV_REQUIRE(p->total_q < (1ll << 30) && p->total_k < (1ll << 30) && p->prefix_len < (1ll << 30) && p->n_seqs < (1 << 24),
                "prompt: too many tokens or sequences");
-  HQKV_REQUIRE(p->scale > 0.f && p->scale < INFINITY, "prompt: the scale must be positive and finite");
+  HQKV_REQUIRE(p->scale > 0.f && p->scale < 1e38f, "prompt: the scale must be positive, and below 1e38");
   const bool own = p->total_k > 0, before = p->prefix_len > 0;
   if (p->total_q > 0) {
     HQKV_REQUIRE(p->q && (!own || (p->k && (p->v || !values))) && (!before || (p->prefix_k && (p->prefix_v || !values))), "prompt: null pointer");

@@ -17,8 +17,10 @@ __device__ __forceinline__ bool elect_one() {
 }
 __device__ __forceinline__ int uniform(int v) { return __shfl_sync(0xffffffffu, v, 0); }
 
-// ---- mbarriers.  Every wait has a limit (a second or so); what runs out sets `stop`, which ends the waits of all roles of the CTA.
-constexpr int WAIT_TRIES = 1 << 24;
+// ---- mbarriers.  Every wait has a limit; what runs out sets `stop`, which ends the waits of all roles of the CTA.  A try that fails takes
+// 4 us: 33 seconds (an item with 2^30 keys takes 15, and some roles wait for all of it), and 4 for what a CTA has under way when
+// something else has gone wrong.
+constexpr int WAIT_TRIES = 1 << 23, DRAIN_TRIES = 1 << 20;
 __device__ __forceinline__ void bar_init(uint32_t bar, unsigned count) {
   asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory");
 }
@@ -45,6 +47,10 @@ __device__ __forceinline__ bool bar_wait(uint32_t bar, unsigned parity, volatile
   }
   *stop = 1;
   return false;
+}
+__device__ __forceinline__ void bar_drain(uint32_t bar, unsigned parity) {
+  for (int i = 0; i < DRAIN_TRIES && !bar_try(bar, parity); ++i) {
+  }
 }
 
 // registers per thread of a warpgroup (four warps, all of which come here)

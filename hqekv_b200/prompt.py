@@ -67,8 +67,8 @@ def _describe(q, k, v, seq_starts, kv_starts, prefix, causal, scale):
     else:
         kv_starts = _starts("kv_starts", kv_starts, q.device, seq_starts.numel())
     scale = HEAD_DIM ** -0.5 if scale is None else float(scale)
-    if not 0.0 < scale < float("inf"):
-        raise ValueError("scale must be positive and finite")
+    if not 0.0 < scale < 1e38:
+        raise ValueError("scale must be positive, and below 1e38")
     p = Prompt()
     p.dtype, p.D, p.nh_q, p.nh_kv = _DTYPES[q.dtype], HEAD_DIM, nh, nkv
     p.n_seqs, p.causal, p.scale = seq_starts.numel() - 1, int(bool(causal)), scale
@@ -98,7 +98,7 @@ def prompt_attention(q, k, v, seq_starts, kv_starts=None, *, prefix=None, causal
     (query heads of one kv head are neighbours).  ``kv_starts``: where the keys of each sequence begin, if they are not those of
     the queries; a causal query sees its own keys up to its distance from the end (query i of Lq sees keys j <= i + Lk - Lq), so a
     chunk of a prompt attends to all that is cached before it.  ``prefix`` = (k, v) [P, nh_kv, 128]: tokens that every query of every
-    sequence sees before its own keys.  ``scale``: 1 / sqrt(128) if not given.  ``out``: a contiguous, 32-byte aligned tensor to write to.
+    sequence sees before its own keys.  ``scale``: 1 / sqrt(128) if not given.  ``out``: a contiguous, 32-byte aligned tensor to write to, other memory than the inputs'.
 
     ``lse`` is the natural logarithm of each row's softmax denominator.  A query that sees no key has output 0 and lse -inf.
     Rows of queries in no sequence (behind the last start, or before the first) are not written: in ``out`` they stay as they were,

@@ -512,7 +512,7 @@ typedef struct {
   int32_t D;             /* head dim, must be 128 */
   int32_t nh_q, nh_kv;   /* nh_q a multiple of nh_kv; query heads of one kv head are neighbours */
   int32_t n_seqs, causal;
-  float scale;           /* multiplies q.k; positive */
+  float scale;           /* multiplies q.k; positive, below 1e38 */
   int64_t total_q, total_k, prefix_len;
   const void *q, *k, *v, *prefix_k, *prefix_v;
   int64_t q_token, q_head, k_token, k_head, v_token, v_head;
@@ -531,7 +531,7 @@ size_t hqkv_prompt_workspace_bytes(const hqkv_prompt_t* prompt_host);
 int hqkv_prompt_attention(const hqkv_prompt_t* prompt_host, void* out, float* lse, void* workspace, size_t workspace_bytes, void* stream);
 
 /*
- * The kernel's waits for its own copies and products have a limit of some seconds.  A CTA in which one runs out ends without a
+ * The kernels' waits for their own copies and products have a limit (33 seconds; an item of 2^30 keys takes 15).  A CTA in which one runs out ends without a
  * result and is counted here: 0 unless the GPU is not working properly.  Waits for the device's work and (optionally) clears the count.
  */
 int hqkv_prompt_waits_expired(int reset, unsigned* count_host);

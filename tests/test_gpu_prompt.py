@@ -221,6 +221,8 @@ def test_nothing_to_do(ops):
     empty, k = randn(1, 0, 4, D), randn(2, 30, 2, D)
     out, lse = ops.attention(empty, k, k, starts([0]), starts([30]))
     assert out.shape == (0, 4, D) and lse.shape == (4, 0)
+    out, lse = ops.attention(randn(1, 5, 4, D), k[:0], k[:0], starts([3, 2]), starts([0, 0]))
+    assert bool((out == 0).all()) and bool((lse == -math.inf).all())
     out, _ = ops.attention(randn(1, 5, 4, D), k, k, starts([]), starts([]), out=torch.full((5, 4, D), 3.0, device="cuda", dtype=torch.float16))
     assert bool((out == 3).all())
     assert bool((ops.importance(empty, k, torch.zeros(4, 0, device="cuda"), starts([0]), starts([30])) == 0).all())
@@ -435,3 +437,19 @@ def test_prompt_then_decode(ops, cuda_device):
     assert float((o[:, :, 0] - out.view(B, S, nh, D)[:, -1]).abs().max()) <= 2.0 ** -9
     got = w.double().sum(1)[:, 0]
     assert float((rows[-1].view(B, S).double() - got).abs().max()) <= 2.0 ** -11 * nh
+
+
+def test_many_sequences(ops):
+    """More sequences than a warp looks up at a time, empty ones among them, more blocks than CTAs."""
+    rng = np.random.default_rng(5)
+    q_len = [int(n) for n in rng.integers(0, 9, 500)]
+    k_len = [n + int(m) for n, m in zip(q_len, rng.integers(0, 200, 500))]
+    q, k, v = randn(1, sum(q_len), 8, D), randn(2, sum(k_len), 2, D), randn(3, sum(k_len), 2, D)
+    check(ops, q, k, v, q_len, k_len)
+
+
+def test_waits_did_not_run_out():
+    import ctypes
+    from hqekv_b200 import _lib
+    count = ctypes.c_uint(7)
+    assert _lib.lib.hqkv_prompt_waits_expired(1, ctypes.byref(count)) == 0 and count.value == 0

@@ -42,6 +42,7 @@ GOOD = dict(q=z(5, 4, 128), k=z(5, 2, 128), v=z(5, 2, 128), seq_starts=starts(0,
     (dict(scale=float("nan")), "scale"),
     (dict(scale=-1.0), "scale"),
     (dict(scale=float("inf")), "scale"),
+    (dict(scale=2e38), "scale"),
 ])
 def test_prompt_attention_refuses(change, text):
     with pytest.raises(ValueError, match=text):
