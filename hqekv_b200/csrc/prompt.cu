@@ -37,6 +37,15 @@ __device__ __forceinline__ int start_of(const int* starts, int s, int total) { r
 // An item is a block of queries, a head group and a share of the keys.  The grid has a CTA per item, but one CTA per SM does the work: when
 // warp 9 begins an item it asks for one that has not been launched yet, looks it up while the others are at work and leaves it in shared
 // memory for them.  (Items in a fixed order per CTA: with four prompts of 4 k, some CTAs had 11 % more than their share.)
+//   What bounds it.  Of 16 k tokens, 32 heads over 8: tensor cores 75 % of the cycles, special function units 74 %, issue slots 40 %, DRAM
+// 3 %.  A tile of keys takes some 3000 cycles, 2048 of them products; a row tile's chain is S (512), softmax (2000: 128 columns at 8 cycles
+// of the special function unit a warp, the maximum before, the last stores after), PV (512), and the other row tile's work lies in its
+// softmax.  32 heads, us and TFLOP/s a call: 8 k tokens 415 and 1325, all of them seen 785 and 1400, 4 x 4 k 442 and 1245, 8 x 1000 92 and
+// 715.  In a long run the power limit decides: 32 k tokens 7.3 ms, 1205 TFLOP/s at 1410 MHz and 990 W (a library product of 8192^3
+// under the same limit 1409).
+//   Why 256 rows: K and V of a tile are 64 KB from L2 for every CTA, 2.6 KB a cycle for all of them at this rate; with 128 rows it would be twice
+// that.  Why heads of a group side by side: a block of four heads is 64 tokens long, so its last tiles are half as empty and its row
+// tiles as long as each other, and eight tokens of 32 heads fill it.
 constexpr int TILE = 128;                                // keys per tile, rows per row tile
 constexpr int TILE_BYTES = TILE * 128 * 2;               // 64 channels of all its tokens, then the other 64
 constexpr int KV_STAGES = 5;
@@ -163,6 +172,8 @@ __device__ __forceinline__ bool look_up(const PromptArgs& A, Walk<ItemCount>& wa
   w.over = false;
   if (!walk.find(item, w.at)) return false;
   const int lq = w.at.lq, lk = w.at.lk, half = 1 << (A.block_shift - 1);
+  // (where keys are shared out, the last block of a sequence comes last: with a single row tile it takes half as long as the others)
+  if (A.shares > 1) w.at.block = ((lq + 2 * half - 1) >> A.block_shift) - 1 - w.at.block;
   w.share = A.shares == 1 ? 0 : w.at.rest / A.groups;
   const int group = w.at.rest - w.share * A.groups;
   w.head0 = group * A.group;
@@ -738,6 +749,9 @@ __global__ void __launch_bounds__(256) prompt_join_kernel(const PromptArgs A) {
 // A tile of keys of one sequence and all heads, HB query heads of a kv head at a time: S^T = K Q^T with the keys as the matrix's rows,
 // so that a thread holds all queries and heads of its key and the sum over the heads needs no other thread.  One CTA per SM goes
 // from tile to tile; what it works on next is on its way meanwhile.
+//   What bounds it: K from HBM, once (10.3 us for 32 k tokens of 8 heads at the copy bandwidth; 16 in a graph of such calls), as long as the
+// first copies of all CTAs, which come together, and the launch are a good part of it.  Beside K every tile takes the queries of all
+// heads from L2, 20 KB a kv head for 28 KB of K.  With a tile per CTA, two buffers and sums in shared memory it took 30 us.
 //   warps 0-3, 4-7   exponentials and sums, a key per thread, every other eight columns (column = query * HB + head) each
 //   warp 8           matrix products, into one of four places in tensor memory
 //   warp 9           copies (K of a kv head and the last queries of the HB heads)
@@ -1026,7 +1040,7 @@ static int prompt_shares(PromptArgs& A) {
       }
     }
     else per = max(int64_t{4}, ceil_div(blocks * average, 3 * PROMPT_CTAS));
-    per = max(per, ceil_div(most, max(int64_t{1}, 8 * PROMPT_CTAS / blocks)));   // (the parts take memory)
+    per = max(per, ceil_div(most, max(int64_t{1}, 10 * PROMPT_CTAS / blocks)));   // (the parts take memory)
   }
   A.per_share = static_cast<int>(per);
   A.shares = static_cast<int>(max(int64_t{1}, ceil_div(most, per)));
