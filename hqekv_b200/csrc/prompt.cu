@@ -171,21 +171,21 @@ struct ItemCount {
 __device__ __forceinline__ bool look_up(const PromptArgs& A, Walk<ItemCount>& walk, int item, Item& w) {
   w.over = false;
   if (!walk.find(item, w.at)) return false;
-  const int lq = w.at.lq, lk = w.at.lk, half = 1 << (A.block_shift - 1);
+  const int lq = w.at.lq, lk = w.at.lk, half = 1 << A.row_shift, block = 1 << A.block_shift;
   // (where keys are shared out, the last block of a sequence comes last: with a single row tile it takes half as long as the others)
-  if (A.shares > 1) w.at.block = ((lq + 2 * half - 1) >> A.block_shift) - 1 - w.at.block;
+  if (A.shares > 1) w.at.block = ((lq + block - 1) >> A.block_shift) - 1 - w.at.block;
   w.share = A.shares == 1 ? 0 : w.at.rest / A.groups;
   const int group = w.at.rest - w.share * A.groups;
   w.head0 = group * A.group;
   w.kv = group / A.groups_per_kv;
   w.i0 = w.at.block << A.block_shift;
   w.part = A.partial || shares_of(A, lq, lk) > 1;
-  w.paired = w.i0 + half >= lq;
+  w.paired = block == half || w.i0 + half >= lq;
   w.before = tiles_of(A.prefix_len);
   w.seen_first = keys_seen(A, w.i0, lq, lk);
-  w.seen_last = keys_seen(A, min(w.i0 + 2 * half, lq) - 1, lq, lk);
+  w.seen_last = keys_seen(A, min(w.i0 + block, lq) - 1, lq, lk);
   const int n0 = w.before + tiles_of(keys_seen(A, min(w.i0 + half, lq) - 1, lq, lk));
-  const int n1 = w.i0 + half < lq ? w.before + tiles_of(w.seen_last) : 0;
+  const int n1 = !w.paired ? w.before + tiles_of(w.seen_last) : 0;
   w.lo = min(w.share * A.per_share, max(n0, n1));
   w.hi = min(w.lo + A.per_share, max(n0, n1));
   w.hi0 = min(w.hi, n0), w.hi1 = min(w.hi, n1);
@@ -219,7 +219,7 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1) prompt_kernel(const __grid_
   const uint32_t q_at = smem_u32(tiles), kv_at = q_at + 2 * TILE_BYTES;
   const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
   asm volatile("griddepcontrol.launch_dependents;");   // (a kernel behind this one waits for its end before it reads results)
-  const int half = 1 << (A.block_shift - 1);   // tokens per row tile
+  const int half = 1 << A.row_shift;   // tokens per row tile
   volatile int* const stop = &sh.stop;
   if (warp == 8) tmem_alloc(smem_u32(&sh.tmem), TMEM_COLUMNS);
   if (threadIdx.x == 0) {
@@ -274,7 +274,7 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1) prompt_kernel(const __grid_
   else fewer_registers<88>();
   if (warp < 8) {
     // ---- softmax
-    const int a = warp >> 2, row = threadIdx.x & 127, token = row >> (8 - A.block_shift);
+    const int a = warp >> 2, row = threadIdx.x & 127, token = row >> (7 - A.row_shift);
     const uint32_t lanes = tmem + (static_cast<uint32_t>(warp & 3) << 21);   // (32 lanes a warp, in bits 16 and up)
     const uint32_t s_at = lanes + a * TILE, o_at = lanes + 2 * TILE + a * 128;
     const float scale = A.scale_log2;
@@ -372,7 +372,7 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1) prompt_kernel(const __grid_
     }
   } else if (warp >= 12) {
     // ---- output: a row of each row tile per thread, or of a paired item the one row that both halves have worked on
-    const int row = threadIdx.x & 127, token = row >> (8 - A.block_shift);
+    const int row = threadIdx.x & 127, token = row >> (7 - A.row_shift);
     const uint32_t o_at = tmem + (static_cast<uint32_t>(warp & 3) << 21) + 2 * TILE;
     const int64_t rows = static_cast<int64_t>(A.total_q) * A.nh_q;
     unsigned ml_phase = 0, o_phase[2] = {0, 0};
@@ -966,8 +966,9 @@ __global__ void __launch_bounds__(IMP_THREADS, 1) importance_kernel(const __grid
 // ------------------------------------------------------------------------------------------------
 // Query heads that share a row tile: those of one kv head, as many of them as a power of two takes (at most 32: four tokens).
 static void set_groups(PromptArgs& A) {
-  A.group = 1, A.block_shift = 8;
-  while (A.group < 32 && A.nh_q / A.nh_kv % (2 * A.group) == 0) A.group *= 2, --A.block_shift;
+  A.group = 1, A.row_shift = 7;
+  while (A.group < 32 && A.nh_q / A.nh_kv % (2 * A.group) == 0) A.group *= 2, --A.row_shift;
+  A.block_shift = A.row_shift + 1;
   A.groups = A.nh_q / A.group;
   A.groups_per_kv = A.groups / A.nh_kv;
 }
@@ -1022,10 +1023,20 @@ static int64_t most_blocks(const PromptArgs& A) {
   return (A.total_q + n * (tokens - 1)) >> A.block_shift;
 }
 
+// Blocks of one row tile, on which both halves of a CTA work, where there are at most two whole ones per SM and they see little but
+// their own prompts.  us, 32 heads over 8, whole blocks / halves: 300 tokens 12.6 / 9.2, 1024 21.2 / 18.6, 2048 44.0 / 42.3, 2500 54 / 58,
+// 4096 117 / 138; 3 x 500 21.7 / 18.1, 8 x 200 18.5 / 16.1, 8 x 300 23.3 / 23.4, 8 x 1000 85 / 96.  (Many keys before the queries are better shared
+// out: two blocks of half the rows read them twice.)
+static void choose_blocks(PromptArgs& A) {
+  if (A.n_seqs > 0 && most_blocks(A) * A.groups <= 2 * PROMPT_CTAS && static_cast<int64_t>(A.prefix_len) + A.total_k - A.total_q <= A.total_q)
+    A.block_shift = A.row_shift;
+}
+
 // Tiles of keys per share, and the shares that a block has at most.  Where the blocks do not fill the GPU, their keys are shared out:
 // for one sequence so that it takes the least time in all - a microsecond a tile, and every share's parts are written and read - with at most
 // an item for every CTA; for several, of unknown lengths, into shares of which a CTA gets about three.
 static int prompt_shares(PromptArgs& A) {
+  choose_blocks(A);
   const int64_t blocks = most_blocks(A) * A.groups, n = max(1, A.n_seqs);
   const int64_t most = ceil_div(A.prefix_len, TILE) + ceil_div(A.total_k, TILE);
   int64_t per = max(int64_t{1}, most);

@@ -15,7 +15,7 @@ struct PromptArgs {
   const int *q_starts, *k_starts;                   // [n_seqs + 1]
   int n_seqs, total_q, total_k, prefix_len, nh_q, nh_kv;
   int group, groups, groups_per_kv;                 // query heads of a kv head that share a row tile; such groups
-  int block_shift;                                  // log2 of the tokens of a block (two row tiles)
+  int row_shift, block_shift;                       // log2 of the tokens of a row tile, of a block (one or two row tiles)
   int per_share, shares;                            // tiles of keys per share of a block's; most shares
   bool causal, bf16, partial;                       // partial: part_o and part_ml are the result
   float scale_log2;                                 // scale * log2(e)
