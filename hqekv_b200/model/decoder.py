@@ -101,13 +101,16 @@ class HqeDecoder(nn.Module):
         P = x.shape[1]
         rope = rotary_tables(torch.arange(P, device=x.device).unsqueeze(0), self.cfg.head_dim, self.cfg.rope_theta, x.dtype)
         starts = torch.tensor([0, P], dtype=torch.int32, device=x.device)
+        prefixes = []
         for layer in self.layers:
             a = layer.self_attn
             q, k, v = (t[0].transpose(0, 1) for t in a._project(layer.input_layernorm(x), rope))
             out, _ = prompt_attention(q, k, v, starts, scale=a.scaling)
             x = x + a.o_proj(out.view(1, P, -1))
             x = x + layer.mlp(layer.post_attention_layernorm(x))
-            a.set_prefix(k.contiguous(), v.contiguous())
+            prefixes.append((k.contiguous(), v.contiguous()))
+        for layer, kv in zip(self.layers, prefixes):   # (all of them or none, should a layer above fail)
+            layer.self_attn.set_prefix(*kv)
         self.prefix_length = P
 
     def start_sequence(self, max_length: int):

@@ -153,3 +153,23 @@ def test_c_abi_refuses_prefix_decodes():
     assert call(pbytes=lib.hqkv_decode_prefix_workspace_bytes(C.byref(d), 6) - 1) == -3
     d.D = 64
     assert lib.hqkv_decode_prefix_workspace_bytes(C.byref(d), 6) == 0 and call() == -1
+
+
+def test_a_prefix_that_fails_leaves_none(monkeypatch):
+    """Every layer has the shared prefix or none has: a failure in the second of two layers leaves none."""
+    from hqekv_b200.model import decoder
+    calls = []
+
+    def attention(q, k, v, starts, **kw):
+        calls.append(1)
+        if len(calls) == 2:
+            raise RuntimeError("out of memory")
+        return torch.zeros_like(q), None
+
+    monkeypatch.setattr(decoder, "prompt_attention", attention)
+    model = decoder.HqeDecoder(decoder.DecoderConfig(hidden_size=64, num_layers=2, num_heads=2, num_kv_heads=1, intermediate_size=64))
+    with pytest.raises(RuntimeError, match="out of memory"):
+        model.share_prefix(torch.randn(1, 5, 64))
+    assert model.prefix_length == 0 and all(layer.self_attn.prefix is None for layer in model.layers)
+    model.share_prefix(torch.randn(1, 5, 64))
+    assert model.prefix_length == 5 and all(layer.self_attn.prefix[0].shape == (5, 1, 128) for layer in model.layers)
