@@ -40,8 +40,8 @@ __device__ __forceinline__ int start_of(const int* starts, int s, int total) { r
 //   What bounds it.  Of 16 k tokens, 32 heads over 8: tensor cores 75 % of the cycles, special function units 74 %, issue slots 40 %, DRAM
 // 3 %.  A tile of keys takes some 3000 cycles, 2048 of them products; a row tile's chain is S (512), softmax (2000: 128 columns at 8 cycles
 // of the special function unit a warp, the maximum before, the last stores after), PV (512), and the other row tile's work lies in its
-// softmax.  32 heads, us and TFLOP/s a call: 8 k tokens 415 and 1325, all of them seen 785 and 1400, 4 x 4 k 442 and 1245, 8 x 1000 92 and
-// 715.  In a long run the power limit decides: 32 k tokens 7.3 ms, 1205 TFLOP/s at 1410 MHz and 990 W (a library product of 8192^3
+// softmax.  32 heads, us and TFLOP/s a call: 8 k tokens 415 and 1325, all of them seen 785 and 1400, 4 x 4 k 442 and 1245, 8 x 1000 85 and
+// 770.  In a long run the power limit decides: 32 k tokens 7.3 ms, 1205 TFLOP/s at 1410 MHz and 990 W (a library product of 8192^3
 // under the same limit 1409).
 //   Why 256 rows: K and V of a tile are 64 KB from L2 for every CTA, 2.6 KB a cycle for all of them at this rate; with 128 rows it would be twice
 // that.  Why heads of a group side by side: a block of four heads is 64 tokens long, so its last tiles are half as empty and its row
@@ -511,9 +511,12 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1) prompt_kernel(const __grid_
       if (!wait(smem_u32(&sh.q_full), q_phase)) break;
       q_phase ^= 1;
       if (paired) {
-        // tile by tile, and those of the other half of the CTA are let go.  (No turns: copies take longer than products here.)
+        // Tile by tile, and those of the other half of the CTA are let go.  Turns as below, given when the next S is under way: a half's
+        // product waits for the other's S of a tile ahead, whose stages its own products have left by then.  (One prompt of 2048
+        // tokens 42.4 us without, 40.4 with; 1500 27.5, 26.8; 4 x 512 22.0, 22.4; 300 and 1024, decodes behind prefixes the same.)
         q_operand = operand(q_at, 16);
         const int first = lo + a;
+        int turns = (hi - lo) / 2;   // products that both halves have
         if (first >= end) commit(sh.q_empty);
 #pragma unroll 1
         for (int i = lo; i < hi; ++i) {
@@ -521,15 +524,26 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1) prompt_kernel(const __grid_
           if (!wait(smem_u32(&sh.kv_full[stage]), kv_phase)) break;
           if (mine) {
             scores();
+            if (i > first && turns > 0) {
+              --turns;
+              if (elect_one()) bar_arrive(smem_u32(&sh.turn[a ^ 1]));
+            }
             if (i + 2 >= end) commit(sh.q_empty);
           }
           release(stage, mine);
           advance();
           if (!wait(smem_u32(&sh.kv_full[stage]), kv_phase)) break;
           if (mine) {
+            if (turns > 0) {
+              if (!wait(smem_u32(&sh.turn[a]), turn)) break;
+              turn ^= 1;
+            }
             values(stage, i > first);
             if (!ok) break;
-            if (i + 2 >= end) commit(sh.o_full[a]);
+            if (i + 2 >= end) {
+              commit(sh.o_full[a]);
+              if (turns > 0 && elect_one()) bar_arrive(smem_u32(&sh.turn[a ^ 1]));
+            }
           }
           release(stage, mine);
           advance();
@@ -1024,7 +1038,7 @@ static int64_t most_blocks(const PromptArgs& A) {
 }
 
 // Blocks of one row tile, on which both halves of a CTA work, where there are at most two whole ones per SM and they see little but
-// their own prompts.  us, 32 heads over 8, whole blocks / halves: 300 tokens 12.6 / 9.2, 1024 21.2 / 18.6, 2048 44.0 / 42.3, 2500 54 / 58,
+// their own prompts.  us, 32 heads over 8, whole blocks / halves: 300 tokens 12.6 / 9.2, 1024 21.2 / 18.7, 2048 44.0 / 40.4, 2500 54 / 58,
 // 4096 117 / 138; 3 x 500 21.7 / 18.1, 8 x 200 18.5 / 16.1, 8 x 300 23.3 / 23.4, 8 x 1000 85 / 96.  (Many keys before the queries are better shared
 // out: two blocks of half the rows read them twice.)
 static void choose_blocks(PromptArgs& A) {
