@@ -8,6 +8,8 @@
 
 #include <cudaTypedefs.h>
 
+#include <limits.h>
+
 #include <type_traits>
 
 #include "tensor.cuh"
@@ -167,24 +169,36 @@ struct ItemCount {
   __device__ __forceinline__ int blocks(int lq, int) const { return (lq + (1 << A.block_shift) - 1) >> A.block_shift; }
   __device__ __forceinline__ int each(int lq, int lk) const { return A.groups * shares_of(A, lq, lk); }
 };
+// Items in front of those that are split: with A.split the ones of an unfilled last round, if they are at most half of one.  Each becomes
+// two, of a row tile each, which both halves of a CTA work on in less than two thirds of the time.  Items and rounds of
+// 32 heads over 8, us without and with: 9 x 300 behind 8192 (2.4 rounds) 324 and 304, 7 x 330 behind 3000 (2.3) 153 and 137,
+// 16 x 256 behind 8192 (3.5) 497 and 465, 20 x 200 behind 500 (4.3) 59.8 and 57.5, 24 x 400 behind 1000 (9.1) 186.4 and 186.1, 3 x 400 behind
+// 1000 (1.1) 38.2 and 38.4.
+__device__ __forceinline__ int whole_items(const PromptArgs& A, const Walk<ItemCount>& walk) {
+  const int all = static_cast<int>(min(__shfl_sync(0xffffffffu, walk.sum, 31), static_cast<long long>(INT_MAX))), rest = all % PROMPT_CTAS;
+  return A.split && rest <= PROMPT_CTAS / 2 ? all - rest : INT_MAX;
+}
 // false: there are fewer items
-__device__ __forceinline__ bool look_up(const PromptArgs& A, Walk<ItemCount>& walk, int item, Item& w) {
+__device__ __forceinline__ bool look_up(const PromptArgs& A, Walk<ItemCount>& walk, int whole, int item, Item& w) {
   w.over = false;
+  const bool split = item >= whole;
+  const int second = split ? (item - whole) & 1 : 0;   // of the two row tiles that a split item's block has
+  if (split) item = whole + ((item - whole) >> 1);
   if (!walk.find(item, w.at)) return false;
-  const int lq = w.at.lq, lk = w.at.lk, half = 1 << A.row_shift, block = 1 << A.block_shift;
+  const int lq = w.at.lq, lk = w.at.lk, half = 1 << A.row_shift, block = 1 << A.block_shift, tokens = split ? half : block;
   // (where keys are shared out, the last block of a sequence comes last: with a single row tile it takes half as long as the others)
   if (A.shares > 1) w.at.block = ((lq + block - 1) >> A.block_shift) - 1 - w.at.block;
   w.share = A.shares == 1 ? 0 : w.at.rest / A.groups;
   const int group = w.at.rest - w.share * A.groups;
   w.head0 = group * A.group;
   w.kv = group / A.groups_per_kv;
-  w.i0 = w.at.block << A.block_shift;
+  w.i0 = (w.at.block << A.block_shift) + second * half;
   w.part = A.partial || shares_of(A, lq, lk) > 1;
-  w.paired = block == half || w.i0 + half >= lq;
+  w.paired = tokens == half || w.i0 + half >= lq;
   w.before = tiles_of(A.prefix_len);
   w.seen_first = keys_seen(A, w.i0, lq, lk);
-  w.seen_last = keys_seen(A, min(w.i0 + block, lq) - 1, lq, lk);
-  const int n0 = w.before + tiles_of(keys_seen(A, min(w.i0 + half, lq) - 1, lq, lk));
+  w.seen_last = keys_seen(A, min(w.i0 + tokens, lq) - 1, lq, lk);
+  const int n0 = w.i0 < lq ? w.before + tiles_of(keys_seen(A, min(w.i0 + half, lq) - 1, lq, lk)) : 0;
   const int n1 = !w.paired ? w.before + tiles_of(w.seen_last) : 0;
   w.lo = min(w.share * A.per_share, max(n0, n1));
   w.hi = min(w.lo + A.per_share, max(n0, n1));
@@ -590,6 +604,7 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1) prompt_kernel(const __grid_
   } else if (warp == 9) {
     // ---- items, and their copies: Q, then K and V of one tile after the other
     Walk<ItemCount> walk(A, ItemCount{A});
+    const int whole = whole_items(A, walk);
     Item w;
     int stage = 0, round = 0, asked = 0;
     unsigned kv_phase = 1, q_phase = 1, to_raw = 0, raw_parity = 0, full_parity = 0, used = 0;   // a bit per stage: of the last copy into it
@@ -609,7 +624,7 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1) prompt_kernel(const __grid_
         bar_expect(smem_u32(&sh.next_full), 16);
         request_cta(smem_u32(&sh.next), smem_u32(&sh.next_full));
       }
-      if (look_up(A, walk, next, w)) publish();
+      if (look_up(A, walk, whole, next, w)) publish();
       else w.lo = w.hi = 0;
       if (ok && w.hi > w.lo && lane == 0) {
         if ((ok = bar_wait(smem_u32(&sh.q_empty), q_phase, stop))) {
@@ -1069,6 +1084,9 @@ static int prompt_shares(PromptArgs& A) {
   }
   A.per_share = static_cast<int>(per);
   A.shares = static_cast<int>(max(int64_t{1}, ceil_div(most, per)));
+  // (as many sequences as a warp counts at a time, and items of like length: most of what they see lies before their queries, or all see all)
+  A.split = A.shares == 1 && A.n_seqs >= 1 && A.n_seqs <= 32 && A.block_shift > A.row_shift &&
+            (!A.causal || int64_t{n} * A.prefix_len + A.total_k - A.total_q >= A.total_q);
   return A.shares;
 }
 
@@ -1129,7 +1147,7 @@ static int launch_prompt(PromptArgs& A, int shares, cudaStream_t st) {
     HQKV_CUDA(cudaFuncSetAttribute(prompt_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(PROMPT_SMEM)));
     if (dev >= 0 && dev < 64) opted_in[dev] = true;
   }
-  const int64_t items = most_blocks(A) * A.groups * shares;
+  const int64_t items = most_blocks(A) * A.groups * shares + (A.split ? PROMPT_CTAS / 2 : 0);
   HQKV_REQUIRE(items < (1ll << 30), "prompt: too many rows");
   return launch_behind(A.bf16 ? prompt_kernel<true> : prompt_kernel<false>, items, PROMPT_THREADS, PROMPT_SMEM, st, A, M);
 }

@@ -17,7 +17,7 @@ struct PromptArgs {
   int group, groups, groups_per_kv;                 // query heads of a kv head that share a row tile; such groups
   int row_shift, block_shift;                       // log2 of the tokens of a row tile, of a block (one or two row tiles)
   int per_share, shares;                            // tiles of keys per share of a block's; most shares
-  bool causal, bf16, partial;                       // partial: part_o and part_ml are the result
+  bool causal, bf16, partial, split;                // partial: part_o and part_ml are the result; split: items of the last round may be (prompt.cu)
   float scale_log2;                                 // scale * log2(e)
   void* out;                                        // [total_q][nh_q][128]
   float* lse;                                       // [nh_q][total_q]

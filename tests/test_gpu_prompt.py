@@ -143,6 +143,39 @@ def test_rising_logits(ops):
         check(ops, q, k, v, [1400], [1400], scale=1.0)
 
 
+@pytest.mark.parametrize("q_len, k_len, heads, before, causal", [
+    ([64] * 20, [64] * 20, (32, 8), 300, True),                       # 160 blocks and head groups: twelve more than SMs
+    ([17] * 21, [17] * 21, (32, 8), 400, True),                       # ... of which the second row tiles are empty
+    ([100, 1, 0, 95, 129, 64, 65, 33, 128, 40, 97, 127, 31], [400, 30, 5, 95, 700, 0, 65, 600, 128, 333, 97, 900, 131], (32, 8), 0, True),
+    ([2600], [2600], (32, 8), 0, False),
+    ([150 + i % 10 for i in range(32)], [400 + 3 * i for i in range(32)], (8, 1), 129, True),
+    ([150 + i % 10 for i in range(33)], [400 + 3 * i for i in range(33)], (8, 1), 129, True),   # more sequences than a warp counts at a time
+    ([70] * 14, [70] * 14, (24, 24), 1000, False),                    # no groups of heads; second row tiles are empty
+])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_last_round_split(ops, q_len, k_len, heads, before, causal, dtype):
+    """A few blocks more than fill the GPU a number of times: those of the last round are halved."""
+    nh, nkv = heads
+    q, k, v = randn(1, sum(q_len), nh, D, dtype=dtype), randn(2, sum(k_len), nkv, D, dtype=dtype), randn(3, sum(k_len), nkv, D, dtype=dtype)
+    prefix = (randn(4, before, nkv, D, dtype=dtype), randn(5, before, nkv, D, dtype=dtype)) if before else None
+    check(ops, q, k, v, q_len, k_len, prefix, causal)
+
+
+def test_last_round_split_odd_values(ops):
+    """Infinities in V at a key that only some rows of a halved block see reach those rows alone, and NaN that none of them sees nobody."""
+    n, length = 20, 64
+    q, k, v = randn(1, n * length, 32, D), randn(2, n * length, 8, D), randn(3, n * length, 8, D)
+    prefix, at = (randn(4, 300, 8, D), randn(5, 300, 8, D)), starts([length] * n)
+    want, want_lse = ops.attention(q, k, v, at, prefix=prefix)
+    first = (n - 1) * length       # the last sequence, whose items are the last
+    v[first + 20, :, 5], v[first + 50, :, 7], k[first + 63, :, 0], v[first + 63, :, 9] = math.inf, -math.inf, math.nan, math.nan
+    out, lse = ops.attention(q, k, v, at, prefix=prefix)
+    assert bool((out[first + 20:first + 63, :, 5] == math.inf).all()) and bool((out[first + 50:first + 63, :, 7] == -math.inf).all())
+    out[first + 20:first + 63, :, 5], out[first + 50:first + 63, :, 7] = want[first + 20:first + 63, :, 5], want[first + 50:first + 63, :, 7]
+    assert bool(out[first + 63].isnan().all()) and bool(lse[:, first + 63].isnan().all())
+    assert torch.equal(out[:first + 63], want[:first + 63]) and torch.equal(lse[:, :first + 63], want_lse[:, :first + 63])
+
+
 def test_strides_and_alignment(ops):
     """Heads before tokens, rows of a wider matrix, expanded heads, and bases on 2-byte boundaries."""
     q_len = [130, 70]
