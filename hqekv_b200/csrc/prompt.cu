@@ -53,6 +53,7 @@ constexpr int TILE_BYTES = TILE * 128 * 2;               // 64 channels of all i
 constexpr int KV_STAGES = 5;
 constexpr int PROMPT_THREADS = 512;
 constexpr int PROMPT_CTAS = 148;                         // one per SM
+constexpr int SHARE_TILES = 4;                           // fewest tiles of keys per share
 constexpr unsigned TMEM_COLUMNS = 512;
 constexpr float RESCALE_AT = 8.f;                        // powers of two that P may exceed 1 by
 
@@ -96,19 +97,59 @@ __device__ __forceinline__ int keys_seen(const PromptArgs& A, int i, int lq, int
   return A.causal ? min(max(i + 1 + lk - lq, 0), lk) : lk;
 }
 __device__ __forceinline__ int tiles_of(int keys) { return (keys + TILE - 1) / TILE; }
-// shares that the keys of a sequence's blocks are divided into
-__device__ __forceinline__ int shares_of(const PromptArgs& A, int lq, int lk) {
-  return A.shares == 1 ? 1 : max(1, (tiles_of(A.prefix_len) + tiles_of(keys_seen(A, lq - 1, lq, lk)) + A.per_share - 1) / A.per_share);
+// tiles of keys that the last of a sequence's blocks sees, and shares of `per` tiles that the keys of its blocks are divided into
+__device__ __forceinline__ int most_tiles(const PromptArgs& A, int lq, int lk) { return tiles_of(A.prefix_len) + tiles_of(keys_seen(A, lq - 1, lq, lk)); }
+__device__ __forceinline__ int shares_of(const PromptArgs& A, int per, int lq, int lk) {
+  return A.shares == 1 ? 1 : max(1, (most_tiles(A, lq, lk) + per - 1) / per);
+}
+// Where the sizes of shares follow from the lengths, a block that begins at query i0 and has one row tile, of two that there may be,
+// gets half as many tiles more (a tile of its keys takes 1.05 us, that of two row tiles 1.7).
+__device__ __forceinline__ int longer(int per) { return per + per / 2; }
+__device__ __forceinline__ bool is_longer(const PromptArgs& A, int i0, int lq) {
+  return A.by_length && A.block_shift > A.row_shift && i0 + (1 << A.row_shift) >= lq;
+}
+// Tiles per share, for a warp that holds a sequence per lane (none: lq = 0): the fewest that make an item for every CTA at most, or
+// two where that is faster - an item takes as long as its tiles and some three more.  Every lane tries another size.  us with one
+// size chosen from the average length for three items per CTA, and with this (queries and keys up to, 32 heads over 8): 4 x 96, 16 k
+// 74.4 and 67.5; 8 heads over 2: 5 x 81, 43 k 68.0 and 49.1, 30 x 60, 3 k 51 and 32, 12 x 243, 11 k 96 and 84.
+__device__ __forceinline__ int share_size(const PromptArgs& A, int lq, int lk) {
+  constexpr unsigned all = 0xffffffffu;
+  const int lane = threadIdx.x & 31, round = PROMPT_CTAS / A.groups;   // blocks of a head group that CTAs are there for
+  const int tiles = lq > 0 ? most_tiles(A, lq, lk) : 0, blocks = min((lq + (1 << A.block_shift) - 1) >> A.block_shift, PROMPT_CTAS);
+  const int shorter = blocks > 0 && is_longer(A, (blocks - 1) << A.block_shift, lq) ? 1 : 0, whole = blocks - shorter;
+  const int least = max(SHARE_TILES, __reduce_max_sync(all, (tiles + A.shares - 1) / A.shares));   // (there is room for A.shares)
+  const int most = max(least, __reduce_max_sync(all, tiles)), n = __reduce_add_sync(all, blocks);
+  // Between work / per and work / per + n items.  (Quotients in fp32 are exact enough for 2^22 tiles; what depends on them is the number
+  // of items alone.)
+  const float work = static_cast<float>(__reduce_add_sync(all, static_cast<unsigned>(3 * whole + 2 * shorter) * tiles)) * (1.f / 3.f);
+  const int low = max(least, static_cast<int>(__fdividef(work, static_cast<float>(2 * round))));
+  const int high = max(low, n < round ? min(most, static_cast<int>(__fdividef(work, static_cast<float>(round - n))) + 2) : most);
+  const int per = low + (high - low) * lane / 31;
+  const float by = __fdividef(1.f, static_cast<float>(per)), by_longer = __fdividef(1.f, static_cast<float>(longer(per)));
+  int items = 0;
+  for (int s = 0; s < A.n_seqs; ++s) {
+    const float t = static_cast<float>(__shfl_sync(all, tiles, s));
+    items += __shfl_sync(all, whole, s) * __float2int_ru(t * by) + __shfl_sync(all, shorter, s) * __float2int_ru(t * by_longer);
+  }
+  const unsigned in_one = __ballot_sync(all, items <= round) | 1u << 31, in_two = __ballot_sync(all, items <= 2 * round) | 1u << 31;
+  const int one = __shfl_sync(all, per, __ffs(in_one) - 1), two = __shfl_sync(all, per, __ffs(in_two) - 1);
+  return one <= 2 * two + 3 ? one : two;
 }
 
 // Walks the sequences in order, 32 at a time (a lane each), to the one that holds an item.  Items are asked for in rising order, mostly.
 template <typename Count>
 struct Walk {
   const PromptArgs& A;
-  Count count;   // items of (lq, lk), and those of one block
+  Count count;   // blocks of (lq, lk), items of each and of the last
   int lane, at = 0, q0 = 0, lq = 0, k0 = 0, lk = 0;
   long long before = 0, sum = 0;   // (what starts that are not in order add up to may be anything)
-  __device__ __forceinline__ Walk(const PromptArgs& args, Count c) : A(args), count(c), lane(threadIdx.x & 31) { look(); }
+  __device__ __forceinline__ Walk(const PromptArgs& args, Count c) : A(args), count(c), lane(threadIdx.x & 31) {
+    look();
+    if constexpr (!Count::EVEN) {
+      count.choose(lq, lk);
+      add_up();
+    }
+  }
   __device__ __forceinline__ void look() {
     const int s = at + lane;
     q0 = lq = k0 = lk = 0;
@@ -117,7 +158,12 @@ struct Walk {
       q0 = start_of(A.q_starts, s, A.total_q), k0 = start_of(A.k_starts, s, A.total_k);
       lq = max(start_of(A.q_starts, s + 1, A.total_q) - q0, 0), lk = max(start_of(A.k_starts, s + 1, A.total_k) - k0, 0);
     }
-    sum = static_cast<long long>(count.blocks(lq, lk)) * count.each(lq, lk);
+    add_up();
+  }
+  __device__ __forceinline__ void add_up() {
+    const int blocks = count.blocks(lq, lk);
+    sum = static_cast<long long>(blocks) * count.each(lq, lk);
+    if constexpr (!Count::EVEN) sum += blocks > 0 ? count.last(lq, lk) - count.each(lq, lk) : 0;
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
       const long long up = __shfl_up_sync(0xffffffffu, sum, d);
@@ -144,7 +190,9 @@ struct Walk {
     auto get = [&](int v) { return __shfl_sync(0xffffffffu, v, from); };
     p.q0 = get(q0), p.lq = get(lq), p.k0 = get(k0), p.lk = get(lk);
     const int each = count.each(p.lq, p.lk), blocks = count.blocks(p.lq, p.lk);
-    const int i = item - static_cast<int>(before + __shfl_sync(0xffffffffu, sum, from) - static_cast<long long>(blocks) * each), at_block = i / each;
+    long long items = static_cast<long long>(blocks) * each;
+    if constexpr (!Count::EVEN) items += count.last(p.lq, p.lk) - each;
+    const int i = item - static_cast<int>(before + __shfl_sync(0xffffffffu, sum, from) - items), at_block = Count::EVEN ? i / each : min(i / each, blocks - 1);
     p.block = blocks - 1 - at_block, p.rest = i - at_block * each;
     return true;
   }
@@ -164,22 +212,32 @@ __device__ __forceinline__ uint32_t add_zeros(uint32_t sum, uint32_t v) {   // s
   return r;
 }
 
+template <bool BY_LENGTH>   // (A.by_length, of which other calls have no instructions to fetch: inside one kernel it cost them 0.4 to 3 us)
 struct ItemCount {
+  static constexpr bool EVEN = !BY_LENGTH;   // all blocks of a sequence have as many items
   const PromptArgs& A;
+  int per;   // tiles per share, where the lengths decide
+  __device__ __forceinline__ void choose(int lq, int lk) { per = share_size(A, lq, lk); }
   __device__ __forceinline__ int blocks(int lq, int) const { return (lq + (1 << A.block_shift) - 1) >> A.block_shift; }
-  __device__ __forceinline__ int each(int lq, int lk) const { return A.groups * shares_of(A, lq, lk); }
+  __device__ __forceinline__ int size(int i0, int lq) const { return !BY_LENGTH ? A.per_share : is_longer(A, i0, lq) ? longer(per) : per; }
+  __device__ __forceinline__ int each(int lq, int lk) const { return A.groups * shares_of(A, BY_LENGTH ? per : A.per_share, lq, lk); }
+  __device__ __forceinline__ int last(int lq, int lk) const {
+    return A.groups * shares_of(A, size((blocks(lq, lk) - 1) << A.block_shift, lq), lq, lk);
+  }
 };
 // Items in front of those that are split: with A.split the ones of an unfilled last round, if they are at most half of one.  Each becomes
 // two, of a row tile each, which both halves of a CTA work on in less than two thirds of the time.  Items and rounds of
 // 32 heads over 8, us without and with: 9 x 300 behind 8192 (2.4 rounds) 324 and 304, 7 x 330 behind 3000 (2.3) 153 and 137,
 // 16 x 256 behind 8192 (3.5) 497 and 465, 20 x 200 behind 500 (4.3) 59.8 and 57.5, 24 x 400 behind 1000 (9.1) 186.4 and 186.1, 3 x 400 behind
 // 1000 (1.1) 38.2 and 38.4.
-__device__ __forceinline__ int whole_items(const PromptArgs& A, const Walk<ItemCount>& walk) {
+template <typename Count>
+__device__ __forceinline__ int whole_items(const PromptArgs& A, const Walk<Count>& walk) {
   const int all = static_cast<int>(min(__shfl_sync(0xffffffffu, walk.sum, 31), static_cast<long long>(INT_MAX))), rest = all % PROMPT_CTAS;
   return A.split && rest <= PROMPT_CTAS / 2 ? all - rest : INT_MAX;
 }
 // false: there are fewer items
-__device__ __forceinline__ bool look_up(const PromptArgs& A, Walk<ItemCount>& walk, int whole, int item, Item& w) {
+template <typename Count>
+__device__ __forceinline__ bool look_up(const PromptArgs& A, Walk<Count>& walk, int whole, int item, Item& w) {
   w.over = false;
   const bool split = item >= whole;
   const int second = split ? (item - whole) & 1 : 0;   // of the two row tiles that a split item's block has
@@ -193,15 +251,16 @@ __device__ __forceinline__ bool look_up(const PromptArgs& A, Walk<ItemCount>& wa
   w.head0 = group * A.group;
   w.kv = group / A.groups_per_kv;
   w.i0 = (w.at.block << A.block_shift) + second * half;
-  w.part = A.partial || shares_of(A, lq, lk) > 1;
+  const int per = walk.count.size(w.i0, lq);
+  w.part = A.partial || shares_of(A, per, lq, lk) > 1;
   w.paired = tokens == half || w.i0 + half >= lq;
   w.before = tiles_of(A.prefix_len);
   w.seen_first = keys_seen(A, w.i0, lq, lk);
   w.seen_last = keys_seen(A, min(w.i0 + tokens, lq) - 1, lq, lk);
   const int n0 = w.i0 < lq ? w.before + tiles_of(keys_seen(A, min(w.i0 + half, lq) - 1, lq, lk)) : 0;
   const int n1 = !w.paired ? w.before + tiles_of(w.seen_last) : 0;
-  w.lo = min(w.share * A.per_share, max(n0, n1));
-  w.hi = min(w.lo + A.per_share, max(n0, n1));
+  w.lo = min(w.share * per, max(n0, n1));
+  w.hi = min(w.lo + per, max(n0, n1));
   w.hi0 = min(w.hi, n0), w.hi1 = min(w.hi, n1);
   return true;
 }
@@ -225,7 +284,7 @@ __device__ __noinline__ void add_odd_values(const PromptArgs& A, const Item& w, 
   }
 }
 
-template <bool BF16>
+template <bool BF16, bool BY_LENGTH>
 __global__ void __launch_bounds__(PROMPT_THREADS, 1) prompt_kernel(const __grid_constant__ PromptArgs A, const __grid_constant__ PromptMaps M) {
   using T = std::conditional_t<BF16, __nv_bfloat16, __half>;
   extern __shared__ __align__(1024) unsigned char tiles[];
@@ -603,8 +662,9 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1) prompt_kernel(const __grid_
     }
   } else if (warp == 9) {
     // ---- items, and their copies: Q, then K and V of one tile after the other
-    Walk<ItemCount> walk(A, ItemCount{A});
-    const int whole = whole_items(A, walk);
+    Walk<ItemCount<BY_LENGTH>> walk(A, ItemCount<BY_LENGTH>{A, A.per_share});
+    const int whole = BY_LENGTH ? INT_MAX : whole_items(A, walk);
+    if (BY_LENGTH && lane == 0) *A.share_size = walk.count.per;   // (for the join; the same from every CTA)
     Item w;
     int stage = 0, round = 0, asked = 0;
     unsigned kv_phase = 1, q_phase = 1, to_raw = 0, raw_parity = 0, full_parity = 0, used = 0;   // a bit per stage: of the last copy into it
@@ -733,7 +793,7 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1) prompt_kernel(const __grid_
   if (threadIdx.x == 0 && *stop) atomicAdd(&g_waits_expired, 1u);
 }
 
-// Joins the parts of a row: a warp per row.
+// Joins the parts of a row: a warp per row.  What takes its time is one round trip to L2 after the other (starts, pairs, outputs).
 template <bool BF16>
 __global__ void __launch_bounds__(256) prompt_join_kernel(const PromptArgs A) {
   using T = std::conditional_t<BF16, __nv_bfloat16, __half>;
@@ -743,28 +803,51 @@ __global__ void __launch_bounds__(256) prompt_join_kernel(const PromptArgs A) {
   const int token = static_cast<int>(row / A.nh_q), head = static_cast<int>(row % A.nh_q);
   asm volatile("griddepcontrol.launch_dependents;");
   asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int per = A.by_length ? __ldcg(A.share_size) : A.per_share;
   int parts = 0;   // of the token's rows; rows in no sequence have none
-  for (int s = lane; s < A.n_seqs; s += 32) {
-    const int q0 = start_of(A.q_starts, s, A.total_q), q1 = start_of(A.q_starts, s + 1, A.total_q);
-    if (token >= q0 && token < q1)
-      parts = shares_of(A, q1 - q0, max(start_of(A.k_starts, s + 1, A.total_k) - start_of(A.k_starts, s, A.total_k), 0));
+  for (int s0 = 0; s0 < A.n_seqs; s0 += 32) {
+    const int s = s0 + lane;
+    int q0 = 0, lq = 0, lk = 0;
+    if (s < A.n_seqs) {
+      q0 = start_of(A.q_starts, s, A.total_q), lq = max(start_of(A.q_starts, s + 1, A.total_q) - q0, 0);
+      lk = max(start_of(A.k_starts, s + 1, A.total_k) - start_of(A.k_starts, s, A.total_k), 0);
+    }
+    const int i0 = (token - q0) >> A.block_shift << A.block_shift;
+    if (token >= q0 && token < q0 + lq) parts = shares_of(A, is_longer(A, i0, lq) ? longer(per) : per, lq, lk);
   }
   parts = __reduce_max_sync(0xffffffffu, parts);
   if (parts < 2) return;   // (in no sequence, or written as a whole)
+  // A lane has the pair of one part, up to 32 at a time; of their outputs eight are on the way at once.
   const float2* const ml = A.part_ml + row;
   const float* const po = A.part_o + row * 128 + 4 * lane;
-  float m = -INFINITY, l = 0.f;
-  for (int s = lane; s < parts; s += 32) m = fmaxf(m, __ldcg(ml + s * rows).x);
-#pragma unroll
-  for (int k = 1; k < 32; k <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, k));
-  const float ref = m == -INFINITY ? 0.f : m;
+  float m = -INFINITY, l = 0.f, ref = 0.f;
   float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-  for (int s = 0; s < parts; ++s) {
-    const float2 part = __ldcg(ml + s * rows);
-    const float4 v = __ldcg(reinterpret_cast<const float4*>(po + s * rows * 128));
-    const float f = exp2_approx(part.x - ref);
-    if (part.y != 0.f) l += f * part.y, o.x += f * v.x, o.y += f * v.y, o.z += f * v.z, o.w += f * v.w;   // (else it has no output)
+#pragma unroll 1
+  for (int first = 0; first < parts; first += 32) {
+    const int n = min(32, parts - first);
+    const float2 part = lane < n ? __ldcg(ml + (first + lane) * rows) : make_float2(-INFINITY, 0.f);
+    float top = part.x;
+#pragma unroll
+    for (int k = 1; k < 32; k <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, k));
+    top = fmaxf(m, top);
+    ref = top == -INFINITY ? 0.f : top;
+    const float before = exp2_approx(m - ref), f = part.y != 0.f ? exp2_approx(part.x - ref) : 0.f;   // (a part whose sum is 0 has no output)
+    float sum = f * part.y;
+#pragma unroll
+    for (int k = 1; k < 32; k <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, k);
+    l = l * before + sum, m = top;
+    o.x *= before, o.y *= before, o.z *= before, o.w *= before;
+#pragma unroll 1
+    for (int s = 0; s < n; s += 8) {
+      float4 v[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v[k] = __ldcg(reinterpret_cast<const float4*>(po + (first + min(s + k, n - 1)) * rows * 128));
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const float by = __shfl_sync(0xffffffffu, f, s + k);   // (0 behind the last)
+        if (by != 0.f) o.x += by * v[k].x, o.y += by * v[k].y, o.z += by * v[k].z, o.w += by * v[k].w;
+      }
+    }
   }
   const float inv = l == 0.f ? 0.f : 1.f / l;
   *reinterpret_cast<uint2*>(static_cast<T*>(A.out) + row * 128 + 4 * lane) =
@@ -801,6 +884,7 @@ static size_t imp_smem(const ImportanceShape& g) {   // (a product reads 128 row
 }
 struct KeyCount {
   int keys;
+  static constexpr bool EVEN = true;
   __device__ __forceinline__ int blocks(int, int lk) const { return (lk + keys - 1) / keys; }
   __device__ __forceinline__ int each(int, int) const { return 1; }
 };
@@ -1063,9 +1147,11 @@ static void choose_blocks(PromptArgs& A) {
 
 // Tiles of keys per share, and the shares that a block has at most.  Where the blocks do not fill the GPU, their keys are shared out:
 // for one sequence so that it takes the least time in all - a microsecond a tile, and every share's parts are written and read - with at most
-// an item for every CTA; for several, of unknown lengths, into shares of which a CTA gets about three.
+// an item for every CTA; for several the kernel chooses when it sees their lengths (share_size), or, where they are more than a warp
+// counts at a time, into shares of which a CTA gets about three on average.
 static int prompt_shares(PromptArgs& A) {
   choose_blocks(A);
+  A.by_length = false;
   const int64_t blocks = most_blocks(A) * A.groups, n = max(1, A.n_seqs);
   const int64_t most = ceil_div(A.prefix_len, TILE) + ceil_div(A.total_k, TILE);
   int64_t per = max(int64_t{1}, most);
@@ -1080,7 +1166,14 @@ static int prompt_shares(PromptArgs& A) {
       }
     }
     else per = max(int64_t{4}, ceil_div(blocks * average, 3 * PROMPT_CTAS));
-    per = max(per, ceil_div(most, max(int64_t{1}, 10 * PROMPT_CTAS / blocks)));   // (the parts take memory)
+    const int64_t room = max(int64_t{1}, 10 * PROMPT_CTAS / blocks);   // (the parts take memory)
+    per = max(per, ceil_div(most, room));
+    // (for few tiles the least share will do, and where the blocks are more than half as many as the CTAs one or two rounds are uneven)
+    A.by_length = n > 1 && n <= 32 && room > 1 && most < (1 << 22) && 5 * blocks <= 3 * PROMPT_CTAS && blocks * average > SHARE_TILES * PROMPT_CTAS;
+    if (A.by_length) {
+      A.per_share = SHARE_TILES;
+      return A.shares = static_cast<int>(min(room, ceil_div(most, SHARE_TILES)));
+    }
   }
   A.per_share = static_cast<int>(per);
   A.shares = static_cast<int>(max(int64_t{1}, ceil_div(most, per)));
@@ -1139,17 +1232,19 @@ static int launch_prompt(PromptArgs& A, int shares, cudaStream_t st) {
     if (int rc = tensor_map(&M.pk, A.pk, A.bf16, A.prefix_len, A.nh_kv, A.pk_token, A.pk_head, 1, TILE)) return rc;
     if (int rc = tensor_map(&M.pv, A.pv, A.bf16, A.prefix_len, A.nh_kv, A.pv_token, A.pv_head, 1, TILE)) return rc;
   }
+  using Kernel = void (*)(PromptArgs, PromptMaps);
+  static const Kernel kernels[4] = {prompt_kernel<false, false>, prompt_kernel<true, false>, prompt_kernel<false, true>, prompt_kernel<true, true>};
   static bool opted_in[64] = {};   // per device
   int dev = 0;
   HQKV_CUDA(cudaGetDevice(&dev));
   if (dev < 0 || dev >= 64 || !opted_in[dev]) {
-    HQKV_CUDA(cudaFuncSetAttribute(prompt_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(PROMPT_SMEM)));
-    HQKV_CUDA(cudaFuncSetAttribute(prompt_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(PROMPT_SMEM)));
+    for (Kernel k : kernels) HQKV_CUDA(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(PROMPT_SMEM)));
     if (dev >= 0 && dev < 64) opted_in[dev] = true;
   }
-  const int64_t items = most_blocks(A) * A.groups * shares + (A.split ? PROMPT_CTAS / 2 : 0);
+  int64_t items = most_blocks(A) * A.groups * shares + (A.split ? PROMPT_CTAS / 2 : 0);
+  if (A.by_length) items = min(items, int64_t{2 * PROMPT_CTAS});
   HQKV_REQUIRE(items < (1ll << 30), "prompt: too many rows");
-  return launch_behind(A.bf16 ? prompt_kernel<true> : prompt_kernel<false>, items, PROMPT_THREADS, PROMPT_SMEM, st, A, M);
+  return launch_behind(kernels[2 * A.by_length + A.bf16], items, PROMPT_THREADS, PROMPT_SMEM, st, A, M);
 }
 
 template <bool BF16, int HB>
@@ -1210,7 +1305,7 @@ int prefix_partial(const hqkv_prompt_t* p, float* part_o, float2* part_ml, cudaS
 static size_t split_bytes(const PromptArgs& A, int shares, size_t* part_ml) {
   const size_t rows = static_cast<size_t>(A.total_q) * A.nh_q * shares;
   *part_ml = rows * 128 * sizeof(float);
-  return shares > 1 ? *part_ml + rows * sizeof(float2) : 0;
+  return shares > 1 ? *part_ml + rows * sizeof(float2) + sizeof(int) : 0;
 }
 
 }  // namespace hqkv
@@ -1240,6 +1335,7 @@ extern "C" int hqkv_prompt_attention(const hqkv_prompt_t* prompt_host, void* out
   if (workspace_bytes < need) return fail(HQKV_E_WORKSPACE, "prompt: the workspace holds %zu bytes, %zu needed", workspace_bytes, need);
   A.part_o = static_cast<float*>(workspace);
   A.part_ml = reinterpret_cast<float2*>(static_cast<unsigned char*>(workspace) + ml);
+  A.share_size = reinterpret_cast<int*>(A.part_ml + static_cast<int64_t>(A.total_q) * A.nh_q * shares);
   if (int rc = launch_prompt(A, shares, st)) return rc;
   return launch_behind(A.bf16 ? prompt_join_kernel<true> : prompt_join_kernel<false>, ceil_div(static_cast<int64_t>(A.total_q) * A.nh_q, 8), 256, 0, st, A);
 }

@@ -16,13 +16,15 @@ struct PromptArgs {
   int n_seqs, total_q, total_k, prefix_len, nh_q, nh_kv;
   int group, groups, groups_per_kv;                 // query heads of a kv head that share a row tile; such groups
   int row_shift, block_shift;                       // log2 of the tokens of a row tile, of a block (one or two row tiles)
-  int per_share, shares;                            // tiles of keys per share of a block's; most shares
-  bool causal, bf16, partial, split;                // partial: part_o and part_ml are the result; split: items of the last round may be (prompt.cu)
+  int per_share, shares;                            // tiles of keys per share of a block's (unless by_length); most shares
+  bool causal, bf16, partial;                       // partial: part_o and part_ml are the result
+  bool split, by_length;                            // items of the last round are halved; tiles per share follow from the lengths (prompt.cu)
   float scale_log2;                                 // scale * log2(e)
   void* out;                                        // [total_q][nh_q][128]
   float* lse;                                       // [nh_q][total_q]
   float* part_o;                                    // [shares][total_q * nh_q][128], not yet normalised
   float2* part_ml;                                  // [shares][total_q * nh_q] (maximum, sum), in powers of two
+  int* share_size;                                  // by_length: what the kernel has chosen
 };
 
 struct PromptMaps {   // the tensors as (channel, head, token), for copies by tiles

@@ -144,6 +144,26 @@ def test_rising_logits(ops):
 
 
 @pytest.mark.parametrize("q_len, k_len, heads, before, causal", [
+    ([96, 37, 73, 14], [5096, 337, 9073, 14], (32, 8), 0, True),      # shares of sizes that follow from the lengths
+    ([96, 37, 0, 73, 14, 60], [5096, 0, 40, 9073, 10, 50], (32, 8), 129, True),   # ... no queries, no keys, fewer keys than queries
+    ([33, 64, 65, 31, 32, 1], [6000, 128, 6001, 129, 2000, 7000], (16, 4), 0, False),
+    ([243 - 20 * i for i in range(12)], [9000 - 700 * i for i in range(12)], (8, 2), 0, True),
+    ([5] * 32, [3000 + 10 * i for i in range(32)], (4, 2), 100, True),
+    ([5] * 33, [3000 + 10 * i for i in range(33)], (4, 2), 100, True),   # more sequences than a warp counts at a time
+    ([300, 290], [12000, 100], (8, 1), 0, True),                      # blocks of 32 tokens
+    ([1, 1], [9000, 20000], (4, 1), 0, True),                         # more shares than a warp joins at a time
+    ([1], [20000], (4, 1), 0, True),
+])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_shares(ops, q_len, k_len, heads, before, causal, dtype):
+    """Few rows and many keys, which are shared out over the GPU and joined."""
+    nh, nkv = heads
+    q, k, v = randn(1, sum(q_len), nh, D, dtype=dtype), randn(2, sum(k_len), nkv, D, dtype=dtype), randn(3, sum(k_len), nkv, D, dtype=dtype)
+    prefix = (randn(4, before, nkv, D, dtype=dtype), randn(5, before, nkv, D, dtype=dtype)) if before else None
+    check(ops, q, k, v, q_len, k_len, prefix, causal)
+
+
+@pytest.mark.parametrize("q_len, k_len, heads, before, causal", [
     ([64] * 20, [64] * 20, (32, 8), 300, True),                       # 160 blocks and head groups: twelve more than SMs
     ([17] * 21, [17] * 21, (32, 8), 400, True),                       # ... of which the second row tiles are empty
     ([100, 1, 0, 95, 129, 64, 65, 33, 128, 40, 97, 127, 31], [400, 30, 5, 95, 700, 0, 65, 600, 128, 333, 97, 900, 131], (32, 8), 0, True),
