@@ -119,7 +119,7 @@ __device__ __forceinline__ int share_size(const PromptArgs& A, int lq, int lk) {
   const int shorter = blocks > 0 && is_longer(A, (blocks - 1) << A.block_shift, lq) ? 1 : 0, whole = blocks - shorter;
   const int least = max(SHARE_TILES, __reduce_max_sync(all, (tiles + A.shares - 1) / A.shares));   // (there is room for A.shares)
   const int most = max(least, __reduce_max_sync(all, tiles)), n = __reduce_add_sync(all, blocks);
-  // Between work / per and work / per + n items.  (Quotients in fp32 are exact enough for 2^22 tiles; what depends on them is the number
+  // Between work / per and work / per + n items.  (Quotients in fp32 are exact enough for 2^21 tiles; what depends on them is the number
   // of items alone.)
   const float work = static_cast<float>(__reduce_add_sync(all, static_cast<unsigned>(3 * whole + 2 * shorter) * tiles)) * (1.f / 3.f);
   const int low = max(least, static_cast<int>(__fdividef(work, static_cast<float>(2 * round))));
@@ -1169,7 +1169,7 @@ static int prompt_shares(PromptArgs& A) {
     const int64_t room = max(int64_t{1}, 10 * PROMPT_CTAS / blocks);   // (the parts take memory)
     per = max(per, ceil_div(most, room));
     // (for few tiles the least share will do, and where the blocks are more than half as many as the CTAs one or two rounds are uneven)
-    A.by_length = n > 1 && n <= 32 && room > 1 && most < (1 << 22) && 5 * blocks <= 3 * PROMPT_CTAS && blocks * average > SHARE_TILES * PROMPT_CTAS;
+    A.by_length = n > 1 && n <= 32 && room > 1 && most < (1 << 21) && 5 * blocks <= 3 * PROMPT_CTAS && blocks * average > SHARE_TILES * PROMPT_CTAS;
     if (A.by_length) {
       A.per_share = SHARE_TILES;
       return A.shares = static_cast<int>(min(room, ceil_div(most, SHARE_TILES)));
