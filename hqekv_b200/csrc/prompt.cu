@@ -486,16 +486,19 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1) prompt_kernel(const __grid_
         float* const part_to = A.part_o + (w.share * rows + at) * 128;
         T* const to = static_cast<T*>(A.out) + at * 128;
         const bool part = w.part;
-        // (Few instructions, gone through eight times: written out at length this took twice as long, most of it to fetch them.)
+        // (Few instructions, gone through eight times: written out at length this took twice as long, most of it to fetch them.  The next
+        // columns are on the way meanwhile: 17 tokens 7.1 / 6.9 us, 2048 41.1 / 40.5.)
+        uint32_t o_next[16] = {}, x[16] = {};
+        if (first) tmem_load16(o_at + half_a * 128, o_next);
 #pragma unroll 1
         for (int c = 0; c < 128; c += 16) {
-          uint32_t o[16] = {}, x[16] = {};
-          if (first) tmem_load16(o_at + half_a * 128 + c, o);
+          uint32_t o[16];
           if (second) tmem_load16(o_at + 128 + c, x);
-          wait_loads(o);
+          wait_loads(o_next);
           wait_loads(x);
 #pragma unroll
-          for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(fmaf(__uint_as_float(x[k]), f1, __uint_as_float(o[k]) * f0));
+          for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(fmaf(__uint_as_float(x[k]), f1, __uint_as_float(o_next[k]) * f0));
+          if (first && c < 112) tmem_load16(o_at + half_a * 128 + c + 16, o_next);
           if (!live) continue;
           if (part) {
             store_sector(part_to + c, o);
