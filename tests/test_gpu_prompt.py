@@ -335,6 +335,31 @@ def test_streams_and_graphs(ops, before):
         assert torch.equal(out, want[i][0]) and torch.equal(lse, want[i][1]) and torch.equal(imp, rows[i])
 
 
+@pytest.mark.parametrize("q_len, k_len, other_q, other_k, before", [
+    ([96, 37, 73, 14], [5096, 337, 9073, 14], [1, 160, 0, 59], [40, 200, 14000, 280], 0),      # shares by length
+    ([64] * 20, [64] * 20, [1280] + [0] * 19, [1280] + [0] * 19, 300),                          # a last round that is halved, and none
+])
+def test_replay_with_other_lengths(ops, q_len, k_len, other_q, other_k, before):
+    """A captured call, whose launches and workspace were chosen without the lengths, replayed with others."""
+    assert sum(q_len) == sum(other_q) and sum(k_len) == sum(other_k)
+    q, k, v = randn(1, sum(q_len), 32, D), randn(2, sum(k_len), 8, D), randn(3, sum(k_len), 8, D)
+    prefix = (randn(4, before, 8, D), randn(5, before, 8, D)) if before else None
+    lengths = [(q_len, k_len), (other_q, other_k)]
+    want = [check(ops, q, k, v, *x, prefix) for x in lengths]
+    at = [(starts(x), starts(y)) for x, y in lengths]
+    a, b = at[0][0].clone(), at[0][1].clone()
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        out, lse = ops.attention(q, k, v, a, b, prefix=prefix)
+    for i in (1, 0, 1):
+        a.copy_(at[i][0])
+        b.copy_(at[i][1])
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want[i][0]) and torch.equal(lse, want[i][1])
+
+
 # ------------------------------------------------------------------------------------------------
 # importance rows
 # ------------------------------------------------------------------------------------------------
