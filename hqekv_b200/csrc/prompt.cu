@@ -291,7 +291,6 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1) prompt_kernel(const __grid_
   PromptShared& sh = *reinterpret_cast<PromptShared*>(tiles + (2 + KV_STAGES) * TILE_BYTES);
   const uint32_t q_at = smem_u32(tiles), kv_at = q_at + 2 * TILE_BYTES;
   const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
-  asm volatile("griddepcontrol.launch_dependents;");   // (a kernel behind this one waits for its end before it reads results)
   const int half = 1 << A.row_shift;   // tokens per row tile
   volatile int* const stop = &sh.stop;
   if (warp == 8) tmem_alloc(smem_u32(&sh.tmem), TMEM_COLUMNS);
@@ -328,6 +327,9 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1) prompt_kernel(const __grid_
   __syncthreads();
   fence_after();
   const uint32_t tmem = uniform(sh.tmem);
+  // The next kernel may start (it waits for this one's end before it reads results) now that the tensor memory is there: a CTA of it
+  // that shared the SM could take all of it, and would keep it while it waits.
+  asm volatile("griddepcontrol.launch_dependents;");
   // (nothing before this reads or writes what an earlier kernel may still be working on)
   asm volatile("griddepcontrol.wait;" ::: "memory");
   // item number `round`, for the warps that work on it; null: there are no more, or a wait has run out
@@ -900,7 +902,6 @@ __global__ void __launch_bounds__(IMP_THREADS, 1) importance_kernel(const __grid
   ImportanceShared& sh = *reinterpret_cast<ImportanceShared*>(tiles + G.stages * stage_bytes + (TILE - G.keys) * 128);
   const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
   const int per_kv = A.nh_q / A.nh_kv / HB, items = A.nh_kv * per_kv;   // products per tile
-  asm volatile("griddepcontrol.launch_dependents;");   // (as in the attention kernel)
   volatile int* const stop = &sh.stop;
   if (warp == 8) tmem_alloc(smem_u32(&sh.tmem), IMP_SLOTS * IMP_COLUMNS);
   if (threadIdx.x == 0) {
@@ -921,6 +922,7 @@ __global__ void __launch_bounds__(IMP_THREADS, 1) importance_kernel(const __grid
   __syncthreads();
   fence_after();
   const uint32_t tmem = uniform(sh.tmem);
+  asm volatile("griddepcontrol.launch_dependents;");   // (with the tensor memory, as in the attention kernel: here two CTAs fit on an SM)
   asm volatile("griddepcontrol.wait;" ::: "memory");
   Walk<KeyCount> walk(A, KeyCount{G.keys});
   Place w;

@@ -17,9 +17,10 @@ __device__ __forceinline__ bool elect_one() {
 }
 __device__ __forceinline__ int uniform(int v) { return __shfl_sync(0xffffffffu, v, 0); }
 
-// ---- mbarriers.  Every wait has a limit; what runs out sets `stop`, which ends the waits of all roles of the CTA.  A try that fails takes
-// 4 us: 33 seconds (an item with 2^30 keys takes 15, and some roles wait for all of it), and 4 for what a CTA has under way when
-// something else has gone wrong.
+// ---- mbarriers.  Every wait for one has a limit; what runs out sets `stop`, which ends the waits of all roles of the CTA.  A try that
+// fails takes 4 us: 33 seconds (an item with 2^30 keys takes 15, and some roles wait for all of it), and 4 for what a CTA has under way
+// when something else has gone wrong.  (Waits for tensor memory and for the kernel before have no limit.  They end: a CTA that has
+// tensor memory waits for earlier kernels at most, whose CTAs have theirs.)
 constexpr int WAIT_TRIES = 1 << 23, DRAIN_TRIES = 1 << 20;
 __device__ __forceinline__ void bar_init(uint32_t bar, unsigned count) {
   asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory");

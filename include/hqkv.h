@@ -531,8 +531,9 @@ size_t hqkv_prompt_workspace_bytes(const hqkv_prompt_t* prompt_host);
 int hqkv_prompt_attention(const hqkv_prompt_t* prompt_host, void* out, float* lse, void* workspace, size_t workspace_bytes, void* stream);
 
 /*
- * The kernels' waits for their own copies and products have a limit (33 seconds; an item of 2^30 keys takes 15).  A CTA in which one runs out ends without a
- * result and is counted here: 0 unless the GPU is not working properly.  Waits for the device's work and (optionally) clears the count.
+ * The kernels' waits for their own copies, products and roles have a limit (33 seconds; an item of 2^30 keys takes 15).  A CTA in which
+ * one runs out ends without a result and is counted here: 0 unless the GPU is not working properly.  (Their waits for tensor memory
+ * and for the kernel before them have none.)  Waits for the device's work and (optionally) clears the count.
  */
 int hqkv_prompt_waits_expired(int reset, unsigned* count_host);
 

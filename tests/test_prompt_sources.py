@@ -1,0 +1,37 @@
+"""CPU-only: an order in the prompt kernels' source that no run shows, since what goes wrong without it is a wait without a limit."""
+import os
+import re
+
+import pytest
+
+CSRC = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "hqekv_b200", "csrc")
+
+
+def kernels():
+    """(name, body) of every kernel, without comments."""
+    found = []
+    for name in sorted(f for f in os.listdir(CSRC) if f.endswith(".cu")):
+        with open(os.path.join(CSRC, name)) as f:
+            text = re.sub(r"//[^\n]*|/\*.*?\*/", "", f.read(), flags=re.S)
+        text = re.sub(r"__launch_bounds__\([^()]*\)", "", text)
+        for m in re.finditer(r"__global__\s+void\s+(\w+)\s*\([^{;]*\)\s*\{", text):
+            end = text.index("\n}", m.end())
+            found.append((m.group(1), text[m.end():end]))
+    return found
+
+
+WITH_TENSOR_MEMORY = [(n, b) for n, b in kernels() if "tmem_alloc(" in b]
+
+
+def test_both_kernels_are_looked_at():
+    assert {n for n, _ in WITH_TENSOR_MEMORY} == {"prompt_kernel", "importance_kernel"}
+
+
+@pytest.mark.parametrize("name, body", WITH_TENSOR_MEMORY, ids=[n for n, _ in WITH_TENSOR_MEMORY])
+def test_tensor_memory_before_the_next_kernel(name, body):
+    """A CTA lets the next kernel start only when it has its tensor memory: a CTA of that kernel which shared the SM could take all
+    of it and would keep it while it waits for this kernel's end."""
+    alloc = body.index("tmem_alloc(")
+    got = body.index("__syncthreads()", alloc)
+    announce = [m.start() for m in re.finditer(r"launch_dependents", body)]
+    assert len(announce) == 1 and alloc < got < announce[0] < body.index("griddepcontrol.wait")
