@@ -335,7 +335,7 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1) prompt_kernel(const __grid_
   // item number `round`, for the warps that work on it; null: there are no more, or a wait has run out
   auto item = [&](int round) -> const Item* {
     const int at = round % ITEMS;
-    if (!__all_sync(0xffffffffu, bar_wait(smem_u32(&sh.item_full[at]), round / ITEMS & 1, stop))) return nullptr;
+    if (!bar_wait(smem_u32(&sh.item_full[at]), round / ITEMS & 1, stop)) return nullptr;
     return sh.items[at].over ? nullptr : &sh.items[at];
   };
   auto done = [&](int round) {
@@ -365,7 +365,7 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1) prompt_kernel(const __grid_
       float ref = -INFINITY, sum = 0.f;
 #pragma unroll 1
       for (int tile = first; tile < end; tile += step) {
-        if (!(ok = __all_sync(0xffffffffu, bar_wait(smem_u32(&sh.s_full[a]), s_phase, stop)))) break;
+        if (!(ok = bar_wait(smem_u32(&sh.s_full[a]), s_phase, stop))) break;
         s_phase ^= 1;
         fence_after();
         uint32_t s[TILE];
@@ -438,7 +438,7 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1) prompt_kernel(const __grid_
         sum += x + y;
       }
       if (!ok) break;
-      if (!(ok = __all_sync(0xffffffffu, bar_wait(smem_u32(&sh.ml_empty), ml_phase, stop)))) break;
+      if (!(ok = bar_wait(smem_u32(&sh.ml_empty), ml_phase, stop))) break;
       ml_phase ^= 1;
       sh.ml[a][row] = make_float2(ref, sum);
       __syncwarp();
@@ -457,7 +457,7 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1) prompt_kernel(const __grid_
       const Item* const item_at = item(round);
       if (!item_at) break;
       const Item& w = *item_at;
-      if (!(ok = __all_sync(0xffffffffu, bar_wait(smem_u32(&sh.ml_full), ml_phase, stop)))) break;
+      if (!(ok = bar_wait(smem_u32(&sh.ml_full), ml_phase, stop))) break;
       ml_phase ^= 1;
       float2 ml[2] = {sh.ml[0][row], sh.ml[1][row]};
       __syncwarp();
@@ -472,7 +472,7 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1) prompt_kernel(const __grid_
       for (int a = 0; a < 2; ++a) {
         const bool any = w.end(a) > w.first(a);
         if (any) {
-          if (!(ok = __all_sync(0xffffffffu, bar_wait(smem_u32(&sh.o_full[a]), o_phase[a], stop)))) break;
+          if (!(ok = bar_wait(smem_u32(&sh.o_full[a]), o_phase[a], stop))) break;
           o_phase[a] ^= 1;
           fence_after();
         }
@@ -676,7 +676,7 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1) prompt_kernel(const __grid_
     bool ok = true;
     auto publish = [&] {
       const int at = round % ITEMS;
-      if (!(ok = __all_sync(0xffffffffu, bar_wait(smem_u32(&sh.item_empty[at]), (round / ITEMS & 1) ^ 1, stop)))) return;
+      if (!(ok = bar_wait(smem_u32(&sh.item_empty[at]), (round / ITEMS & 1) ^ 1, stop))) return;
       if (lane == 0) {
         sh.items[at] = w;
         bar_arrive(smem_u32(&sh.item_full[at]));
@@ -692,7 +692,7 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1) prompt_kernel(const __grid_
       if (look_up(A, walk, whole, next, w)) publish();
       else w.lo = w.hi = 0;
       if (ok && w.hi > w.lo && lane == 0) {
-        if ((ok = bar_wait(smem_u32(&sh.q_empty), q_phase, stop))) {
+        if ((ok = bar_wait_one(smem_u32(&sh.q_empty), q_phase, stop))) {
           q_phase ^= 1;
           bar_expect(smem_u32(&sh.q_full), w.paired ? TILE_BYTES : 2 * TILE_BYTES);
           for (int a = 0; a < (w.paired ? 1 : 2); ++a)
@@ -705,7 +705,7 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1) prompt_kernel(const __grid_
           const int token = own ? w.at.k0 + (i - w.before) * TILE : i * TILE;
 #pragma unroll 1
           for (int side = 0; side < 2; ++side) {
-            if (!(ok = bar_wait(smem_u32(&sh.kv_empty[stage]), kv_phase, stop))) break;
+            if (!(ok = bar_wait_one(smem_u32(&sh.kv_empty[stage]), kv_phase, stop))) break;
             const CUtensorMap* map = side ? (own ? &M.v : &M.pv) : (own ? &M.k : &M.pk);
             const bool raw_first = side && w.partly_seen(i);
             const uint32_t bar = smem_u32(raw_first ? &sh.v_raw[stage] : &sh.kv_full[stage]), bit = 1u << stage;
@@ -721,7 +721,7 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1) prompt_kernel(const __grid_
       }
       ok = __all_sync(0xffffffffu, ok);
       // (an answer that does not come is waited for even where something else has gone wrong: it lands in this CTA's memory)
-      if (!__all_sync(0xffffffffu, bar_wait(smem_u32(&sh.next_full), asked & 1, stop)) || !ok) {
+      if (!bar_wait(smem_u32(&sh.next_full), asked & 1, stop) || !ok) {
         bar_drain(smem_u32(&sh.next_full), asked & 1);
         ok = false;
         break;
@@ -755,7 +755,7 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1) prompt_kernel(const __grid_
       for (int i = max(w.lo, w.before + w.seen_first / TILE); i < w.hi; ++i) {
         const int stage = (fills + 2 * (i - w.lo) + 1) % KV_STAGES, first = (i - w.before) * TILE;
         if (!w.partly_seen(i)) continue;
-        if (!(ok = __all_sync(0xffffffffu, bar_wait(smem_u32(&sh.v_raw[stage]), parity >> stage & 1, stop)))) break;
+        if (!(ok = bar_wait(smem_u32(&sh.v_raw[stage]), parity >> stage & 1, stop))) break;
         parity ^= 1u << stage;
         // x * 0 added up is 0 as long as x is finite.  (Looked at one by one, the values of a tile took 7000 cycles.)
         uint4* const v = reinterpret_cast<uint4*>(tiles + (2 + stage) * TILE_BYTES);   // (which piece of a row comes where does not matter)
@@ -948,7 +948,7 @@ __global__ void __launch_bounds__(IMP_THREADS, 1) importance_kernel(const __grid
       if (t > 0) {
 #pragma unroll 1
         for (int item = 0; item < items; ++item) {
-          if (!(ok = __all_sync(0xffffffffu, bar_wait(smem_u32(&sh.s_full[slot]), slot_phase, stop)))) break;
+          if (!(ok = bar_wait(smem_u32(&sh.s_full[slot]), slot_phase, stop))) break;
           fence_after();
           const uint32_t at = lanes + slot * IMP_COLUMNS;
           const float* const log_sum = sh.log_sum[slot] + 8 * side;
@@ -1026,7 +1026,7 @@ __global__ void __launch_bounds__(IMP_THREADS, 1) importance_kernel(const __grid
       if (lane == 0)
 #pragma unroll 1
         for (int item = 0; item < n; ++item) {
-          if (!(ok = bar_wait(smem_u32(&sh.empty[stage]), phase, stop))) break;
+          if (!(ok = bar_wait_one(smem_u32(&sh.empty[stage]), phase, stop))) break;
           const uint32_t k_at = tiles_at + stage * stage_bytes, q_at = k_at + G.keys * 256, bar = smem_u32(&sh.full[stage]);
           bar_expect(bar, bytes);
           for (int c = 0; c < 2; ++c) {
@@ -1061,7 +1061,7 @@ __global__ void __launch_bounds__(IMP_THREADS, 1) importance_kernel(const __grid
       load(0);
 #pragma unroll 1
       for (int item = 0; item < n; ++item) {
-        if (!(ok = __all_sync(0xffffffffu, bar_wait(smem_u32(&sh.s_empty[slot]), slot_phase ^ 1, stop)))) break;
+        if (!(ok = bar_wait(smem_u32(&sh.s_empty[slot]), slot_phase ^ 1, stop))) break;
 #pragma unroll
         for (int k = 0; k < 4; ++k) sh.log_sum[slot][lane + 32 * k] = v[k];
         load(item + 1);

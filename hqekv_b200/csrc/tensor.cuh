@@ -40,7 +40,8 @@ __device__ __forceinline__ bool bar_try(uint32_t bar, unsigned parity) {
                : "memory");
   return ok != 0;
 }
-__device__ __forceinline__ bool bar_wait(uint32_t bar, unsigned parity, volatile int* stop) {
+// by one thread
+__device__ __forceinline__ bool bar_wait_one(uint32_t bar, unsigned parity, volatile int* stop) {
 #pragma unroll 1
   for (int i = 0; i < WAIT_TRIES; ++i) {
     if (bar_try(bar, parity)) return true;
@@ -48,6 +49,10 @@ __device__ __forceinline__ bool bar_wait(uint32_t bar, unsigned parity, volatile
   }
   *stop = 1;
   return false;
+}
+// By a whole warp, which goes on or gives up as one: what follows (elected threads, copies, barriers of the warp) needs all its lanes.
+__device__ __forceinline__ bool bar_wait(uint32_t bar, unsigned parity, volatile int* stop) {
+  return __all_sync(0xffffffffu, bar_wait_one(bar, parity, stop));
 }
 __device__ __forceinline__ void bar_drain(uint32_t bar, unsigned parity) {
   for (int i = 0; i < DRAIN_TRIES && !bar_try(bar, parity); ++i) {

@@ -35,3 +35,25 @@ def test_tensor_memory_before_the_next_kernel(name, body):
     got = body.index("__syncthreads()", alloc)
     announce = [m.start() for m in re.finditer(r"launch_dependents", body)]
     assert len(announce) == 1 and alloc < got < announce[0] < body.index("griddepcontrol.wait")
+
+
+def branches(body):
+    """What each role of a kernel's warps does."""
+    parts = re.split(r"\n  (?:\} else )?if \(warp [^\n]*\) \{\n", body)
+    return parts[1:]
+
+
+def test_warps_that_elect_give_up_as_one():
+    """An elected thread needs its whole warp: a warp whose lanes left a wait that ran out one by one would wait for them for good.  The
+    waits of one thread belong where that thread alone is at work."""
+    found = 0
+    for name, body in WITH_TENSOR_MEMORY:
+        for part in branches(body):
+            if "elect_one()" in part:
+                found += 1
+                assert "bar_wait_one(" not in part and "bar_wait(" in part, name
+        for m in re.finditer(r"bar_wait_one\(", body):
+            assert "lane == 0" in body[max(0, m.start() - 1200):m.start()], name
+    with open(os.path.join(CSRC, "tensor.cuh")) as f:
+        assert re.search(r"bool bar_wait\([^)]*\) \{\s*return __all_sync\(0xffffffffu, bar_wait_one\(", f.read())
+    assert found >= 2
