@@ -78,10 +78,14 @@ struct Item {
 };
 constexpr int ITEMS = 4;   // looked up at a time
 
+struct LastCopies {   // a bit per stage: of the last copy into it
+  unsigned q_phase, used, to_raw, raw_parity, full_parity;
+};
 struct PromptShared {
   unsigned long long item_full[ITEMS], item_empty[ITEMS], next_full, q_full, q_empty, kv_full[KV_STAGES], kv_empty[KV_STAGES], v_raw[KV_STAGES];
   unsigned long long s_full[2], p_first[2], p_rest[2], o_full[2], o_empty[2], turn[2], drained[2], ml_full, ml_empty;
   uint32_t tmem;
+  LastCopies copies;
   alignas(16) uint4 next;   // answer to the request for an item
   Item items[ITEMS];
   float2 ml[2][TILE];       // (maximum, sum) of the rows
@@ -661,10 +665,6 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1) prompt_kernel(const __grid_
         }
       }
     }
-    if (!ok && lane == 0) {   // products in flight end before the CTA does
-      mma_commit(smem_u32(&sh.drained[a]));
-      bar_drain(smem_u32(&sh.drained[a]), 0);
-    }
   } else if (warp == 9) {
     // ---- items, and their copies: Q, then K and V of one tile after the other
     Walk<ItemCount<BY_LENGTH>> walk(A, ItemCount<BY_LENGTH>{A, A.per_share});
@@ -733,15 +733,7 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1) prompt_kernel(const __grid_
     }
     w.over = true;
     if (ok) publish();
-    if (lane == 0 && !ok) {   // copies in flight land before the CTA ends
-      auto landed = [&](const unsigned long long& bar, unsigned parity) { bar_drain(smem_u32(&bar), parity); };
-      if (used) landed(sh.q_full, q_phase);
-      for (int k = 0; k < KV_STAGES; ++k) {
-        if (!(used >> k & 1)) continue;
-        if (to_raw >> k & 1) landed(sh.v_raw[k], (raw_parity >> k & 1) ^ 1);
-        else landed(sh.kv_full[k], full_parity >> k & 1);
-      }
-    }
+    if (lane == 0) sh.copies = {q_phase, used, to_raw, raw_parity, full_parity};
   } else if (warp == 10) {
     // ---- V tiles that not every row sees
     unsigned parity = 0, fills = 0;   // a bit per stage; copies into stages before this item's
@@ -794,6 +786,23 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1) prompt_kernel(const __grid_
   fence_before();
   __syncthreads();
   fence_after();
+  if (*stop) {   // a wait has run out: what the roles have left in flight ends before the CTA does
+    if ((warp == 8 || warp == 11) && elect_one()) {
+      const uint32_t drained = smem_u32(&sh.drained[warp == 8 ? 0 : 1]);
+      mma_commit(drained);
+      bar_drain(drained, 0);
+    }
+    if (warp == 9 && lane == 0) {
+      const LastCopies c = sh.copies;
+      if (c.used || c.q_phase == 0) bar_drain(smem_u32(&sh.q_full), c.q_phase);
+      for (int k = 0; k < KV_STAGES; ++k) {
+        if (!(c.used >> k & 1)) continue;
+        if (c.to_raw >> k & 1) bar_drain(smem_u32(&sh.v_raw[k]), (c.raw_parity >> k & 1) ^ 1);
+        else bar_drain(smem_u32(&sh.kv_full[k]), c.full_parity >> k & 1);
+      }
+    }
+    __syncthreads();
+  }
   if (warp == 8) tmem_free(tmem, TMEM_COLUMNS);
   if (threadIdx.x == 0 && *stop) atomicAdd(&g_waits_expired, 1u);
 }
@@ -927,6 +936,8 @@ __global__ void __launch_bounds__(IMP_THREADS, 1) importance_kernel(const __grid
   Walk<KeyCount> walk(A, KeyCount{G.keys});
   Place w;
   auto next = [&](int tile) { return tile < G.tiles && walk.find(tile, w); };   // (never more than the starts allow when in order)
+  int copy_stage = 0, used = 0;   // warp 9: where the next copy goes, stages in use
+  unsigned copy_phase = 1;
   int slot = 0;
   unsigned slot_phase = 0;
   auto next_slot = [&] {
@@ -1010,40 +1021,28 @@ __global__ void __launch_bounds__(IMP_THREADS, 1) importance_kernel(const __grid
         next_slot();
       }
     }
-    if (!ok && lane == 0) {   // products in flight end before the CTA does
-      mma_commit(smem_u32(&sh.drained));
-      bar_drain(smem_u32(&sh.drained), 0);
-    }
   } else if (warp == 9) {
     const uint32_t tiles_at = smem_u32(tiles);
     const unsigned bytes = 256u * (G.keys + G.rows * HB);
     bool ok = true;
-    int stage = 0, used = 0;
-    unsigned phase = 1;
 #pragma unroll 1
     for (int tile = blockIdx.x; ok && next(tile); tile += gridDim.x) {
       const int n = w.lq > 0 ? items : 0, token = w.k0 + w.block * G.keys, query = w.q0 + w.lq - min(G.rows, w.lq);
       if (lane == 0)
 #pragma unroll 1
         for (int item = 0; item < n; ++item) {
-          if (!(ok = bar_wait_one(smem_u32(&sh.empty[stage]), phase, stop))) break;
-          const uint32_t k_at = tiles_at + stage * stage_bytes, q_at = k_at + G.keys * 256, bar = smem_u32(&sh.full[stage]);
+          if (!(ok = bar_wait_one(smem_u32(&sh.empty[copy_stage]), copy_phase, stop))) break;
+          const uint32_t k_at = tiles_at + copy_stage * stage_bytes, q_at = k_at + G.keys * 256, bar = smem_u32(&sh.full[copy_stage]);
           bar_expect(bar, bytes);
           for (int c = 0; c < 2; ++c) {
             copy_box(k_at + c * k_half, &M.k, 64 * c, item / per_kv, token, bar);
             copy_box(q_at + c * G.columns * 128, &M.q, 64 * c, item * HB, query, bar);
           }
           if (used < G.stages) ++used;
-          if (++stage == G.stages) stage = 0, phase ^= 1;
+          if (++copy_stage == G.stages) copy_stage = 0, copy_phase ^= 1;
         }
       ok = __all_sync(0xffffffffu, ok);
     }
-    if (!ok && lane == 0)   // copies in flight land before the CTA ends: the last `used` of them, in front of `stage`
-      for (int i = 1; i <= used; ++i) {
-        const int at = (stage - i + G.stages) % G.stages;
-        const unsigned parity = at < stage ? phase ^ 1 : phase;
-        bar_drain(smem_u32(&sh.full[at]), parity);
-      }
   } else if (warp == 10) {
     bool ok = true;
 #pragma unroll 1
@@ -1075,6 +1074,18 @@ __global__ void __launch_bounds__(IMP_THREADS, 1) importance_kernel(const __grid
   fence_before();
   __syncthreads();
   fence_after();
+  if (*stop) {   // as in the attention kernel
+    if (warp == 8 && elect_one()) {
+      mma_commit(smem_u32(&sh.drained));
+      bar_drain(smem_u32(&sh.drained), 0);
+    }
+    if (warp == 9 && lane == 0)
+      for (int i = 1; i <= used; ++i) {   // the last `used` copies, in front of `copy_stage`
+        const int at = (copy_stage - i + G.stages) % G.stages;
+        bar_drain(smem_u32(&sh.full[at]), at < copy_stage ? copy_phase ^ 1 : copy_phase);
+      }
+    __syncthreads();
+  }
   if (warp == 8) tmem_free(tmem, IMP_SLOTS * IMP_COLUMNS);
   if (threadIdx.x == 0 && *stop) atomicAdd(&g_waits_expired, 1u);
 }

@@ -57,3 +57,15 @@ def test_warps_that_elect_give_up_as_one():
     with open(os.path.join(CSRC, "tensor.cuh")) as f:
         assert re.search(r"bool bar_wait\([^)]*\) \{\s*return __all_sync\(0xffffffffu, bar_wait_one\(", f.read())
     assert found >= 2
+
+
+def test_work_in_flight_is_waited_for_whichever_role_gave_up():
+    """A role ends with its own waits in order where another one has given up, too.  So what is under way (products that read shared memory
+    and write tensor memory, copies into shared memory) is waited for when all roles have ended, if any of them gave up."""
+    for name, body in WITH_TENSOR_MEMORY:
+        ended = body.rindex("__syncthreads()", 0, body.rindex("__syncthreads()"))
+        last = re.match(r"__syncthreads\(\);\s*fence_after\(\);\s*if \(\*stop\) \{(.*?)\n    __syncthreads\(\);\n  \}\s*if \(warp == 8\) tmem_free", body[ended:], re.S)
+        assert last, name
+        for what in ("sh.drained", "sh.full[" if name == "importance_kernel" else "sh.kv_full["):
+            assert what in last.group(1), (name, what)
+        assert not re.search(r"(?<!next_full\), )bar_drain\((?!smem_u32\(&sh\.next_full)", body[:ended]), name
