@@ -124,6 +124,7 @@ _SIGNATURES = {
     "hqkv_prompt_workspace_bytes": (C.c_size_t, [C.POINTER(Prompt)]),
     "hqkv_prompt_attention": (C.c_int, [C.POINTER(Prompt), C.c_void_p, C.c_void_p, C.c_void_p, C.c_size_t, C.c_void_p]),
     "hqkv_prompt_waits_expired": (C.c_int, [C.c_int, C.POINTER(C.c_uint)]),
+    "hqkv_prompt_limit_waits": (C.c_int, [C.c_int]),
     "hqkv_prompt_importance": (C.c_int, [C.POINTER(Prompt), C.c_void_p, C.c_int, C.c_void_p, C.c_void_p]),
     "hqkv_decode_prefix_workspace_bytes": (C.c_size_t, [C.POINTER(CacheDesc), C.c_int64]),
     "hqkv_decode_attention_prefix": (C.c_int, [C.POINTER(CacheDesc), C.c_void_p, C.c_void_p, C.c_void_p, C.c_int64, C.c_int64,

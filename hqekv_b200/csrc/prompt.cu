@@ -1364,6 +1364,18 @@ extern "C" int hqkv_prompt_waits_expired(int reset, unsigned* count_host) {
   return HQKV_OK;
 }
 
+extern "C" int hqkv_prompt_limit_waits(int tries) {
+#if HQKV_CHECKS_ENABLED
+  const int n = tries > 0 ? min(tries, WAIT_TRIES) : WAIT_TRIES;
+  HQKV_CUDA(cudaDeviceSynchronize());
+  HQKV_CUDA(cudaMemcpyToSymbol(hqkv::g_wait_tries, &n, sizeof(int)));
+  return HQKV_OK;
+#else
+  (void)tries;
+  return fail(HQKV_E_UNSUPPORTED, "prompt_limit_waits: only the bounds-check build has a limit that can be set");
+#endif
+}
+
 extern "C" int hqkv_prompt_importance(const hqkv_prompt_t* prompt_host, const float* lse, int rows, void* out_f16, void* stream) {
   PromptArgs A;
   if (int rc = prompt_args(prompt_host, false, A)) return rc;

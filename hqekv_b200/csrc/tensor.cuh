@@ -4,6 +4,8 @@
 #include <cuda.h>
 #include <stdint.h>
 
+#include "common.cuh"
+
 namespace hqkv {
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
@@ -22,6 +24,12 @@ __device__ __forceinline__ int uniform(int v) { return __shfl_sync(0xffffffffu, 
 // when something else has gone wrong.  (Waits for tensor memory and for the kernel before have no limit.  They end: a CTA that has
 // tensor memory waits for earlier kernels at most, whose CTAs have theirs.)
 constexpr int WAIT_TRIES = 1 << 23, DRAIN_TRIES = 1 << 20;
+#if HQKV_CHECKS_ENABLED
+static __device__ int g_wait_tries = WAIT_TRIES;   // (the bounds-check build can be told to give up early: hqkv_prompt_limit_waits)
+__device__ __forceinline__ int wait_tries() { return *const_cast<volatile int*>(&g_wait_tries); }
+#else
+__device__ __forceinline__ constexpr int wait_tries() { return WAIT_TRIES; }
+#endif
 __device__ __forceinline__ void bar_init(uint32_t bar, unsigned count) {
   asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory");
 }
@@ -42,8 +50,9 @@ __device__ __forceinline__ bool bar_try(uint32_t bar, unsigned parity) {
 }
 // by one thread
 __device__ __forceinline__ bool bar_wait_one(uint32_t bar, unsigned parity, volatile int* stop) {
+  const int tries = wait_tries();
 #pragma unroll 1
-  for (int i = 0; i < WAIT_TRIES; ++i) {
+  for (int i = 0; i < tries; ++i) {
     if (bar_try(bar, parity)) return true;
     if (*stop) return false;
   }

@@ -150,3 +150,14 @@ def prompt_importance(q, k, lse, seq_starts, kv_starts=None, *, rows=20, causal=
     with torch.cuda.device(q.device):
         check(lib.hqkv_prompt_importance(C.byref(p), ptr(lse), rows, ptr(out), stream_ptr(q.device)))
     return out
+
+
+def waits_expired(device=None, *, reset=False):
+    """How many CTAs of these kernels have given up waiting for their own copies and products on ``device`` (the current one if not
+    given) since the library was loaded or the count was last ``reset``: 0 unless the GPU is not working properly.  What such a CTA should have
+    written stays as it was, and no call can say so when it returns, since it does not wait for the GPU: a program that wants to know
+    asks here, which does wait.  Not for calls that are being captured."""
+    count = C.c_uint()
+    with torch.cuda.device(device):
+        check(lib.hqkv_prompt_waits_expired(int(bool(reset)), C.byref(count)))
+    return count.value

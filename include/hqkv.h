@@ -532,10 +532,17 @@ int hqkv_prompt_attention(const hqkv_prompt_t* prompt_host, void* out, float* ls
 
 /*
  * The kernels' waits for their own copies, products and roles have a limit (33 seconds; an item of 2^30 keys takes 15).  A CTA in which
- * one runs out ends without a result and is counted here: 0 unless the GPU is not working properly.  (Their waits for tensor memory
- * and for the kernel before them have none.)  Waits for the device's work and (optionally) clears the count.
+ * one runs out ends without a result - what it should have written stays as it was - and is counted here: 0 unless the GPU is not working
+ * properly.  (Their waits for tensor memory and for the kernel before them have none.)  Waits for the device's work and (optionally)
+ * clears the count.
  */
 int hqkv_prompt_waits_expired(int reset, unsigned* count_host);
+
+/*
+ * For tests of that: from now on the waits on the current device give up after so many tries (of up to 4 us each); 0: after as many as
+ * ever.  Bounds-check build only, HQKV_E_UNSUPPORTED in the regular one.
+ */
+int hqkv_prompt_limit_waits(int tries);
 
 /*
  * Rows that seed the importance ring (the probabilities of a prompt's last queries, model/llama_hqe.py:124, 141-166, summed over

@@ -34,3 +34,15 @@ def cuda_device():
     if not torch.cuda.is_available():
         pytest.skip("no CUDA device")
     return torch.device("cuda:0")
+
+
+@pytest.fixture(scope="module", autouse=True)
+def no_wait_has_run_out(request):
+    """After every module of GPU tests of the prompt operators: none of their kernels has given up a wait."""
+    yield
+    if not request.module.__name__.rpartition(".")[2].startswith("test_gpu_prompt"):
+        return
+    import torch
+    if torch.cuda.is_available():
+        from hqekv_b200.prompt import waits_expired
+        assert waits_expired() == 0
