@@ -1359,6 +1359,7 @@ extern "C" int hqkv_prompt_attention(const hqkv_prompt_t* prompt_host, void* out
 extern "C" int hqkv_prompt_waits_expired(int reset, unsigned* count_host) {
   HQKV_REQUIRE(count_host != nullptr, "prompt_waits_expired: null pointer");
   const unsigned zero = 0;
+  HQKV_CUDA(cudaDeviceSynchronize());   // (the copy alone does not wait for streams that do not wait for the default one)
   HQKV_CUDA(cudaMemcpyFromSymbol(count_host, hqkv::g_waits_expired, sizeof(unsigned)));
   if (reset) HQKV_CUDA(cudaMemcpyToSymbol(hqkv::g_waits_expired, &zero, sizeof(unsigned)));
   return HQKV_OK;

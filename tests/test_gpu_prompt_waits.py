@@ -91,3 +91,33 @@ def test_the_regular_build_has_one_limit(cuda_device):
         pytest.skip("the bounds-check build is loaded")
     assert _lib.lib.hqkv_prompt_limit_waits(1) == -2 and "bounds-check build" in _lib.lib.hqkv_last_error().decode()
     assert waits_expired() == 0
+
+
+COUNT = r"""
+import sys
+import torch
+sys.path.insert(0, {root!r})
+from hqekv_b200 import _lib
+from hqekv_b200.prompt import prompt_attention, waits_expired
+q, k = (torch.randn(6000, h, 128, device="cuda").half() for h in (32, 8))
+at = torch.tensor([0, 6000], dtype=torch.int32, device="cuda")
+prompt_attention(q, k, k, at)
+assert waits_expired(reset=True) == 0
+_lib.check(_lib.lib.hqkv_prompt_limit_waits(1))
+with torch.cuda.stream(torch.cuda.Stream()):
+    torch.cuda._sleep(400_000_000)     # a fifth of a second
+    prompt_attention(q, k, k, at)
+n = waits_expired()
+assert n > 0, "read before the call had ended"
+torch.cuda.synchronize()
+assert waits_expired(reset=True) == n
+print("counted", n)
+"""
+
+
+def test_the_count_waits_for_every_stream(cuda_device):
+    """torch's streams do not wait for the default one, nor it for them."""
+    from hqekv_b200 import build
+    env = dict(os.environ, HQKV_LIB=build.build(checks=True))
+    r = subprocess.run([sys.executable, "-c", COUNT.format(root=ROOT)], env=env, capture_output=True, text=True, timeout=600)
+    assert r.returncode == 0 and "counted" in r.stdout, r.stdout[-3000:] + r.stderr[-4000:]
