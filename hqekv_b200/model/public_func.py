@@ -135,8 +135,12 @@ class last_attn_weights:
 
     def seed(self, rows: torch.Tensor):
         """What ``update`` does with the probabilities of a prompt, from their sums over the heads: ``rows`` float16
-        [n, L], the n last queries' (``prompt_importance``)."""
+        [n, L], the last n = min(last_length, Lq) queries' of a prompt of Lq (``prompt_importance``).  ``prompt_importance`` fills up the
+        rows of prompts that have fewer queries than it was asked for; they are not the ring's: of packed prompts hand over
+        ``rows[:min(last_length, Lq), a:b]`` each."""
         n, L = rows.shape
+        if n > L:   # (every query of a sequence is one of its positions)
+            raise ValueError(f"rows holds {n} queries for {L} positions: leave out the rows behind the prompt's last query")
         cap = self.max_length if self.weights is None else self.weights.shape[1]
         if L > cap or n > self.last_length:
             raise ValueError(f"rows holds {n} queries and {L} positions but the ring is sized for {self.last_length} and {cap} "

@@ -128,7 +128,8 @@ def prompt_importance(q, k, lse, seq_starts, kv_starts=None, *, rows=20, causal=
     """Head-summed probabilities of each sequence's last ``rows`` queries -> float16 [rows, Tk].
 
     Row r holds, for every key of a sequence, what the r-th of the sequence's last t = min(rows, Lq) queries gives it, summed over
-    the query heads in fp32 and rounded once; rows r >= t are 0, and so are keys that the query does not see.  ``lse`` [nh_q, Tq] as
+    the query heads in fp32 and rounded once; rows r >= t are 0 (a ring is seeded with the first t), and so are keys that the query
+    does not see.  ``lse`` [nh_q, Tq] as
     ``prompt_attention`` returned it for the same q and keys; only those queries' entries are read.  (With a prefix the rows of a head add up to 1
     minus the prefix's share.)  ``rows``: 1 to 64.  Columns of keys in no sequence are not written: in ``out`` they stay as they were, in
     a result allocated here they are undefined."""
