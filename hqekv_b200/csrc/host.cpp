@@ -266,12 +266,15 @@ PyObject* decode(PyObject*, PyObject* const* a, Py_ssize_t na) {
   END_HANDLE_TH_ERRORS
 }
 
+// whether derivatives are asked of a tensor, by either mode (the operators here have none)
+inline bool differentiated(const at::Tensor& x) { return (x.requires_grad() && c10::GradMode::is_enabled()) || x._fw_grad(0).defined(); }
+
 // a [tokens, heads, 128] operand that the prompt kernels read where it is
 inline bool packed(const at::Tensor& x) {
   if (!x.is_cuda() || x.dim() != 3 || x.size(2) != 128 || x.stride(2) != 1 || reinterpret_cast<uintptr_t>(x.data_ptr()) % 16) return false;
   for (int d = 0; d < 2; ++d)
     if (x.size(d) > 1 && (x.stride(d) <= 0 || x.stride(d) % 8)) return false;
-  return !(x.requires_grad() && c10::GradMode::is_enabled());
+  return !differentiated(x);
 }
 
 // decode_prefix(q, cache, prefix_k, prefix_v, block_size, group_size, low_codec) -> (attn_weights, attn_output) | None
@@ -285,7 +288,7 @@ PyObject* decode_prefix(PyObject*, PyObject* const* a, Py_ssize_t na) {
     if (!packed(*x) || x->scalar_type() != at::kHalf || x->device() != q.device() || x->size(1) != d.H || x->size(2) != d.D ||
         x->size(0) != pk.size(0) || x->size(0) == 0)
       return none();
-  if (!q.is_contiguous() || reinterpret_cast<uintptr_t>(q.data_ptr()) % 16 || (q.requires_grad() && c10::GradMode::is_enabled())) return none();
+  if (!q.is_contiguous() || reinterpret_cast<uintptr_t>(q.data_ptr()) % 16 || differentiated(q)) return none();
   const size_t need = L.decode_workspace_bytes(&d), more = L.decode_prefix_workspace_bytes(&d, pk.size(0));
   if (need == 0 || more == 0) return none();
   const c10::cuda::OptionalCUDAGuard guard(q.device());
@@ -389,7 +392,7 @@ PyObject* prompt_importance(PyObject*, PyObject* const* a, Py_ssize_t na) {
   }
   const at::Tensor& q = THPVariable_Unpack(a[0]);
   if (lse->scalar_type() != at::kFloat || lse->device() != q.device() || lse->dim() != 2 || lse->size(0) != p.nh_q || lse->size(1) != p.total_q ||
-      rows < 1 || rows > HQKV_IMPORTANCE_ROWS)
+      rows < 1 || rows > HQKV_IMPORTANCE_ROWS || differentiated(*lse))
     return none();
   const c10::cuda::OptionalCUDAGuard guard(q.device());
   at::Tensor out = at::empty({rows, p.total_k}, q.options().dtype(at::kHalf));

@@ -12,6 +12,7 @@ the tensors' device) says where each sequence begins and the last one ends.  A p
 import ctypes as C
 
 import torch
+from torch.autograd import forward_ad
 
 from ._lib import Prompt, check, host, lib, ptr, require_cuda, stream_ptr
 
@@ -25,6 +26,17 @@ def usable(x):
     return x.stride(2) == 1 and x.data_ptr() % 16 == 0 and all(x.shape[d] < 2 or (x.stride(d) > 0 and x.stride(d) % 8 == 0) for d in (0, 1))
 
 
+def no_gradient(*tensors):
+    """Refuse what derivatives are asked of (of a dual tensor under no_grad, too: that does not end forward mode)."""
+    for x in tensors:
+        if x is None:
+            continue
+        if x.requires_grad and torch.is_grad_enabled():
+            raise RuntimeError("these operators have no backward pass: call them under torch.no_grad()")
+        if forward_ad.unpack_dual(x).tangent is not None:
+            raise RuntimeError("these operators have no forward derivatives: unpack dual tensors before the call")
+
+
 def _tensor(name, x, like=None, heads=None, tokens=None):
     """A [tokens, heads, 128] operand as the kernels take it: channels adjacent, 16-byte aligned rows (copied where it is not)."""
     if x.dim() != 3 or x.shape[2] != HEAD_DIM:
@@ -35,8 +47,7 @@ def _tensor(name, x, like=None, heads=None, tokens=None):
         raise ValueError(f"{name} must have {heads} heads (got {x.shape[1]})")
     if tokens is not None and x.shape[0] != tokens:
         raise ValueError(f"{name} must have {tokens} tokens (got {x.shape[0]})")
-    if x.requires_grad and torch.is_grad_enabled():
-        raise RuntimeError("the prompt operators have no backward pass: call them under torch.no_grad()")
+    no_gradient(x)
     return x if usable(x) else x.clone(memory_format=torch.contiguous_format)
 
 
@@ -110,6 +121,7 @@ def prompt_attention(q, k, v, seq_starts, kv_starts=None, *, prefix=None, causal
         if done is not None:
             return done
     # what the native path does not take as it is: operands to be copied, and everything that is an error
+    no_gradient(out)
     p, keep = _describe(q, k, v, seq_starts, kv_starts, prefix, causal, scale)
     q = keep[0]
     if out is None:
@@ -139,6 +151,7 @@ def prompt_importance(q, k, lse, seq_starts, kv_starts=None, *, rows=20, causal=
         done = host.prompt_importance(q, k, None, seq_starts, kv_starts, None, None, causal, scale, lse, rows)
         if done is not None:
             return done
+    no_gradient(lse, out)
     p, keep = _describe(q, k, None, seq_starts, kv_starts, None, causal, scale)
     q, k = keep[0], keep[1]
     if lse.shape != (q.shape[1], q.shape[0]) or lse.dtype != torch.float32 or lse.device != q.device:

@@ -8,7 +8,7 @@ from typing import Tuple
 import torch
 
 from .._lib import CODEC_NORMAL, CODEC_UNIFORM, HqkvError, check, decode_workspace, host, lib, ptr, require_cuda, stream_ptr
-from ..prompt import usable
+from ..prompt import no_gradient, usable
 from ._cache import UNIFORM_STRATEGIES, cached_cache_desc
 
 
@@ -97,8 +97,7 @@ def qkv_matmul_hqe_prefix(q: torch.Tensor, past_key_value: Tuple, prefix: Tuple[
         return done
     if q.dtype != torch.float16 or q.dim() != 4 or q.shape[2] != 1:
         raise ValueError("q must be float16 of shape [B, nh_q, 1, head_dim]")
-    if torch.is_grad_enabled() and (q.requires_grad or pk.requires_grad or pv.requires_grad):
-        raise RuntimeError("the decode has no backward pass: call it under torch.no_grad()")
+    no_gradient(q, pk, pv)
     desc, keep, L, dev = cached_cache_desc(past_key_value, q.shape[1], block_size, group_size, low_codec)
     if dev != q.device or q.shape[0] != desc.B or q.shape[3] != desc.D:
         raise ValueError("q does not match the cache (device, batch or head_dim)")
