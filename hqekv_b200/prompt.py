@@ -77,7 +77,7 @@ def _describe(q, k, v, seq_starts, kv_starts, prefix, causal, scale):
         kv_starts = seq_starts
     else:
         kv_starts = _starts("kv_starts", kv_starts, q.device, seq_starts.numel())
-    scale = HEAD_DIM ** -0.5 if scale is None else float(scale)
+    scale = C.c_float(HEAD_DIM ** -0.5 if scale is None else scale).value   # as the kernels take it
     if not 0.0 < scale < 1e38:
         raise ValueError("scale must be positive, and below 1e38")
     p = Prompt()

@@ -52,3 +52,18 @@ def test_no_derivatives_by_either_mode(i):
             with mode(), pytest.raises(RuntimeError, match="no forward derivatives"):
                 call(x)
     assert len(calls) == 13
+
+
+@pytest.mark.parametrize("scale", [1e-46, 1e-300, 1e39, float("nan")])
+def test_scales_outside_of_float32(scale):
+    """What is 0 or infinite as the kernels take it is refused like a 0 or an infinity."""
+    from hqekv_b200.prompt import prompt_attention, prompt_importance
+    x, _ = operands()
+    at = torch.tensor([0, 5], dtype=torch.int32)
+    with pytest.raises(ValueError, match="scale"):
+        prompt_attention(x["q"], x["k"], x["v"], at, scale=scale)
+    with pytest.raises(ValueError, match="scale"):
+        prompt_importance(x["q"], x["k"], x["lse"], at, scale=scale)
+    for small in (1e-40, 2.0 ** -149):
+        with pytest.raises(RuntimeError, match="CUDA tensors only"):
+            prompt_attention(x["q"], x["k"], x["v"], at, scale=small)
