@@ -161,7 +161,8 @@ class HqeAttention(nn.Module):
         self.schedule = TierSchedule(bit_0, bit_4, bit_2, bit_1)
         self.last_weights = last_attn_weights(last_length=SEED_QUERIES)
         self.fused_prompt = fused_prompt
-        self.prefix = None
+        for name in ("prefix_k", "prefix_v"):   # (buffers: they go where the module goes, but into no checkpoint)
+            self.register_buffer(name, None, persistent=False)
 
     # -- per-sequence state ---------------------------------------------------------------------
     def reset(self):
@@ -179,7 +180,11 @@ class HqeAttention(nn.Module):
         for x in (k, v):
             if x is not None and (x.dim() != 3 or x.shape[0] == 0 or x.shape != k.shape or tuple(x.shape[1:]) != (self.num_kv_heads, self.head_dim)):
                 raise ValueError(f"a prefix must be [P, {self.num_kv_heads}, {self.head_dim}] with at least one token")
-        self.prefix = None if k is None else (k, v)
+        self.prefix_k, self.prefix_v = k, v
+
+    @property
+    def prefix(self):
+        return None if self.prefix_k is None else (self.prefix_k, self.prefix_v)
 
     @property
     def current_length(self):
