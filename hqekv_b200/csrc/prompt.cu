@@ -45,9 +45,11 @@ __device__ __forceinline__ int start_of(const int* starts, int s, int total) { r
 // softmax.  32 heads, us and TFLOP/s a call: 8 k tokens 415 and 1325, all of them seen 785 and 1400, 4 x 4 k 442 and 1245, 8 x 1000 85 and
 // 770.  In a long run the power limit decides: 32 k tokens 7.3 ms, 1205 TFLOP/s at 1410 MHz and 990 W (a library product of 8192^3
 // under the same limit 1409).
-//   Why 256 rows: K and V of a tile are 64 KB from L2 for every CTA, 2.6 KB a cycle for all of them at this rate; with 128 rows it would be twice
-// that.  Why heads of a group side by side: a block of four heads is 64 tokens long, so its last tiles are half as empty and its row
-// tiles as long as each other, and eight tokens of 32 heads fill it.
+//   Why 256 rows: K and V of a tile are 64 KB from L2 for every CTA, 3.2 KB a cycle for all of them at this rate (3.7 with Q and what is read
+// twice); with 128 rows it would be twice that.  Why heads of a group side by side: a block of four heads is 64 tokens long, so its
+// last tiles are half as empty and its row tiles as long as each other, and eight tokens of 32 heads fill it.
+//   P is rounded to V's type because it is the second product's left operand, which has to have the type of the right one; the sum that
+// divides is taken before that, in fp32.
 constexpr int TILE = 128;                                // keys per tile, rows per row tile
 constexpr int TILE_BYTES = TILE * 128 * 2;               // 64 channels of all its tokens, then the other 64
 constexpr int KV_STAGES = 5;
@@ -114,8 +116,10 @@ __device__ __forceinline__ bool is_longer(const PromptArgs& A, int i0, int lq) {
 }
 // Tiles per share, for a warp that holds a sequence per lane (none: lq = 0): the fewest that make an item for every CTA at most, or
 // two where that is faster - an item takes as long as its tiles and some three more.  Every lane tries another size.  us with one
-// size chosen from the average length for three items per CTA, and with this (queries and keys up to, 32 heads over 8): 4 x 96, 16 k
-// 74.4 and 67.5; 8 heads over 2: 5 x 81, 43 k 68.0 and 49.1, 30 x 60, 3 k 51 and 32, 12 x 243, 11 k 96 and 84.
+// size chosen from the average length for three items per CTA, and with this, in graphs of repeated calls whose K and V the L2 holds
+// in part (queries and keys up to, 32 heads over 8): 4 x 96, 16 k 73.4 and 67.3; 8 heads over 2: 5 x 81, 43 k 65.1 and 48.7, 30 x 60,
+// 3 k 51 and 32, 12 x 243, 11 k 100 and 75.  Where one item per CTA leaves each a single short one it loses a little: 6 x 31, 11 k, 8 heads over 8
+// 41.6 and 43.9, 8 x 50, 31 k, 8 over 2 47.4 and 48.3.
 __device__ __forceinline__ int share_size(const PromptArgs& A, int lq, int lk) {
   constexpr unsigned all = 0xffffffffu;
   const int lane = threadIdx.x & 31, round = PROMPT_CTAS / A.groups;   // blocks of a head group that CTAs are there for
@@ -123,8 +127,10 @@ __device__ __forceinline__ int share_size(const PromptArgs& A, int lq, int lk) {
   const int shorter = blocks > 0 && is_longer(A, (blocks - 1) << A.block_shift, lq) ? 1 : 0, whole = blocks - shorter;
   const int least = max(SHARE_TILES, __reduce_max_sync(all, (tiles + A.shares - 1) / A.shares));   // (there is room for A.shares)
   const int most = max(least, __reduce_max_sync(all, tiles)), n = __reduce_add_sync(all, blocks);
-  // Between work / per and work / per + n items.  (Quotients in fp32 are exact enough for 2^21 tiles; what depends on them is the number
-  // of items alone.)
+  // Between work / per and work / (per - 1/3) + n items: a block of one row tile counts as two thirds of one of two, but longer(per) may be
+  // 1/2 short of 3/2 per.  So work / (round - n) + 1/3 tiles are enough for one round at most; `high` adds 2 to the truncated quotient
+  // for that third and for the quotient's own error (fp32: below 2/3 up to a million tiles, and only the number of items hangs on it: the
+  // grid has two rounds).
   const float work = static_cast<float>(__reduce_add_sync(all, static_cast<unsigned>(3 * whole + 2 * shorter) * tiles)) * (1.f / 3.f);
   const int low = max(least, static_cast<int>(__fdividef(work, static_cast<float>(2 * round))));
   const int high = max(low, n < round ? min(most, static_cast<int>(__fdividef(work, static_cast<float>(round - n))) + 2) : most);
