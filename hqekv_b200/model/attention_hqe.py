@@ -264,7 +264,6 @@ class HqeAttention(nn.Module):
         attn_weights, past_key_value, auxiliary_parameters)."""
         B, _, S, _ = q.shape
         kv_seq_len = S
-        self.schedule.append(S)
         if past_key_value is not None:
             kv_seq_len += past_key_value[-1]
             new_k = k if past_key_value[-3] is None else torch.cat((past_key_value[-3], k), dim=2)
@@ -293,6 +292,7 @@ class HqeAttention(nn.Module):
             self.last_weights.seed(rows)
         else:
             self.last_weights.update(attn_weights)
+        self.schedule.append(S)   # (behind everything that refuses a call)
         if self.schedule.due():
             past_key_value, auxiliary_parameters = self._flush(past_key_value, auxiliary_parameters)
         else:

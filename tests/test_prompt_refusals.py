@@ -67,3 +67,16 @@ def test_scales_outside_of_float32(scale):
     for small in (1e-40, 2.0 ** -149):
         with pytest.raises(RuntimeError, match="CUDA tensors only"):
             prompt_attention(x["q"], x["k"], x["v"], at, scale=small)
+
+
+def test_a_refused_prefill_leaves_the_layer_as_it_was():
+    """No tokens are counted that were not taken: a mask, a prompt that needs a gradient, a type that is not served."""
+    from hqekv_b200.model.attention_hqe import HqeAttention
+    layer = HqeAttention(64, 2, 1, fused_prompt=True)
+    layer.set_max_length(64)
+    q, k = torch.zeros(1, 2, 40, 128).half(), torch.zeros(1, 1, 40, 128).half()
+    for args, error in (((q, k, k, torch.zeros(1, 1, 40, 40)), ValueError), ((q.clone().requires_grad_(), k, k), RuntimeError),
+                        ((q.float(), k.float(), k.float()), ValueError), ((q, k, k), RuntimeError)):
+        with pytest.raises(error):
+            layer.attend(*args)
+        assert (layer.current_length, layer.history_reserve_length, layer.last_weights.next_line) == (0, 0, 0)
