@@ -6,7 +6,8 @@ which seed the importance ring (:124, 141-166; model/public_func.py:247-252).  B
 (hqekv_b200/csrc/prompt.cu).  They have no backward pass, like every operator of this package, and refuse inputs that need one.
 
 Layout: tokens x heads x channels, the tokens of all sequences one behind another.  ``seq_starts`` (int32 or int64, ``n + 1`` entries on
-the tensors' device) says where each sequence begins and the last one ends.  A padded batch ``[B, heads, S, 128]`` is packed as
+the tensors' device) says where each sequence begins and the last one ends.  They do not decrease; what lies outside of the tokens is taken
+as the nearest end of them.  A padded batch ``[B, heads, S, 128]`` is packed as
 ``x.transpose(1, 2).reshape(B * S, heads, 128)`` with starts ``0, S, 2 S, ...`` - a view where the batch is stored token by token.
 """
 import ctypes as C
@@ -56,6 +57,8 @@ def _starts(name, x, device, n=None):
         raise ValueError(f"{name} must be a 1-D int32 or int64 tensor on the device of q")
     if n is not None and x.numel() != n:
         raise ValueError(f"{name} must have {n} entries like seq_starts (got {x.numel()})")
+    if x.dtype == torch.int64:   # (starts out of range are taken as the nearest, also those that int32 does not hold)
+        x = x.clamp(-1, 2 ** 31 - 1)
     return x.to(torch.int32).contiguous()
 
 
